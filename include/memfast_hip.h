@@ -548,6 +548,69 @@ int mf_rng_uniform(const uint64_t *address, int64_t count, uint64_t seed, uint32
 int mf_rng_normal(const uint64_t *address, int64_t count, uint64_t seed, uint32_t stream,
                   float *out, void *stream_handle);
 
+/* ---- 4-bit microscaled operands (microscaling.hip) ------------------------ */
+/* Element types of the operands below. */
+enum { MF_F32 = 0, MF_BF16 = 1, MF_F16 = 2 };
+
+/* Blocks of 32 consecutive values of a row share a power-of-two scale 2^e with
+ * e = max(floor(log2 max|x|) - 2, -126), held as the byte e + 127 (255: the block holds a NaN or an
+ * infinity and stands for NaN).  A value's code is x / 2^e rounded to nearest even on
+ * {0, 0.5, 1, 1.5, 2, 3, 4, 6}, saturating at 6, with the sign in bit 3.  With S = ceil(k / 256), codes
+ * are [n, 128 * S] bytes (the even value in the lower half of a byte) and scales [n, 8 * S]; codes past
+ * k are 0.  codes 16-byte, scales 8-byte aligned.
+ *
+ * x: [n, k], rows ldx values apart. */
+int mf_mx_quantize(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, uint8_t *codes,
+                   uint8_t *scales, void *stream);
+/* out [n, k]: code * scale, rounded to the output's type. */
+int mf_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, void *out,
+                     int32_t type, void *stream);
+/* out [n, o] = Q(x) W^T + bias (bias: o values of x's type, or NULL), FP32 sums; W [o, k] in codes.
+ * xcodes and xscales receive Q(x). */
+int mf_mx_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx,
+                 const uint8_t *wcodes, const uint8_t *wscales, int64_t o, const void *bias,
+                 uint8_t *xcodes, uint8_t *xscales, void *out, void *stream);
+/* Gradients of mf_mx_linear straight through the quantizers, for dy [n, o] (rows ldy apart), FP32
+ * sums: dx [n, k] = dy Q(W), dw [o, k] = dy^T Q(x), db [o] = column sums of dy.  They share a workspace
+ * of mf_mx_grad_workspace bytes (16-byte aligned), one after the other on one stream. */
+int mf_mx_grad_workspace(int32_t type, int64_t n, int64_t o, int64_t *bytes);
+int mf_mx_grad_input(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
+                     const uint8_t *wcodes, const uint8_t *wscales, int64_t k, void *dx,
+                     void *workspace, int64_t bytes, void *stream);
+int mf_mx_grad_weight(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
+                      const uint8_t *xcodes, const uint8_t *xscales, int64_t k, void *dw,
+                      void *workspace, int64_t bytes, void *stream);
+int mf_mx_grad_bias(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy, void *db,
+                    void *workspace, int64_t bytes, void *stream);
+
+/* ---- distillation from a teacher's top logits (distillation.hip) ---------- */
+/* The k largest of each row of logits [n, v] (rows ld apart), in descending order, the lowest index
+ * first among equal ones (NaN counts as the largest, -0 as 0): values [n, k] of the logits' type, indices
+ * [n, k], and tail [n] = log(sum(exp(logits / temperature))) of the row's other logits (-inf where
+ * there is none).  k <= 1024, v <= 2^20. */
+int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld, int64_t k,
+                  float temperature, void *values, int64_t *indices, float *tail, void *stream);
+
+enum { MF_SUM_NONE = 0, MF_SUM_SUM = 1, MF_SUM_MEAN = 2 };
+/* The loss of student logits [n, v] against a teacher's entries: values and indices [n, k] (an index
+ * of -1: no entry) and tail [n] (NULL: no mass outside the entries).
+ *   p = softmax([values / T, tail]), q = softmax(logits / T), both over the entries and one bucket
+ *   for all other classes;  row_loss = T^2 sum p log(p / q).
+ * A row with an index outside -1 .. v - 1 or a repeated one has a NaN loss and gradient; a row without
+ * any entry or tail, and one whose weight is 0 (whatever its logits), has neither.  Unless reduction
+ * is MF_SUM_NONE, *loss = sum(weight * row_loss) (MF_SUM_MEAN: over sum(weight), 0 if that is 0).
+ * ref [n], coef [n], entry_grad [n, k] and *norm are what mf_distill_grad needs. */
+int mf_distill_loss(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld,
+                    const void *values, int32_t values_type, const int64_t *indices,
+                    const float *tail, int64_t k, float temperature, const float *weight,
+                    int32_t reduction, float *row_loss, float *ref, float *coef, float *entry_grad, float *loss, float *norm,
+                    void *stream);
+/* grad [n, v] of the logits: weight * norm * incoming[r * incoming_step] times the row loss's. */
+int mf_distill_grad(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld,
+                    const int64_t *indices, int64_t k, float temperature, const float *weight,
+                    const float *ref, const float *coef, const float *entry_grad, const float *norm,
+                    const float *incoming, int64_t incoming_step, void *grad, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,140 @@
+"""Distillation of a student from a teacher's top logits.
+
+A network converted to analog layers (``convert_model(..., training=True)``) is tuned against
+its digital original.  The original's whole output need not be kept: ``top_logits`` gives its k
+largest logits per row and the logarithm of the mass of all others, and ``distillation_loss``
+the student's loss against them, with its gradient.
+
+Both run in one pass over the logits each way, hold their sums in FP32 and read nothing back
+to the host; a row whose indices are wrong has a NaN loss.
+"""
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import hip
+from .microscaling import _check_floating
+
+MOST_ENTRIES, MOST_CLASSES = 1024, 1 << 20
+
+
+def _check_temperature(temperature):
+    if isinstance(temperature, bool) or not isinstance(temperature, (int, float)):
+        raise TypeError("temperature must be a number")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError("temperature must be positive and finite")
+    return float(temperature)
+
+
+def _check_logits(logits):
+    _check_floating("logits", logits)
+    if logits.ndim == 0 or logits.shape[-1] == 0:
+        raise ValueError("logits must have at least one class in their last dimension")
+    if logits.shape[-1] > MOST_CLASSES:
+        raise NotImplementedError(f"more than {MOST_CLASSES} classes")
+
+
+def top_logits(logits, k, *, temperature=1.0):
+    """(values, indices, tail) of ``logits`` [..., V]: the ``k`` largest in descending order
+    [..., k], the lowest index first among equal ones (NaN counts as the largest), their indices
+    (int64), and ``log(sum(exp(logits / temperature)))`` of the others [...] in FP32 (-inf where
+    none is left).  No gradient flows through them."""
+    _check_logits(logits)
+    temperature = _check_temperature(temperature)
+    if isinstance(k, bool) or not isinstance(k, int):
+        raise TypeError("k must be an integer")
+    if not 1 <= k <= logits.shape[-1]:
+        raise ValueError("k must be between 1 and the number of classes")
+    if k > MOST_ENTRIES:
+        raise NotImplementedError(f"more than {MOST_ENTRIES} entries")
+    hip.require_device(logits)
+    lead = logits.shape[:-1]
+    rows = logits.detach()
+    rows = hip.rows_of(rows) if rows.numel() else rows.reshape(0, rows.shape[-1])
+    values, indices, tail = hip.top_logits(rows, k, temperature)
+    return values.reshape(lead + (k,)), indices.reshape(lead + (k,)), tail.reshape(lead)
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, indices, tail, weight, temperature, reduction):
+        row_loss, total, kept = hip.distill_loss(logits, values, indices, tail, temperature, weight,
+                                                 reduction)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, indices, weight, *kept)
+            ctx.temperature = temperature
+        if reduction != "none":
+            return total
+        return row_loss if weight is None else torch.where(weight == 0, 0.0, weight * row_loss)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, incoming):
+        logits, indices, weight, *kept = ctx.saved_tensors
+        grad = hip.distill_grad(logits, indices, ctx.temperature, weight, kept,
+                                incoming.to(torch.float32).contiguous())
+        return (grad,) + (None,) * 6
+
+
+def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, weight=None,
+                      reduction="mean"):
+    """Loss of the student's ``logits`` [..., V] against a teacher's top logits.
+
+    ``values`` and ``indices`` [..., k] are the teacher's logits and their classes, ``tail`` [...]
+    the logarithm of its other classes' sum at ``temperature`` (``top_logits`` gives all three).
+    An index of -1 marks an entry that is absent.  With ``p = softmax([values / T, tail])`` and ``q``
+    the student's ``softmax(logits / T)`` over the same entries and one bucket for all other
+    classes, a row's loss is ``T**2 * sum(p * log(p / q))``; without ``tail`` the teacher's bucket is
+    empty.  A row without any entry or tail has no loss.  A row with an index outside -1 .. V - 1
+    or with a repeated one has a NaN loss.
+
+    ``weight`` [...] weighs the rows (bool or floating; a row of weight 0 is not read).
+    ``reduction``: "mean" (over the weights' sum; 0 if that is 0), "sum" or "none".  The loss is FP32;
+    gradients reach ``logits`` alone."""
+    _check_logits(logits)
+    _check_floating("values", values)
+    temperature = _check_temperature(temperature)
+    if reduction not in hip.REDUCTIONS:
+        raise ValueError("reduction must be mean, sum or none")
+    if not isinstance(indices, torch.Tensor) or indices.dtype not in (torch.int64, torch.int32):
+        raise TypeError("indices must be an int64 or int32 tensor")
+    lead = logits.shape[:-1]
+    if values.ndim != logits.ndim or values.shape[:-1] != lead or values.shape[-1] == 0:
+        raise ValueError("values must have the rows of logits and at least one entry")
+    if indices.shape != values.shape:
+        raise ValueError("values and indices must have the same shape")
+    k = values.shape[-1]
+    if k > logits.shape[-1]:
+        raise ValueError("more entries than classes")
+    if k > MOST_ENTRIES:
+        raise NotImplementedError(f"more than {MOST_ENTRIES} entries")
+    for label, value in (("tail", tail), ("weight", weight)):
+        if value is None:
+            continue
+        if not isinstance(value, torch.Tensor) or not (
+                value.is_floating_point() or label == "weight" and value.dtype == torch.bool):
+            raise TypeError(f"{label} must be a floating tensor")
+        if value.shape != lead:
+            raise ValueError(f"{label} must have one value per row")
+    for label, value in (("values", values), ("indices", indices), ("tail", tail),
+                         ("weight", weight)):
+        if value is not None and value.device != logits.device:
+            raise ValueError(f"logits and {label} must use the same device")
+    hip.require_device(logits)
+    if logits.numel() == 0:
+        zero = logits.sum(-1).float()
+        return zero if reduction == "none" else zero.sum()
+
+    def per_row(value):
+        return None if value is None else value.detach().to(torch.float32).reshape(-1).contiguous()
+
+    entries = values.detach().reshape(-1, k).contiguous()
+    loss = _Distillation.apply(hip.rows_of(logits), entries,
+                               indices.to(torch.int64).reshape(-1, k).contiguous(), per_row(tail),
+                               per_row(weight), temperature, reduction)
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+__all__ = ["top_logits", "distillation_loss"]

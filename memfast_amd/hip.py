@@ -200,6 +200,18 @@ SIGNATURES = {
     "mf_resources_query": ([_CFG, _I32, _I64, _I32, ct.POINTER(MFResources)], ct.c_int),
     "mf_resources_shape": ([_CFG, _I32, _I64, _I64, _I64, _I32, ct.POINTER(MFResources)],
                            ct.c_int),
+    "mf_mx_quantize": ([_P, _I32, _I64, _I64, _I64, _P, _P, _P], ct.c_int),
+    "mf_mx_dequantize": ([_P, _P, _I64, _I64, _P, _I32, _P], ct.c_int),
+    "mf_mx_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _P], ct.c_int),
+    "mf_mx_grad_workspace": ([_I32, _I64, _I64, ct.POINTER(_I64)], ct.c_int),
+    "mf_mx_grad_input": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P], ct.c_int),
+    "mf_mx_grad_weight": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P], ct.c_int),
+    "mf_mx_grad_bias": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P], ct.c_int),
+    "mf_top_logits": ([_P, _I32, _I64, _I64, _I64, _I64, ct.c_float, _P, _P, _P, _P], ct.c_int),
+    "mf_distill_loss": ([_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, ct.c_float, _P, _I32,
+                         _P, _P, _P, _P, _P, _P, _P], ct.c_int),
+    "mf_distill_grad": ([_P, _I32, _I64, _I64, _I64, _P, _I64, ct.c_float, _P, _P, _P, _P, _P, _P,
+                         _I64, _P, _P], ct.c_int),
     "mf_rng_uniform": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
     "mf_rng_normal": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
 }
@@ -1411,3 +1423,164 @@ __all__ = [
     "ResourceError", "BackendError", "cache_root", "atomic_write", "partial", "program",
     "identity", "mm", "restore", "input_tiles", "weight_tiles", "transpose_packed",
 ]
+
+
+# ---------------------------------------------------------------------------
+# 4-bit microscaled operands
+# ---------------------------------------------------------------------------
+FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MF_F32, MF_BF16, MF_F16
+MX_SEGMENT, MX_SEGMENT_BYTES, MX_SEGMENT_SCALES = 256, 128, 8
+
+
+def rows_of(x):
+    """``x`` [..., k] as a matrix whose rows are contiguous (a view where it has such a layout)."""
+    flat = x.reshape(-1, x.shape[-1])
+    if flat.stride(1) != 1 and flat.shape[1] > 1 or flat.stride(0) < flat.shape[1]:
+        flat = flat.contiguous()
+    return flat
+
+
+def mx_empty(n, k, device):
+    """Uninitialised codes and scales of ``n`` rows of ``k`` values."""
+    segments = -(-k // MX_SEGMENT)
+    return (torch.empty((n, MX_SEGMENT_BYTES * segments), dtype=torch.uint8, device=device),
+            torch.empty((n, MX_SEGMENT_SCALES * segments), dtype=torch.uint8, device=device))
+
+
+def mx_quantize(x):
+    """Codes and scales of the rows of ``x`` [n, k] (mf_mx_quantize)."""
+    require_device(x)
+    n, k = x.shape
+    codes, scales = mx_empty(n, k, x.device)
+    if codes.numel():
+        with _on(x.device):
+            check(library().mf_mx_quantize(_ptr(x), FLOAT_TYPES[x.dtype], n, k, x.stride(0),
+                                           _ptr(codes), _ptr(scales), _stream(x.device)),
+                  "microscaled quantization")
+    return codes, scales
+
+
+def mx_dequantize(codes, scales, k, dtype):
+    """The values [n, k] of codes and scales (mf_mx_dequantize)."""
+    require_device(codes)
+    n = codes.shape[0]
+    out = torch.empty((n, k), dtype=dtype, device=codes.device)
+    if out.numel():
+        with _on(codes.device):
+            check(library().mf_mx_dequantize(_ptr(codes), _ptr(scales), n, k, _ptr(out),
+                                             FLOAT_TYPES[dtype], _stream(codes.device)),
+                  "microscaled dequantization")
+    return out
+
+
+def mx_linear(x, codes, scales, bias):
+    """``Q(x) W^T + bias`` [n, o] (mf_mx_linear) and Q(x)'s codes and scales."""
+    require_device(x)
+    n, k = x.shape
+    o = codes.shape[0]
+    xcodes, xscales = mx_empty(n, k, x.device)
+    out = torch.empty((n, o), dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        check(library().mf_mx_linear(_ptr(x), FLOAT_TYPES[x.dtype], n, k, x.stride(0), _ptr(codes),
+                                     _ptr(scales), o, _ptr(bias), _ptr(xcodes), _ptr(xscales),
+                                     _ptr(out), _stream(x.device)), "microscaled product")
+    return out, xcodes, xscales
+
+
+def mx_grad_workspace(dy):
+    """The workspace that the gradients of ``dy`` [n, o] share."""
+    size = _I64()
+    check(library().mf_mx_grad_workspace(FLOAT_TYPES[dy.dtype], dy.shape[0], dy.shape[1],
+                                         ct.byref(size)), "microscaled gradient workspace")
+    return torch.empty(size.value, dtype=torch.uint8, device=dy.device)
+
+
+def mx_grad_input(dy, codes, scales, k, workspace):
+    """``dy Q(W)`` [n, k] (mf_mx_grad_input)."""
+    n, o = dy.shape
+    dx = torch.empty((n, k), dtype=dy.dtype, device=dy.device)
+    with _on(dy.device):
+        check(library().mf_mx_grad_input(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0),
+                                         _ptr(codes), _ptr(scales), k, _ptr(dx), _ptr(workspace),
+                                         workspace.numel(), _stream(dy.device)),
+              "microscaled input gradient")
+    return dx
+
+
+def mx_grad_weight(dy, xcodes, xscales, k, workspace):
+    """``dy^T Q(x)`` [o, k] (mf_mx_grad_weight)."""
+    n, o = dy.shape
+    dw = torch.empty((o, k), dtype=dy.dtype, device=dy.device)
+    with _on(dy.device):
+        check(library().mf_mx_grad_weight(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0),
+                                          _ptr(xcodes), _ptr(xscales), k, _ptr(dw), _ptr(workspace),
+                                          workspace.numel(), _stream(dy.device)),
+              "microscaled weight gradient")
+    return dw
+
+
+def mx_grad_bias(dy, workspace):
+    """Column sums of ``dy`` [n, o] (mf_mx_grad_bias)."""
+    n, o = dy.shape
+    db = torch.empty(o, dtype=dy.dtype, device=dy.device)
+    with _on(dy.device):
+        check(library().mf_mx_grad_bias(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0), _ptr(db),
+                                        _ptr(workspace), workspace.numel(), _stream(dy.device)),
+              "microscaled bias gradient")
+    return db
+
+
+# ---------------------------------------------------------------------------
+# Distillation
+# ---------------------------------------------------------------------------
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def top_logits(logits, k, temperature):
+    """The ``k`` largest of the rows of ``logits`` [n, v], their indices and the logarithm of the
+    others' sum (mf_top_logits)."""
+    require_device(logits)
+    n, v = logits.shape
+    values = torch.empty((n, k), dtype=logits.dtype, device=logits.device)
+    indices = torch.empty((n, k), dtype=torch.int64, device=logits.device)
+    tail = torch.empty(n, dtype=torch.float32, device=logits.device)
+    if n:
+        with _on(logits.device):
+            check(library().mf_top_logits(_ptr(logits), FLOAT_TYPES[logits.dtype], n, v,
+                                          logits.stride(0), k, temperature, _ptr(values),
+                                          _ptr(indices), _ptr(tail), _stream(logits.device)),
+                  "top logits")
+    return values, indices, tail
+
+
+def distill_loss(logits, values, indices, tail, temperature, weight, reduction):
+    """Row losses [n], their sum or mean [] (None for "none"), and what ``distill_grad`` needs
+    (mf_distill_loss)."""
+    require_device(logits)
+    n, v = logits.shape
+    k = indices.shape[1]
+    stats = torch.empty(n * (3 + k) + 2, dtype=torch.float32, device=logits.device)
+    row_loss, ref, coef, entry_grad, total, norm = stats.split((n, n, n, n * k, 1, 1))
+    with _on(logits.device):
+        check(library().mf_distill_loss(
+            _ptr(logits), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), _ptr(values),
+            FLOAT_TYPES[values.dtype], _ptr(indices), _ptr(tail), k, temperature, _ptr(weight), REDUCTIONS[reduction],
+            _ptr(row_loss), _ptr(ref), _ptr(coef), _ptr(entry_grad), _ptr(total), _ptr(norm),
+            _stream(logits.device)), "distillation loss")
+    none = reduction == "none"
+    return row_loss, None if none else total.reshape(()), (ref, coef, entry_grad,
+                                                           None if none else norm)
+
+
+def distill_grad(logits, indices, temperature, weight, kept, incoming):
+    """The gradient [n, v] of ``distill_loss`` for the incoming gradient: one value, or one a row."""
+    n, v = logits.shape
+    ref, coef, entry_grad, norm = kept
+    grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+    with _on(logits.device):
+        check(library().mf_distill_grad(
+            _ptr(logits), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), _ptr(indices),
+            indices.shape[1], temperature, _ptr(weight), _ptr(ref), _ptr(coef), _ptr(entry_grad),
+            _ptr(norm), _ptr(incoming), int(incoming.numel() > 1), _ptr(grad),
+            _stream(logits.device)), "distillation gradient")
+    return grad

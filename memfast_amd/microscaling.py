@@ -1,0 +1,157 @@
+"""4-bit microscaled floating point: quantized tensors and their linear product.
+
+The digital number format that an analog layer is compared with, and that the layers which
+stay digital (a classifier head, a distillation teacher) are held in.  Blocks of 32
+consecutive values along the last dimension share a power-of-two scale 2**e with
+``e = max(floor(log2(max|x|)) - 2, -126)``; a value's code is ``x / 2**e`` rounded to nearest even
+on {0, 0.5, 1, 1.5, 2, 3, 4, 6} with a sign, saturating at 6.  A block that holds a NaN or an
+infinity stands for NaN.
+
+``mx_quantize`` makes an ``MXTensor`` of codes and scales, ``mx_linear`` multiplies two such
+operands on the matrix cores with FP32 sums.  Its backward passes gradients straight through
+both quantizers: ``dx = dy Q(W)``, ``dw = dy^T Q(x)``, as the surrogate of the hardware-aware layers
+does (memfast_amd/nn/training.py).  Nothing is read back to the host, so a non-finite operand
+shows as NaN in the result and raises nothing.
+"""
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import hip
+
+
+def _check_floating(label, value):
+    if not isinstance(value, torch.Tensor):
+        raise TypeError(f"{label} must be a torch.Tensor")
+    if value.layout != torch.strided or value.dtype not in hip.FLOAT_TYPES:
+        raise TypeError(f"{label} must be a dense float32, bfloat16 or float16 tensor")
+
+
+class MXTensor:
+    """Codes and scales of a 4-bit tensor of ``shape``, whose last dimension k is blocked.
+
+    ``codes`` is uint8 [rows, 128 * S] with S = ceil(k / 256), two codes a byte, the even value in
+    the lower half, codes past k zero; ``scales`` is uint8 [rows, 8 * S], e + 127 of each block (255:
+    NaN).  rows is the product of the other dimensions."""
+
+    def __init__(self, codes, scales, shape):
+        shape = torch.Size(shape)
+        if not shape:
+            raise ValueError("an MXTensor has at least one dimension")
+        rows, segments = math.prod(shape[:-1]), -(-shape[-1] // hip.MX_SEGMENT)
+        for label, value, width in (("codes", codes, hip.MX_SEGMENT_BYTES * segments),
+                                    ("scales", scales, hip.MX_SEGMENT_SCALES * segments)):
+            if not isinstance(value, torch.Tensor) or value.dtype != torch.uint8:
+                raise TypeError(f"{label} must be a uint8 tensor")
+            if value.shape != (rows, width):
+                raise ValueError(f"{label} must have shape {(rows, width)}")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales must use the same device")
+        self.codes, self.scales = (_aligned(v) for v in (codes, scales))
+        self.shape = shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.float32):
+        """The values that the codes stand for, rounded to ``dtype``."""
+        if dtype not in hip.FLOAT_TYPES:
+            raise TypeError("dtype must be float32, bfloat16 or float16")
+        return hip.mx_dequantize(self.codes, self.scales, self.shape[-1], dtype).reshape(self.shape)
+
+    def __repr__(self):
+        return f"MXTensor(shape={tuple(self.shape)}, device={self.device})"
+
+
+def _aligned(value):
+    """``value`` contiguous at a 16-byte address, as the kernels load it."""
+    value = value.contiguous()
+    return value if value.data_ptr() % 16 == 0 else value.clone()
+
+
+def mx_quantize(x):
+    """``x`` (float32, bfloat16 or float16, blocked along its last dimension) as an MXTensor."""
+    _check_floating("x", x)
+    if x.ndim == 0:
+        raise ValueError("x must have at least one dimension")
+    hip.require_device(x)
+    if x.numel() == 0:
+        codes, scales = hip.mx_empty(math.prod(x.shape[:-1]), x.shape[-1], x.device)
+        return MXTensor(codes, scales, x.shape)
+    codes, scales = hip.mx_quantize(hip.rows_of(x.detach()))
+    return MXTensor(codes, scales, x.shape)
+
+
+class _MXLinear(torch.autograd.Function):
+    """Product of Q(x) and a quantized weight.  ``weight`` is the tensor that ``codes`` and
+    ``scales`` were made of, or None for a weight that is held in codes alone."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, codes, scales):
+        y, xcodes, xscales = hip.mx_linear(x, codes, scales, bias)
+        keep = ctx.needs_input_grad
+        ctx.width = x.shape[1]
+        ctx.save_for_backward(*((codes, scales) if keep[0] else (None, None)),
+                              *((xcodes, xscales) if keep[1] else (None, None)))
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scales, xcodes, xscales = ctx.saved_tensors
+        dy = hip.rows_of(dy)
+        work = hip.mx_grad_workspace(dy)
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            dx = hip.mx_grad_input(dy, codes, scales, ctx.width, work)
+        if ctx.needs_input_grad[1]:
+            dw = hip.mx_grad_weight(dy, xcodes, xscales, ctx.width, work)
+        if ctx.needs_input_grad[2]:
+            db = hip.mx_grad_bias(dy, work)
+        return dx, dw, db, None, None
+
+
+def mx_linear(x, weight, bias=None):
+    """``Q(x) Q(weight)^T + bias`` for ``x`` [..., k] and ``weight`` [o, k], in x's dtype.
+
+    ``weight`` is an MXTensor, or a tensor of x's dtype that is quantized in the call and gets a
+    gradient.  ``bias`` [o] has x's dtype."""
+    _check_floating("x", x)
+    held = isinstance(weight, MXTensor)
+    if not held:
+        _check_floating("weight", weight)
+    if bias is not None:
+        _check_floating("bias", bias)
+    for label, value in (("weight", None if held else weight), ("bias", bias)):
+        if value is not None and value.dtype != x.dtype:
+            raise ValueError(f"x and {label} must have the same dtype")
+    for label, value in (("weight", weight), ("bias", bias)):
+        if value is not None and value.device != x.device:
+            raise ValueError(f"x and {label} must use the same device")
+    if x.ndim == 0 or len(weight.shape) != 2:
+        raise ValueError("mx_linear takes x [..., k] and weight [o, k]")
+    (o, k) = weight.shape
+    if x.shape[-1] != k:
+        raise ValueError("x and weight have incompatible reduction dimensions")
+    if bias is not None and bias.shape != (o,):
+        raise ValueError("bias must have one value per output")
+    hip.require_device(x)
+    shape = x.shape[:-1] + (o,)
+    if x.numel() == 0 or o == 0:
+        # Nothing to sum: zeros, or the bias, tied to the operands for autograd.
+        y = x.sum(-1, keepdim=True).expand(shape) * 0
+        if not held:
+            y = y + weight.sum(-1) * 0
+        return y if bias is None else y + bias
+    if not held:
+        codes, scales = hip.mx_quantize(hip.rows_of(weight.detach()))
+    else:
+        codes, scales, weight = weight.codes, weight.scales, None
+    bias = None if bias is None else bias.contiguous()
+    return _MXLinear.apply(hip.rows_of(x), weight, bias, codes, scales).reshape(shape)
+
+
+__all__ = ["MXTensor", "mx_quantize", "mx_linear"]
