@@ -566,14 +566,22 @@ int mf_mx_quantize(const void *x, int32_t type, int64_t n, int64_t k, int64_t ld
 int mf_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, void *out,
                      int32_t type, void *stream);
 /* out [n, o] = Q(x) W^T + bias (bias: o values of x's type, or NULL), FP32 sums; W [o, k] in codes.
- * xcodes and xscales receive Q(x). */
+ * xcodes and xscales receive Q(x), the scales segment by segment ([S, n, 8]), as mf_mx_grad_weight
+ * takes them; where mf_mx_linear_sizes gives 0 bytes of codes they may be NULL and are not written
+ * (`keep`: they always are). workspace: the bytes that it gives, 8-byte aligned.
+ * n, o < 2^28, k < 2^24. */
+int mf_mx_linear_sizes(int32_t type, int64_t n, int64_t k, int64_t o, int32_t keep, int64_t *codes,
+                       int64_t *workspace);
 int mf_mx_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx,
                  const uint8_t *wcodes, const uint8_t *wscales, int64_t o, const void *bias,
-                 uint8_t *xcodes, uint8_t *xscales, void *out, void *stream);
+                 int32_t keep, uint8_t *xcodes, uint8_t *xscales, void *out, void *workspace,
+                 int64_t bytes, void *stream);
 /* Gradients of mf_mx_linear straight through the quantizers, for dy [n, o] (rows ldy apart), FP32
  * sums: dx [n, k] = dy Q(W), dw [o, k] = dy^T Q(x), db [o] = column sums of dy.  They share a workspace
- * of mf_mx_grad_workspace bytes (16-byte aligned), one after the other on one stream. */
-int mf_mx_grad_workspace(int32_t type, int64_t n, int64_t o, int64_t *bytes);
+ * of mf_mx_grad_workspace bytes (16-byte aligned), one after the other on one stream: it holds the
+ * 4-bit operand in BF16 and, where dy cannot be read in place, its BF16 terms.
+ * n < 2^28, o <= 2^22, k < 2^24. */
+int mf_mx_grad_workspace(int32_t type, int64_t n, int64_t k, int64_t o, int64_t *bytes);
 int mf_mx_grad_input(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
                      const uint8_t *wcodes, const uint8_t *wscales, int64_t k, void *dx,
                      void *workspace, int64_t bytes, void *stream);

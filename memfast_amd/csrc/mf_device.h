@@ -111,6 +111,17 @@ __device__ __forceinline__ void xcd_tile(u32 L, u32 nx, u32 ny, u32 &x, u32 &y) 
     y = P / nx;
 }
 
+// One 1 KiB LDS DMA: lane l's 16 bytes at src go to lds_base + 16 * l.  Issued
+// as inline assembly so that the compiler's wait-count analysis does not track
+// it (it would otherwise wait for it at the next loop header); the kernel waits
+// for it explicitly (s_waitcnt vmcnt(0) and a barrier) before reading the data.
+__device__ __forceinline__ void lds_dma_16(const void *src, u32 lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(src), "s"(lds_base)
+                 : "memory", "m0");
+}
+
 // Copy a status word to a caller's pinned host word, marked MF_STATUS_PUBLISHED.  Called by
 // one lane of a kernel that started after the kernels setting those bits had finished: the
 // device-scope load sees their atomics, and the system-scope store writes through to host

@@ -18,6 +18,7 @@
 // (two significant bits), so the 4-bit operand is expanded to BF16 in LDS, and dy enters as
 // BF16 terms whose sum is its value exactly: one for BF16, two for FP16, three for FP32.
 #include <algorithm>
+#include <type_traits>
 
 #include "mf_float.h"
 
@@ -80,10 +81,11 @@ __device__ __forceinline__ u32 codes8(const float (&v)[8], u32 byte) {
 }
 
 // One lane quantizes eight values and four neighbours share a block.  1 << lanes lanes lie along a
-// row, the others take further rows.
+// row, the others take further rows. Scales go to [n, segs * 8], or to [segs, n, 8] if `turned`.
 template <typename T>
 __global__ __launch_bounds__(256) void k_mx_quantize(const T *x, i64 n, i64 k, i64 ldx, bool vec,
-                                                     int lanes, u8 *codes, u8 *scales) {
+                                                     int lanes, bool turned, u8 *codes,
+                                                     u8 *scales) {
     const i64 segs = segments(k), units = segs * 32;
     const i64 unit = (i64(blockIdx.x) << lanes) + (threadIdx.x & ((1 << lanes) - 1));
     const i64 step = i64(gridDim.y) * (256 >> lanes);
@@ -96,7 +98,9 @@ __global__ __launch_bounds__(256) void k_mx_quantize(const T *x, i64 n, i64 k, i
         peak = max(peak, u32(__shfl_xor(int(peak), 2)));
         const u32 byte = scale_byte(peak);
         reinterpret_cast<u32 *>(codes + r * segs * SEG_BYTES)[unit] = codes8(v, byte);
-        if ((unit & 3) == 0) scales[r * segs * SEG_SCALES + unit / 4] = u8(byte);
+        if ((unit & 3) == 0)
+            scales[turned ? (unit / 32 * n + r) * SEG_SCALES + (unit / 4 & 7)
+                          : r * segs * SEG_SCALES + unit / 4] = u8(byte);
     }
 }
 
@@ -161,64 +165,246 @@ __device__ __forceinline__ v16f mfma_step(v4u a, v4u b, v16f c, u32 sa, u32 sb) 
 }
 
 struct MxArgs {
-    const u8 *xc, *xs;      // [n, segs * 128], [n, segs * 8]
-    const u8 *wc, *ws;      // [o, ...]
+    const u8 *xc, *xs;      // codes [n, segs * 128], scales [segs, n, 8]
+    const u8 *wc, *ws;      // codes [o, segs * 128], scales [o, segs * 8] (tiles: [segs, o, 8])
+    const void *x;          // k_mx_few<..., true>: the input itself, rows ldx apart
+    i64 ldx, k;
+    bool vec;
     const void *bias;       // [o] or nullptr
     void *out;              // [n, o]
     i64 n, o, segs;
 };
 
-// A wave takes 32 rows by 32 columns of y straight from global memory.
-template <typename T>
-__global__ __launch_bounds__(256) void k_mx_mm(const MxArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int half = lane >> 5;
-    const i64 n0 = (i64(blockIdx.y) * 2 + (wave >> 1)) * 32;
-    const i64 o0 = (i64(blockIdx.x) * 2 + (wave & 1)) * 32;
-    if (n0 >= a.n || o0 >= a.o) return;
+// ---- few rows --------------------------------------------------------------
+// Up to 64 rows of x: the weight's bytes bound it, so each is loaded once, straight into the operand
+// registers. A workgroup takes 16 rows of W; its eight waves split the segments and add their
+// sums in LDS in the order of the waves. QUANTIZE: the workgroup quantizes x into LDS itself, while
+// its first weights are on their way, which saves a launch; else Q(x) is read from the cache.
+constexpr int FEW_WAVES = 8, FEW_TILE = 16;
+
+__device__ __forceinline__ v4f mfma_few(v4u a, v4u b, v4f c, u32 sa, u32 sb) {
+    const v8i av = {int(a.x), int(a.y), int(a.z), int(a.w), 0, 0, 0, 0};
+    const v8i bv = {int(b.x), int(b.y), int(b.z), int(b.w), 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, int(sa), 0, int(sb));
+}
+
+__host__ __device__ inline i64 few_pitch(i64 segs) { return segs * SEG_BYTES + 16; }
+
+__host__ inline i64 few_lds(i64 n, i64 segs) {
+    return n * few_pitch(segs) + n * segs * SEG_SCALES;
+}
+
+template <typename T, int NT, bool QUANTIZE>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_mx_few(const MxArgs a) {
+    extern __shared__ __align__(16) u8 staged[];
+    __shared__ float part[FEW_WAVES][NT][FEW_TILE * FEW_TILE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = lane & 15, block = lane >> 4;
+    const i64 o0 = i64(blockIdx.x) * FEW_TILE;
+    const i64 per = (a.segs + FEW_WAVES - 1) / FEW_WAVES;
+    const i64 first = min(wave * per, a.segs), last = min(first + per, a.segs);
     // Rows past the end read the last row; their results are not stored.
-    const i64 row = min(n0 + (lane & 31), a.n - 1), col = min(o0 + (lane & 31), a.o - 1);
-    const u8 *xc = a.xc + row * a.segs * SEG_BYTES + half * 16;
-    const u8 *wc = a.wc + col * a.segs * SEG_BYTES + half * 16;
-    const u8 *xs = a.xs + row * a.segs * SEG_SCALES, *ws = a.ws + col * a.segs * SEG_SCALES;
-    v16f acc = {};
-    for (i64 s = 0; s < a.segs; ++s) {
-        const u32 sx = half_scales(reinterpret_cast<const v2u *>(xs)[s], half);
-        const u32 sw = half_scales(reinterpret_cast<const v2u *>(ws)[s], half);
-        const v4u *x4 = reinterpret_cast<const v4u *>(xc + s * SEG_BYTES);
-        const v4u *w4 = reinterpret_cast<const v4u *>(wc + s * SEG_BYTES);
-        acc = mfma_step<0>(x4[0], w4[0], acc, sx, sw);
-        acc = mfma_step<1>(x4[2], w4[2], acc, sx, sw);
-        acc = mfma_step<2>(x4[4], w4[4], acc, sx, sw);
-        acc = mfma_step<3>(x4[6], w4[6], acc, sx, sw);
+    const i64 o = min(o0 + row, a.o - 1);
+    const u8 *wc = a.wc + o * a.segs * SEG_BYTES + block * 16, *ws = a.ws + o * a.segs * SEG_SCALES;
+
+    v4u w[2];
+    v2u sw;
+    auto load_weight = [&](i64 s) {
+        w[0] = *reinterpret_cast<const v4u *>(wc + s * SEG_BYTES);
+        w[1] = *reinterpret_cast<const v4u *>(wc + s * SEG_BYTES + 64);
+        sw = *reinterpret_cast<const v2u *>(ws + s * SEG_SCALES);
+    };
+    if (first < last) load_weight(first);
+
+    const i64 pitch = few_pitch(a.segs);
+    u8 *const staged_scales = staged + a.n * pitch;
+    if (QUANTIZE) {
+        const i64 units = a.segs * 32;
+        for (i64 r = 0; r < a.n; ++r)
+            for (i64 unit = tid; unit < units; unit += 64 * FEW_WAVES) {
+                float v[8];
+                load8(static_cast<const T *>(a.x) + r * a.ldx, unit * 8, a.k, a.vec, v);
+                u32 peak = peak8(v);
+                peak = max(peak, u32(__shfl_xor(int(peak), 1)));
+                peak = max(peak, u32(__shfl_xor(int(peak), 2)));
+                const u32 byte = scale_byte(peak);
+                reinterpret_cast<u32 *>(staged + r * pitch)[unit] = codes8(v, byte);
+                if ((unit & 3) == 0)
+                    staged_scales[r * a.segs * SEG_SCALES + unit / 4] = u8(byte);
+            }
+        __syncthreads();
     }
-    const i64 c = o0 + (lane & 31);
-    if (c >= a.o) return;
-    const float bias = a.bias ? float(static_cast<const T *>(a.bias)[c]) : 0.0f;
+
+    v4f acc[NT] = {};
+    for (i64 s = first; s < last; ++s) {
+        const v4u w0 = w[0], w1 = w[1];
+        const v2u scale = sw;
+        if (s + 1 < last) load_weight(s + 1);
+        const u32 sw0 = scale.x >> (8 * block), sw1 = scale.y >> (8 * block);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const i64 r = min(i64(16 * t + row), a.n - 1);
+            const u8 *xc = QUANTIZE ? staged + r * pitch : a.xc + r * a.segs * SEG_BYTES;
+            const u8 *xs = QUANTIZE ? staged_scales + r * a.segs * SEG_SCALES + s * SEG_SCALES
+                                    : a.xs + (s * a.n + r) * SEG_SCALES;
+            const v4u x0 = *reinterpret_cast<const v4u *>(xc + s * SEG_BYTES + block * 16);
+            const v4u x1 = *reinterpret_cast<const v4u *>(xc + s * SEG_BYTES + 64 + block * 16);
+            const v2u sx = *reinterpret_cast<const v2u *>(xs);
+            acc[t] = mfma_few(x0, w0, acc[t], sx.x >> (8 * block), sw0);
+            acc[t] = mfma_few(x1, w1, acc[t], sx.y >> (8 * block), sw1);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][t][(4 * block + i) * FEW_TILE + row] = acc[t][i];
+    __syncthreads();
+    for (int e = tid; e < NT * FEW_TILE * FEW_TILE; e += 64 * FEW_WAVES) {
+        const int t = e / (FEW_TILE * FEW_TILE), at = e % (FEW_TILE * FEW_TILE);
+        const i64 n = 16 * t + at / FEW_TILE, c = o0 + at % FEW_TILE;
+        if (n >= a.n || c >= a.o) continue;
+        float sum = part[0][t][at];
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; ++w) sum += part[w][t][at];
+        if (a.bias) sum += float(static_cast<const T *>(a.bias)[c]);
+        static_cast<T *>(a.out)[n * a.o + c] = T(sum);
+    }
+}
+
+// ---- many rows -------------------------------------------------------------
+// WN x WO waves of TN x TO tiles of 32 x 32. A stage is one segment (128 bytes) of every row of the
+// tile, copied to LDS without passing through registers, one stage ahead of the matrix cores.
+// The 16-byte pieces of row r lie rotated by r & 7, so that the eight rows that a read serves at
+// once are in different banks. Scales come segment by segment ([segs, rows, 8]): a wave reads those
+// of 32 rows as 256 consecutive bytes, one segment ahead, into registers.
+template <typename T, int WN, int WO, int TN, int TO>
+__global__ __launch_bounds__(64 * WN * WO) void k_mx_tile(const MxArgs a) {
+    constexpr int BN = 32 * WN * TN, BO = 32 * WO * TO, WAVES = WN * WO;
+    constexpr int COPIES = (BN + BO) / 8 / WAVES;   // of 8 rows, by each wave
+    static_assert((BN + BO) % (8 * WAVES) == 0, "whole copies");
+    extern __shared__ __align__(16) u8 staged[];      // [2][BN + BO][128]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int half = lane >> 5, row = lane & 31;
+    u32 tx, ty;
+    xcd_tile(blockIdx.x, u32((a.n + BN - 1) / BN), u32((a.o + BO - 1) / BO), tx, ty);
+    const i64 n0 = i64(tx) * BN, o0 = i64(ty) * BO;
+    const i64 pitch = a.segs * SEG_BYTES;
+
+    // Where this lane's copies come from, eight rows of one operand each: rows past the end read
+    // the last row.
+    const int first_copy = __builtin_amdgcn_readfirstlane(wave * COPIES);
+    const u8 *const x0 = a.xc + n0 * pitch, *const w0 = a.wc + o0 * pitch;
+    u32 offset[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+        const int r = (first_copy + i) * 8 + (lane >> 3);
+        const i64 at = r < BN ? min(i64(r), a.n - n0 - 1) : min(i64(r - BN), a.o - o0 - 1);
+        offset[i] = u32(at * pitch) + u32(((lane & 7) ^ (lane >> 3)) * 16);
+    }
+    const u32 lds = u32(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) u8 *)staged));
+    auto copy = [&](i64 s, int buffer) {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            const int r = (first_copy + i) * 8;
+            lds_dma_16((r < BN ? x0 : w0) + s * SEG_BYTES + offset[i],
+                       __builtin_amdgcn_readfirstlane(lds + (buffer * (BN + BO) + r) * SEG_BYTES));
+        }
+    };
+
+    const int wn = (wave / WO) * TN * 32, wo = (wave % WO) * TO * 32;
+    u32 xat[TN], wat[TO];       // scale offsets of this lane's rows in a segment
+#pragma unroll
+    for (int i = 0; i < TN; ++i) xat[i] = u32(min(n0 + wn + 32 * i + row, a.n - 1)) * SEG_SCALES;
+#pragma unroll
+    for (int j = 0; j < TO; ++j) wat[j] = u32(min(o0 + wo + 32 * j + row, a.o - 1)) * SEG_SCALES;
+    v2u xs[TN], ws[TO];
+    auto load_scales = [&](i64 s) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+            xs[i] = *reinterpret_cast<const v2u *>(a.xs + s * a.n * SEG_SCALES + xat[i]);
+#pragma unroll
+        for (int j = 0; j < TO; ++j)
+            ws[j] = *reinterpret_cast<const v2u *>(a.ws + s * a.o * SEG_SCALES + wat[j]);
+    };
+
+    v16f acc[TN][TO] = {};
+    copy(0, 0);
+    load_scales(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    for (i64 s = 0; s < a.segs; ++s) {
+        u32 sx[TN], sw[TO];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) sx[i] = half_scales(xs[i], half);
+#pragma unroll
+        for (int j = 0; j < TO; ++j) sw[j] = half_scales(ws[j], half);
+        if (s + 1 < a.segs) {
+            copy(s + 1, int(s + 1) & 1);
+            load_scales(s + 1);
+        }
+        const u8 *xt = staged + (int(s) & 1) * (BN + BO) * SEG_BYTES + (wn + row) * SEG_BYTES;
+        const u8 *wt = staged + (int(s) & 1) * (BN + BO) * SEG_BYTES + (BN + wo + row) * SEG_BYTES;
+        auto step = [&](auto number) {
+            constexpr int STEP = decltype(number)::value;
+            const int piece = ((2 * STEP + half) ^ (row & 7)) * 16;
+            v4u fx[TN], fw[TO];
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+                fx[i] = *reinterpret_cast<const v4u *>(xt + i * 32 * SEG_BYTES + piece);
+#pragma unroll
+            for (int j = 0; j < TO; ++j)
+                fw[j] = *reinterpret_cast<const v4u *>(wt + j * 32 * SEG_BYTES + piece);
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int j = 0; j < TO; ++j)
+                    acc[i][j] = mfma_step<STEP>(fx[i], fw[j], acc[i][j], sx[i], sw[j]);
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+        // The copies are not in the compiler's count of outstanding loads.
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+    }
     T *out = static_cast<T *>(a.out);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const i64 r = n0 + 8 * (i / 4) + 4 * half + (i & 3);
-        if (r < a.n) out[r * a.o + c] = T(acc[i] + bias);
+    for (int j = 0; j < TO; ++j) {
+        const i64 c = o0 + wo + 32 * j + row;
+        if (c >= a.o) continue;
+        const float bias = a.bias ? float(static_cast<const T *>(a.bias)[c]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const i64 r = n0 + wn + 32 * i + 8 * (e / 4) + 4 * half + (e & 3);
+                if (r < a.n) out[r * a.o + c] = T(acc[i][j][e] + bias);
+            }
     }
+}
+
+// Scales [rows, segs * 8] as [segs, rows, 8].
+__global__ __launch_bounds__(256) void k_mx_turn_scales(const v2u *in, i64 rows, i64 segs, v2u *out) {
+    const i64 r = i64(blockIdx.x) * 256 + threadIdx.x;
+    if (r < rows) out[blockIdx.y * rows + r] = in[r * segs + blockIdx.y];
 }
 
 // ---------------------------------------------------------------------------
 // Gradients
 // ---------------------------------------------------------------------------
-constexpr int GRAD_TILE = 128, GRAD_STEP = 64;
-constexpr int GRAD_PITCH = 160;   // BF16 values of an LDS row of 128, padded against bank conflicts
+constexpr int GRAD_STEP = 64;     // of the contraction in one stage
 
 struct GradArgs {
-    const bf16 *a;          // dy terms: plane t at a + t * plane, rows of lda values
+    const bf16 *a;      // dy terms: plane t at a + t * plane, rows of lda values
     i64 plane, lda;
-    i64 width;              // values of a row that may be read, a multiple of 8
+    i64 width;          // values of a row that may be read, a multiple of 8
     int terms;
-    const u8 *codes, *scales;   // the 4-bit operand [contraction, segs * 128]
-    i64 segs;
-    i64 rows, cols;         // of the result
-    i64 depth;              // contraction
-    void *out;              // [rows, cols]
+    const bf16 *b;      // the 4-bit operand expanded, [depth in whole steps, cols in segments]
+    i64 ldb;
+    i64 rows, cols;     // of the result
+    i64 depth;          // contraction
+    void *out;          // [rows, cols]
 };
 
 // dy [n, o] as `terms` planes of BF16, [terms][rows][cols] with zeros past n and o: the terms add
@@ -242,116 +428,165 @@ __global__ __launch_bounds__(256) void k_mx_terms(const T *dy, i64 n, i64 o, i64
     }
 }
 
+// Codes [n, segs * 128] as BF16 [rows, segs * 256], zeros past n; scales [n, segs * 8], or
+// [segs, n, 8] if `turned`. A lane expands eight values.
+__global__ __launch_bounds__(256) void k_mx_expand(const u32 *codes, const u8 *scales, i64 n, i64 segs,
+                                                   bool turned, i64 rows, bf16 *out) {
+    const i64 unit = i64(blockIdx.x) * 256 + threadIdx.x;
+    if (unit >= segs * 32) return;
+    for (i64 r = blockIdx.y; r < rows; r += gridDim.y) {
+        v8bf v = {};
+        if (r < n) {
+            const u32 word = codes[r * segs * 32 + unit];
+            const float scale =
+                scale_of(scales[turned ? (unit / 32 * n + r) * SEG_SCALES + (unit / 4 & 7)
+                                       : r * segs * SEG_SCALES + unit / 4]);
+            float x[8];
+            values8(word, scale, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = bf16(x[i]);
+        }
+        *reinterpret_cast<v8bf *>(out + (r * segs * 32 + unit) * 8) = v;
+    }
+}
+
 typedef __attribute__((address_space(3))) v4s *lds_v4s;
 
-// Four rows by sixteen columns per sixteen lanes, transposed: the lane gets its column's values
-// of rows c .. c + 3 (and, with a second read, c + 4 .. c + 7).
-__device__ __forceinline__ v8bf transposed(const bf16 *tile, int c, int col, int lane) {
-    const int i = lane & 15;
-    const bf16 *p = tile + (c + (i >> 2)) * GRAD_PITCH + col + 4 * (i & 3);
+// The values of rows r .. r + 3 and r + 4 .. r + 7 of a lane's column, from the address of the four
+// columns' piece that this lane supplies of row r + (lane & 15) / 4.
+__device__ __forceinline__ v8bf transposed(const u8 *p, int four_rows) {
     union {
         v4s s[2];
         v8bf v;
     } u;
     u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(p));
-    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(p + 4 * GRAD_PITCH));
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(p + four_rows));
     return u.v;
 }
 
-// The 32 values of a block as BF16.
-__device__ __forceinline__ void expand_block(v4u codes, u32 byte, bf16 *to) {
-    const float scale = scale_of(byte);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        float v[8];
-        values8(codes[w], scale, v);
-        v8bf out;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = bf16(v[i]);
-        *reinterpret_cast<v8bf *>(to + 8 * w) = out;
-    }
+// How far the 16-byte pieces of row r lie rotated in LDS, in rows of that many pieces: four
+// consecutive rows' reads of 64 bytes are then in different banks.
+template <int PIECES> __device__ __forceinline__ int rotation(int r) {
+    static_assert(PIECES == 8 || PIECES == 16 || PIECES == 32, "the rotation stays within the row");
+    return PIECES == 8 ? 4 * (r >> 1 & 1) : 4 * (r & 3);
 }
 
-// out[m, c] = sum_t sum_d A_t[m, d] B[d, c] over 128 x 128 tiles, 64 of the contraction at a time.
-// DEPTH_ROWS: A's rows run along the contraction (dw: A is dy^T); else along m (dx).
-// A has GRAD_STEP-padded contraction with zeros in the padding, B's rows past depth are zeros here.
-template <typename T, bool DEPTH_ROWS>
-__global__ __launch_bounds__(256) void k_mx_grad(const GradArgs a) {
-    __shared__ alignas(16) bf16 tile_a[GRAD_TILE * GRAD_STEP > GRAD_STEP * GRAD_PITCH ? GRAD_TILE * GRAD_STEP
-                                                                         : GRAD_STEP * GRAD_PITCH];
-    __shared__ alignas(16) bf16 tile_b[GRAD_STEP * GRAD_PITCH];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const i64 m0 = i64(blockIdx.y) * GRAD_TILE, c0 = i64(blockIdx.x) * GRAD_TILE;
-    const int wm = (wave >> 1) * 64, wc = (wave & 1) * 64;
-    const int tr_col = 16 * ((lane >> 4) & 1), tr_row = 8 * (lane >> 5);
-    v16f acc[2][2] = {};
-    for (int t = a.terms - 1; t >= 0; --t) {
-        const bf16 *plane = a.a + t * a.plane;
-        for (i64 d0 = 0; d0 < a.depth; d0 += GRAD_STEP) {
-            __syncthreads();
-            if (DEPTH_ROWS) {   // 64 rows of 128 values, 16 pieces each
-                for (int u = tid; u < GRAD_STEP * 16; u += 256) {
-                    const int r = u >> 4, p = u & 15;
-                    const i64 m = min(m0 + p * 8, a.width - 8);
-                    *reinterpret_cast<v4u *>(tile_a + r * GRAD_PITCH + p * 8) =
-                        *reinterpret_cast<const v4u *>(plane + (d0 + r) * a.lda + m);
-                }
-            } else {            // 128 rows of 64 values, 8 pieces each, rotated by the row
-                for (int u = tid; u < GRAD_TILE * 8; u += 256) {
-                    const int r = u >> 3, p = u & 7;
-                    const i64 m = min(m0 + r, a.rows - 1);
-                    *reinterpret_cast<v4u *>(tile_a + r * GRAD_STEP + (p ^ (r & 7)) * 8) =
-                        *reinterpret_cast<const v4u *>(plane + m * a.lda + d0 + p * 8);
-                }
-            }
-            {                   // 64 rows of four blocks: one block a thread
-                const int r = tid >> 2, b = tid & 3;
-                const i64 d = d0 + r;
-                v4u codes = {0, 0, 0, 0};
-                u32 byte = 1;
-                if (d < a.depth) {
-                    codes = *reinterpret_cast<const v4u *>(a.codes + d * a.segs * SEG_BYTES +
-                                                           c0 / 2 + b * 16);
-                    byte = a.scales[d * a.segs * SEG_SCALES + c0 / 32 + b];
-                }
-                expand_block(codes, byte, tile_b + r * GRAD_PITCH + b * 32);
-            }
-            __syncthreads();
+// out[m, c] = sum_t sum_d A_t[m, d] B[d, c], WM x WC waves of TM x TC tiles of 32 x 32, 64 of the
+// contraction a stage, copied to LDS one stage ahead without passing through registers.
+// DEPTH_ROWS: A's rows run along the contraction (dw: A is dy^T); else along m (dx). Operands whose rows
+// run along the contraction are read transposed, four rows of 16 columns by 16 lanes.
+template <typename T, bool DEPTH_ROWS, int WM, int WC, int TM, int TC>
+__global__ __launch_bounds__(64 * WM * WC) void k_mx_grad(const GradArgs a) {
+    constexpr int BM = 32 * WM * TM, BC = 32 * WC * TC, WAVES = WM * WC;
+    constexpr int A_BYTES = BM * GRAD_STEP * 2, STAGE = (BM + BC) * GRAD_STEP * 2;
+    constexpr int COPIES = STAGE / 1024 / WAVES;
+    static_assert(STAGE % (1024 * WAVES) == 0 && A_BYTES % 1024 == 0, "whole copies");
+    extern __shared__ __align__(16) u8 staged[];    // [2][A, B]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    u32 tx, ty;
+    xcd_tile(blockIdx.x, u32((a.rows + BM - 1) / BM), u32((a.cols + BC - 1) / BC), tx, ty);
+    const i64 m0 = i64(tx) * BM, c0 = i64(ty) * BC;
+
+    const int first_copy = __builtin_amdgcn_readfirstlane(wave * COPIES);
+    u32 offset[COPIES];
 #pragma unroll
-            for (int s = 0; s < GRAD_STEP / 16; ++s) {
-                v8bf fa[2], fb[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (DEPTH_ROWS) {
-                        fa[i] = transposed(tile_a, 16 * s + tr_row, wm + 32 * i + tr_col, lane);
-                    } else {
-                        const int r = wm + 32 * i + (lane & 31), p = 2 * s + (lane >> 5);
-                        fa[i] = *reinterpret_cast<const v8bf *>(tile_a + r * GRAD_STEP +
-                                                                (p ^ (r & 7)) * 8);
-                    }
-                    fb[i] = transposed(tile_b, 16 * s + tr_row, wc + 32 * i + tr_col, lane);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j],
-                                                                            acc[i][j], 0, 0, 0);
-            }
+    for (int i = 0; i < COPIES; ++i) {
+        const int at = (first_copy + i) * 1024;
+        if (at < A_BYTES && !DEPTH_ROWS) {      // rows of 64 values, 8 pieces rotated by the row
+            const int piece = at / 16 + lane, r = piece >> 3;
+            offset[i] = u32(min(i64(r), a.rows - m0 - 1) * a.lda * 2) + u32(((piece ^ r) & 7) * 16);
+        } else if (at < A_BYTES) {
+            constexpr int PIECES = BM / 8;
+            const int piece = at / 16 + lane, r = piece / PIECES;
+            const int p = piece % PIECES ^ rotation<PIECES>(r);
+            offset[i] = u32(r * a.lda * 2) + u32(min(m0 + p * 8, a.width - 8) - m0) * 2;
+        } else {
+            constexpr int PIECES = BC / 8;
+            const int piece = (at - A_BYTES) / 16 + lane, r = piece / PIECES;
+            offset[i] = u32(r * a.ldb * 2) + u32((piece % PIECES ^ rotation<PIECES>(r)) * 16);
         }
+    }
+    const u32 lds = u32(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) u8 *)staged));
+    const i64 steps = (a.depth + GRAD_STEP - 1) / GRAD_STEP, stages = steps * a.terms;
+    int term = a.terms - 1;     // the smallest terms first
+    i64 step = 0;               // of the next copy
+    auto copy = [&](int buffer) {
+        const bf16 *plane = a.a + term * a.plane;
+        const u8 *a0 = reinterpret_cast<const u8 *>(
+            DEPTH_ROWS ? plane + step * GRAD_STEP * a.lda + m0 : plane + m0 * a.lda + step * GRAD_STEP);
+        const u8 *b0 = reinterpret_cast<const u8 *>(a.b + step * GRAD_STEP * a.ldb + c0);
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            const int at = (first_copy + i) * 1024;
+            lds_dma_16((at < A_BYTES ? a0 : b0) + offset[i],
+                       __builtin_amdgcn_readfirstlane(lds + buffer * STAGE + at));
+        }
+        if (++step == steps) {
+            step = 0;
+            --term;
+        }
+    };
+
+    // Where this lane's fragments start in a stage.
+    const int wm = (wave / WC) * TM * 32, wc = (wave % WC) * TC * 32;
+    const int i16 = lane & 15, side = lane >> 4 & 1, half = lane >> 5;
+    int at_a[TM], at_b[TC];
+    auto turned_at = [&](int col, auto width) {
+        constexpr int PIECES = decltype(width)::value / 8;
+        const int r = 8 * half + (i16 >> 2), piece = (col + 16 * side) / 8 + (i16 & 3) / 2;
+        return r * PIECES * 16 + (piece ^ rotation<PIECES>(r)) * 16 + (i16 & 1) * 8;
+    };
+    const std::integral_constant<int, BM> bm{};
+    const std::integral_constant<int, BC> bc{};
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+        at_a[i] = DEPTH_ROWS ? turned_at(wm + 32 * i, bm) : (wm + 32 * i + (lane & 31)) * GRAD_STEP * 2;
+#pragma unroll
+    for (int j = 0; j < TC; ++j) at_b[j] = A_BYTES + turned_at(wc + 32 * j, bc);
+
+    v16f acc[TM][TC] = {};
+    copy(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    for (i64 stage = 0; stage < stages; ++stage) {
+        if (stage + 1 < stages) copy(int(stage + 1) & 1);
+        const u8 *tile = staged + (int(stage) & 1) * STAGE;
+#pragma unroll
+        for (int s = 0; s < GRAD_STEP / 16; ++s) {
+            v8bf fa[TM], fb[TC];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                fa[i] = DEPTH_ROWS
+                            ? transposed(tile + at_a[i] + s * 16 * BM * 2, 4 * BM * 2)
+                            : *reinterpret_cast<const v8bf *>(
+                                  tile + at_a[i] + ((2 * s + half) ^ (lane & 7)) * 16);
+#pragma unroll
+            for (int j = 0; j < TC; ++j)
+                fb[j] = transposed(tile + at_b[j] + s * 16 * BC * 2, 4 * BC * 2);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TC; ++j)
+                    acc[i][j] =
+                        __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
+        // The copies are not in the compiler's count of outstanding loads.
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
     }
     T *out = static_cast<T *>(a.out);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < TC; ++j) {
+        const i64 c = c0 + wc + 32 * j + (lane & 31);
+        if (c >= a.cols) continue;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const i64 c = c0 + wc + 32 * j + (lane & 31);
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const i64 m = m0 + wm + 32 * i + 8 * (e / 4) + 4 * (lane >> 5) + (e & 3);
-                if (m < a.rows && c < a.cols) out[m * a.cols + c] = T(acc[i][j][e]);
+                const i64 m = m0 + wm + 32 * i + 8 * (e / 4) + 4 * half + (e & 3);
+                if (m < a.rows) out[m * a.cols + c] = T(acc[i][j][e]);
             }
-        }
+    }
 }
 
 // Sums of `rows` values down each column, 64 columns by 4 rows a workgroup; FP32 sums of chunk
@@ -395,6 +630,11 @@ constexpr i64 MOST = i64(1) << 30;   // rows and columns of an operand
 
 static bool sizes_ok(i64 n, i64 k) { return n >= 1 && k >= 1 && n < MOST && k < MOST; }
 
+// A tile's offsets into dy and the expanded operand stay in 32 bits.
+static bool grad_ok(i64 n, i64 k, i64 o) {
+    return n >= 1 && k >= 1 && o >= 1 && n < i64(1) << 28 && o <= i64(1) << 22 && k < i64(1) << 24;
+}
+
 static int terms_of(int32_t type) { return type == MF_BF16 ? 1 : type == MF_F16 ? 2 : 3; }
 
 static i64 padded(i64 v) { return (v + GRAD_STEP - 1) / GRAD_STEP * GRAD_STEP; }
@@ -402,7 +642,7 @@ static i64 padded(i64 v) { return (v + GRAD_STEP - 1) / GRAD_STEP * GRAD_STEP; }
 // BF16 gradients whose contraction is whole steps and whose rows are whole pieces are read in place.
 static bool terms_in_place(const void *dy, int32_t type, i64 n, i64 o, i64 ldy, bool depth_rows) {
     return type == MF_BF16 && (depth_rows ? n : o) % GRAD_STEP == 0 && o % 8 == 0 && ldy % 8 == 0 &&
-           aligned(dy, 16);
+           ldy <= i64(1) << 22 && aligned(dy, 16);
 }
 
 static i64 terms_bytes(int32_t type, i64 n, i64 o) {
@@ -436,15 +676,127 @@ static int make_terms(const void *dy, int32_t type, i64 n, i64 o, i64 ldy, bool 
     });
 }
 
-template <bool DEPTH_ROWS> static int launch_grad(const GradArgs &args, int32_t type, hipStream_t s) {
-    const i64 gx = (args.cols + GRAD_TILE - 1) / GRAD_TILE, gy = (args.rows + GRAD_TILE - 1) / GRAD_TILE;
-    if (gy > 65535) return fail(MF_E_UNSUPPORTED, "too many rows of a gradient");
+static i64 expanded_bytes(i64 depth, i64 k) { return padded(depth) * segments(k) * SEG * 2; }
+
+// dy's terms and the expanded operand, one behind the other.
+static i64 grad_bytes(int32_t type, i64 n, i64 o, i64 depth, i64 k) {
+    return terms_bytes(type, n, o) + expanded_bytes(depth, k);
+}
+
+template <typename T, bool DEPTH_ROWS, int WM, int WC, int TM, int TC>
+static int launch_grad_tile(const GradArgs &args, hipStream_t s) {
+    constexpr int BM = 32 * WM * TM, BC = 32 * WC * TC, LDS = 2 * (BM + BC) * GRAD_STEP * 2;
+    static_assert(BC <= SEG, "a tile's columns are within the padding of the rows");
+    const i64 tiles = (args.rows + BM - 1) / BM * ((args.cols + BC - 1) / BC);
+    if (tiles > i64(1) << 30) return fail(MF_E_UNSUPPORTED, "gradient too large");
+    auto kernel = k_mx_grad<T, DEPTH_ROWS, WM, WC, TM, TC>;
+    if (LDS > 64 << 10) {
+        const hipError_t e = hipFuncSetAttribute(
+            reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return fail(MF_E_RESOURCE, "LDS of a gradient: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3(unsigned(tiles)), dim3(64 * WM * WC), LDS, s, args);
+    return check_launch("microscaled gradient");
+}
+
+template <bool DEPTH_ROWS>
+static int launch_grad(GradArgs args, int32_t type, i64 n, i64 o, const u8 *codes, const u8 *scales,
+                       void *workspace, i64 bytes, hipStream_t s) {
+    if (!workspace || bytes < grad_bytes(type, n, o, args.depth, args.cols) || !aligned(workspace, 16))
+        return fail(MF_E_INVALID, "gradient workspace is missing, unaligned or too small");
+    const i64 segs = segments(args.cols), rows = padded(args.depth);
+    bf16 *const b = reinterpret_cast<bf16 *>(static_cast<u8 *>(workspace) + terms_bytes(type, n, o));
+    const dim3 grid(unsigned((segs * 32 + 255) / 256), unsigned(std::min<i64>(rows, 65535)));
+    hipLaunchKernelGGL(k_mx_expand, grid, dim3(256), 0, s, reinterpret_cast<const u32 *>(codes), scales,
+                       args.depth, segs, DEPTH_ROWS, rows, b);
+    args.b = b;
+    args.ldb = segs * SEG;
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL((k_mx_grad<T, DEPTH_ROWS>), dim3(unsigned(gx), unsigned(gy)), dim3(256), 0,
-                           s, args);
-        return check_launch("microscaled gradient");
+        // The largest tile of which every compute unit gets one (us, 64 x 64 / 128 x 128 /
+        // 256 x 256, n x k x o): dw of 2048 x 11008 x 4096 402 / 262 / 191, dx of it 359 / 277 / 220, dx of
+        // 2048 x 4096 x 11008 341 / 200 / 273, dx of 512 x 1024 x 1024 9 / 15 / 31.
+        const auto tiles = [&](i64 edge) {
+            return (args.rows + edge - 1) / edge * ((args.cols + edge - 1) / edge);
+        };
+        if (tiles(256) >= 256) return launch_grad_tile<T, DEPTH_ROWS, 2, 4, 4, 2>(args, s);
+        if (tiles(128) >= 256) return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 2, 2>(args, s);
+        return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 1, 1>(args, s);
     });
+}
+
+static int launch_quantize(const void *x, int32_t type, i64 n, i64 k, i64 ldx, bool turned, u8 *codes,
+                           u8 *scales, hipStream_t s) {
+    if (!x || !codes || !scales || !known_type(type) || !sizes_ok(n, k) || (n > 1 && ldx < k) ||
+        !aligned(codes, 16) || !aligned(scales, 8))
+        return fail(MF_E_INVALID, "invalid microscaled quantization arguments");
+    const i64 units = segments(k) * 32;
+    const int lanes = row_lanes(units);
+    return with_type(type, [&](auto zero) {
+        using T = decltype(zero);
+        const bool vec = aligned(x, 16) && (n == 1 || ldx % PIECE<T> == 0);
+        hipLaunchKernelGGL(k_mx_quantize<T>, row_grid(units, n, lanes), dim3(256), 0, s,
+                           static_cast<const T *>(x), n, k, ldx, vec, lanes, turned, codes, scales);
+        return check_launch("microscaled quantization");
+    });
+}
+
+// Rows and columns whose scale offsets stay in 32 bits, and depths whose tiles' code offsets do.
+static bool product_ok(i64 n, i64 k, i64 o) {
+    return n >= 1 && k >= 1 && o >= 1 && n < i64(1) << 28 && o < i64(1) << 28 && k < i64(1) << 24;
+}
+
+struct ProductPlan {
+    bool few;        // k_mx_few, else k_mx_tile
+    bool quantize;   // Q(x) goes through memory
+};
+
+constexpr i64 FEW_ROWS = 64;
+constexpr i64 FEW_QUANTIZE = 32768;   // values of x that every workgroup may quantize again
+
+static ProductPlan plan_product(i64 n, i64 k, bool keep) {
+    const bool few = n <= FEW_ROWS;
+    return {few, keep || !few || n > 16 || n * segments(k) * SEG > FEW_QUANTIZE};
+}
+
+template <typename T> static int launch_few(const MxArgs &args, const ProductPlan &plan, hipStream_t s) {
+    const dim3 grid(unsigned((args.o + FEW_TILE - 1) / FEW_TILE)), block(64 * FEW_WAVES);
+    if (!plan.quantize)
+        hipLaunchKernelGGL((k_mx_few<T, 1, true>), grid, block, few_lds(args.n, args.segs), s, args);
+    else if (args.n <= 16)
+        hipLaunchKernelGGL((k_mx_few<T, 1, false>), grid, block, 0, s, args);
+    else if (args.n <= 32)
+        hipLaunchKernelGGL((k_mx_few<T, 2, false>), grid, block, 0, s, args);
+    else if (args.n <= 48)
+        hipLaunchKernelGGL((k_mx_few<T, 3, false>), grid, block, 0, s, args);
+    else
+        hipLaunchKernelGGL((k_mx_few<T, 4, false>), grid, block, 0, s, args);
+    return check_launch("microscaled product");
+}
+
+template <typename T, int WN, int WO, int TN, int TO>
+static int launch_tile(const MxArgs &args, hipStream_t s) {
+    constexpr int BN = 32 * WN * TN, BO = 32 * WO * TO, LDS = 2 * (BN + BO) * SEG_BYTES;
+    const i64 tiles = (args.n + BN - 1) / BN * ((args.o + BO - 1) / BO);
+    if (tiles > i64(1) << 30) return fail(MF_E_UNSUPPORTED, "product too large");
+    auto kernel = k_mx_tile<T, WN, WO, TN, TO>;
+    if (LDS > 64 << 10) {
+        const hipError_t e = hipFuncSetAttribute(
+            reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return fail(MF_E_RESOURCE, "LDS of a product: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3(unsigned(tiles)), dim3(64 * WN * WO), LDS, s, args);
+    return check_launch("microscaled product");
+}
+
+template <typename T> static int launch_tiles(const MxArgs &args, hipStream_t s) {
+    // The largest tile of which every compute unit gets one (us, 64 x 64 / 128 x 128 / 128 x 256):
+    // 2048 x 11008 x 4096 97 / 64 / 62, 2048 x 4096 x 11008 101 / 82 / 77, 300 x 4096 x 4096
+    // 12.6 / 18 / 23, 777 x 1500 x 1111 6.1 / 9.5 / 11.8.
+    const auto tiles = [&](i64 bn, i64 bo) { return (args.n + bn - 1) / bn * ((args.o + bo - 1) / bo); };
+    if (tiles(128, 256) >= 256) return launch_tile<T, 2, 4, 2, 2>(args, s);
+    if (tiles(128, 128) >= 256) return launch_tile<T, 2, 2, 2, 2>(args, s);
+    return launch_tile<T, 2, 2, 1, 1>(args, s);
 }
 
 }  // namespace mf
@@ -455,19 +807,7 @@ extern "C" {
 
 int mf_mx_quantize(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, uint8_t *codes,
                    uint8_t *scales, void *stream) {
-    if (!x || !codes || !scales || !known_type(type) || !sizes_ok(n, k) || (n > 1 && ldx < k) ||
-        !aligned(codes, 16) || !aligned(scales, 8))
-        return fail(MF_E_INVALID, "invalid microscaled quantization arguments");
-    const i64 units = segments(k) * 32;
-    const int lanes = row_lanes(units);
-    return with_type(type, [&](auto zero) {
-        using T = decltype(zero);
-        const bool vec = aligned(x, 16) && (n == 1 || ldx % PIECE<T> == 0);
-        hipLaunchKernelGGL(k_mx_quantize<T>, row_grid(units, n, lanes), dim3(256), 0,
-                           static_cast<hipStream_t>(stream), static_cast<const T *>(x), n, k, ldx,
-                           vec, lanes, codes, scales);
-        return check_launch("microscaled quantization");
-    });
+    return launch_quantize(x, type, n, k, ldx, false, codes, scales, static_cast<hipStream_t>(stream));
 }
 
 int mf_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, void *out,
@@ -487,70 +827,97 @@ int mf_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int
     });
 }
 
+int mf_mx_linear_sizes(int32_t type, int64_t n, int64_t k, int64_t o, int32_t keep, int64_t *codes,
+                       int64_t *workspace) {
+    if (!codes || !workspace || !known_type(type) || !product_ok(n, k, o))
+        return fail(MF_E_INVALID, "invalid microscaled product sizes");
+    const ProductPlan plan = plan_product(n, k, keep);
+    *codes = plan.quantize ? n * segments(k) * SEG_BYTES : 0;
+    *workspace = plan.few ? 0 : o * segments(k) * SEG_SCALES;
+    return MF_OK;
+}
+
 int mf_mx_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx,
                  const uint8_t *wcodes, const uint8_t *wscales, int64_t o, const void *bias,
-                 uint8_t *xcodes, uint8_t *xscales, void *out, void *stream) {
-    if (!wcodes || !wscales || !out || o < 1 || o >= MOST || !aligned(wcodes, 16) ||
-        !aligned(wscales, 8))
+                 int32_t keep, uint8_t *xcodes, uint8_t *xscales, void *out, void *workspace,
+                 int64_t bytes, void *stream) {
+    if (!x || !known_type(type) || !product_ok(n, k, o) || (n > 1 && ldx < k) || !wcodes || !wscales ||
+        !out || !aligned(wcodes, 16) || !aligned(wscales, 8))
         return fail(MF_E_INVALID, "invalid microscaled product arguments");
-    const int status = mf_mx_quantize(x, type, n, k, ldx, xcodes, xscales, stream);
-    if (status) return status;
-    const MxArgs args{xcodes, xscales, wcodes, wscales, bias, out, n, o, segments(k)};
-    if ((n + 63) / 64 > 65535) return fail(MF_E_UNSUPPORTED, "too many rows of a product");
-    const dim3 grid(unsigned((o + 63) / 64), unsigned((n + 63) / 64));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const ProductPlan plan = plan_product(n, k, keep);
+    if (plan.quantize) {
+        const int status = launch_quantize(x, type, n, k, ldx, true, xcodes, xscales, s);
+        if (status) return status;
+    }
+    MxArgs args{};
+    args.xc = xcodes;
+    args.xs = xscales;
+    args.wc = wcodes;
+    args.ws = wscales;
+    args.x = x;
+    args.ldx = ldx;
+    args.k = k;
+    args.bias = bias;
+    args.out = out;
+    args.n = n;
+    args.o = o;
+    args.segs = segments(k);
+    if (!plan.few) {
+        if (!workspace || bytes < o * args.segs * SEG_SCALES || !aligned(workspace, 8))
+            return fail(MF_E_INVALID, "product workspace is missing, unaligned or too small");
+        hipLaunchKernelGGL(k_mx_turn_scales, dim3(unsigned((o + 255) / 256), unsigned(args.segs)),
+                           dim3(256), 0, s, reinterpret_cast<const v2u *>(wscales), o, args.segs,
+                           static_cast<v2u *>(workspace));
+        args.ws = static_cast<const u8 *>(workspace);
+    }
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL(k_mx_mm<T>, grid, dim3(256), 0, static_cast<hipStream_t>(stream), args);
-        return check_launch("microscaled product");
+        args.vec = aligned(x, 16) && (n == 1 || ldx % PIECE<T> == 0);
+        return plan.few ? launch_few<T>(args, plan, s) : launch_tiles<T>(args, s);
     });
 }
 
-int mf_mx_grad_workspace(int32_t type, int64_t n, int64_t o, int64_t *bytes) {
-    if (!bytes || !known_type(type) || !sizes_ok(n, o))
+int mf_mx_grad_workspace(int32_t type, int64_t n, int64_t k, int64_t o, int64_t *bytes) {
+    if (!bytes || !known_type(type) || !grad_ok(n, k, o))
         return fail(MF_E_INVALID, "invalid gradient workspace arguments");
     const i64 sums = (n + SUM_ROWS - 1) / SUM_ROWS * o * 4;
-    *bytes = std::max(terms_bytes(type, n, o), sums);
+    *bytes = std::max(grad_bytes(type, n, o, std::max(n, o), k), sums);
     return MF_OK;
 }
 
 int mf_mx_grad_input(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
                      const uint8_t *wcodes, const uint8_t *wscales, int64_t k, void *dx,
                      void *workspace, int64_t bytes, void *stream) {
-    if (!dy || !wcodes || !wscales || !dx || !known_type(type) || !sizes_ok(n, o) || !sizes_ok(n, k) ||
+    if (!dy || !wcodes || !wscales || !dx || !known_type(type) || !grad_ok(n, k, o) ||
         (n > 1 && ldy < o) || !aligned(wcodes, 16) || !aligned(wscales, 8))
         return fail(MF_E_INVALID, "invalid input gradient arguments");
     hipStream_t s = static_cast<hipStream_t>(stream);
     GradArgs args{};
     const int status = make_terms(dy, type, n, o, ldy, false, workspace, bytes, s, args);
     if (status) return status;
-    args.codes = wcodes;
-    args.scales = wscales;
-    args.segs = segments(k);
     args.rows = n;
     args.cols = k;
     args.depth = o;
     args.out = dx;
-    return launch_grad<false>(args, type, s);
+    return launch_grad<false>(args, type, n, o, wcodes, wscales, workspace, bytes, s);
 }
 
 int mf_mx_grad_weight(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
                       const uint8_t *xcodes, const uint8_t *xscales, int64_t k, void *dw,
                       void *workspace, int64_t bytes, void *stream) {
-    if (!dy || !xcodes || !xscales || !dw || !known_type(type) || !sizes_ok(n, o) || !sizes_ok(n, k) ||
+    if (!dy || !xcodes || !xscales || !dw || !known_type(type) || !grad_ok(n, k, o) ||
         (n > 1 && ldy < o) || !aligned(xcodes, 16) || !aligned(xscales, 8))
         return fail(MF_E_INVALID, "invalid weight gradient arguments");
     hipStream_t s = static_cast<hipStream_t>(stream);
     GradArgs args{};
     const int status = make_terms(dy, type, n, o, ldy, true, workspace, bytes, s, args);
     if (status) return status;
-    args.codes = xcodes;
-    args.scales = xscales;
-    args.segs = segments(k);
     args.rows = o;
     args.cols = k;
     args.depth = n;
     args.out = dw;
-    return launch_grad<true>(args, type, s);
+    return launch_grad<true>(args, type, n, o, xcodes, xscales, workspace, bytes, s);
 }
 
 int mf_mx_grad_bias(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy, void *db,

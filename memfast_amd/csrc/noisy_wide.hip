@@ -71,17 +71,6 @@ __device__ __forceinline__ v8h_w digits_magic(uint4 c, int shift, u32 mask2, u32
     return __builtin_bit_cast(v8h_w, make_uint4(o[0], o[1], o[2], o[3]));
 }
 
-// One 1 KiB LDS DMA: lane l's 16 bytes at src go to lds_base + 16 * l.  Issued
-// as inline assembly so that the compiler's wait-count analysis does not track
-// it (it would otherwise wait for it at the next loop header); the kernel waits
-// for it explicitly (s_waitcnt vmcnt(0) and a barrier) before reading the data.
-__device__ __forceinline__ void lds_dma_16(const void *src, u32 lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, off"
-                 :
-                 : "v"(src), "s"(lds_base)
-                 : "memory", "m0");
-}
-
 // After an explicit s_waitcnt vmcnt(0): re-define the loaded registers so the
 // compiler's wait-count analysis no longer sees a load pending on them (it
 // would otherwise flush vmcnt at the next loop header, where the next read's

@@ -202,8 +202,11 @@ SIGNATURES = {
                            ct.c_int),
     "mf_mx_quantize": ([_P, _I32, _I64, _I64, _I64, _P, _P, _P], ct.c_int),
     "mf_mx_dequantize": ([_P, _P, _I64, _I64, _P, _I32, _P], ct.c_int),
-    "mf_mx_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _P], ct.c_int),
-    "mf_mx_grad_workspace": ([_I32, _I64, _I64, ct.POINTER(_I64)], ct.c_int),
+    "mf_mx_linear_sizes": ([_I32, _I64, _I64, _I64, _I32, ct.POINTER(_I64), ct.POINTER(_I64)],
+                           ct.c_int),
+    "mf_mx_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P, _P, _P, _I64, _P],
+                     ct.c_int),
+    "mf_mx_grad_workspace": ([_I32, _I64, _I64, _I64, ct.POINTER(_I64)], ct.c_int),
     "mf_mx_grad_input": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P], ct.c_int),
     "mf_mx_grad_weight": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P], ct.c_int),
     "mf_mx_grad_bias": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P], ct.c_int),
@@ -1473,24 +1476,37 @@ def mx_dequantize(codes, scales, k, dtype):
     return out
 
 
-def mx_linear(x, codes, scales, bias):
-    """``Q(x) W^T + bias`` [n, o] (mf_mx_linear) and Q(x)'s codes and scales."""
-    require_device(x)
+@lru_cache(maxsize=4096)
+def _mx_linear_sizes(kind, n, k, o, keep):
+    codes, work = _I64(), _I64()
+    check(library().mf_mx_linear_sizes(kind, n, k, o, keep, ct.byref(codes), ct.byref(work)),
+          "microscaled product")
+    return codes.value, work.value
+
+
+def mx_linear(x, codes, scales, bias, keep):
+    """``Q(x) W^T + bias`` [n, o] (mf_mx_linear); with ``keep`` also the block of Q(x)'s codes
+    [n, 128 S] and scales [S, n, 8]."""
     n, k = x.shape
-    o = codes.shape[0]
-    xcodes, xscales = mx_empty(n, k, x.device)
+    o, kind = codes.shape[0], FLOAT_TYPES[x.dtype]
+    size, work = _mx_linear_sizes(kind, n, k, o, keep)
+    # One allocation: the codes, their scales (8 bytes for 128 of codes) and the workspace.
+    held = size + size // 16
+    block = torch.empty(held + work, dtype=torch.uint8, device=x.device) if held + work else None
+    base = block.data_ptr() if held + work else 0
     out = torch.empty((n, o), dtype=x.dtype, device=x.device)
     with _on(x.device):
-        check(library().mf_mx_linear(_ptr(x), FLOAT_TYPES[x.dtype], n, k, x.stride(0), _ptr(codes),
-                                     _ptr(scales), o, _ptr(bias), _ptr(xcodes), _ptr(xscales),
-                                     _ptr(out), _stream(x.device)), "microscaled product")
-    return out, xcodes, xscales
+        check(library().mf_mx_linear(
+            _ptr(x), kind, n, k, x.stride(0), _ptr(codes), _ptr(scales), o, _ptr(bias), keep,
+            base if size else None, base + size if size else None, _ptr(out),
+            base + held if work else None, work, _stream(x.device)), "microscaled product")
+    return out, block if keep else None
 
 
-def mx_grad_workspace(dy):
+def mx_grad_workspace(dy, k):
     """The workspace that the gradients of ``dy`` [n, o] share."""
     size = _I64()
-    check(library().mf_mx_grad_workspace(FLOAT_TYPES[dy.dtype], dy.shape[0], dy.shape[1],
+    check(library().mf_mx_grad_workspace(FLOAT_TYPES[dy.dtype], dy.shape[0], k, dy.shape[1],
                                          ct.byref(size)), "microscaled gradient workspace")
     return torch.empty(size.value, dtype=torch.uint8, device=dy.device)
 
@@ -1507,14 +1523,15 @@ def mx_grad_input(dy, codes, scales, k, workspace):
     return dx
 
 
-def mx_grad_weight(dy, xcodes, xscales, k, workspace):
-    """``dy^T Q(x)`` [o, k] (mf_mx_grad_weight)."""
+def mx_grad_weight(dy, block, k, workspace):
+    """``dy^T Q(x)`` [o, k] (mf_mx_grad_weight) for the ``block`` that ``mx_linear`` kept."""
     n, o = dy.shape
     dw = torch.empty((o, k), dtype=dy.dtype, device=dy.device)
+    codes = n * -(-k // MX_SEGMENT) * MX_SEGMENT_BYTES
     with _on(dy.device):
         check(library().mf_mx_grad_weight(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0),
-                                          _ptr(xcodes), _ptr(xscales), k, _ptr(dw), _ptr(workspace),
-                                          workspace.numel(), _stream(dy.device)),
+                                          block.data_ptr(), block.data_ptr() + codes, k, _ptr(dw),
+                                          _ptr(workspace), workspace.numel(), _stream(dy.device)),
               "microscaled weight gradient")
     return dw
 

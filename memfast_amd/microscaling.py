@@ -91,24 +91,23 @@ class _MXLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, codes, scales):
-        y, xcodes, xscales = hip.mx_linear(x, codes, scales, bias)
         keep = ctx.needs_input_grad
+        y, block = hip.mx_linear(x, codes, scales, bias, keep[1])
         ctx.width = x.shape[1]
-        ctx.save_for_backward(*((codes, scales) if keep[0] else (None, None)),
-                              *((xcodes, xscales) if keep[1] else (None, None)))
+        ctx.save_for_backward(*((codes, scales) if keep[0] else (None, None)), block)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        codes, scales, xcodes, xscales = ctx.saved_tensors
+        codes, scales, block = ctx.saved_tensors
         dy = hip.rows_of(dy)
-        work = hip.mx_grad_workspace(dy)
+        work = hip.mx_grad_workspace(dy, ctx.width)
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             dx = hip.mx_grad_input(dy, codes, scales, ctx.width, work)
         if ctx.needs_input_grad[1]:
-            dw = hip.mx_grad_weight(dy, xcodes, xscales, ctx.width, work)
+            dw = hip.mx_grad_weight(dy, block, ctx.width, work)
         if ctx.needs_input_grad[2]:
             db = hip.mx_grad_bias(dy, work)
         return dx, dw, db, None, None
