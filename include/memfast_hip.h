@@ -607,17 +607,21 @@ enum { MF_SUM_NONE = 0, MF_SUM_SUM = 1, MF_SUM_MEAN = 2 };
  * A row with an index outside -1 .. v - 1 or a repeated one has a NaN loss and gradient; a row without
  * any entry or tail, and one whose weight is 0 (whatever its logits), has neither.  Unless reduction
  * is MF_SUM_NONE, *loss = sum(weight * row_loss) (MF_SUM_MEAN: over sum(weight), 0 if that is 0).
- * ref [n], coef [n], entry_grad [n, k] and *norm are what mf_distill_grad needs. */
+ * ref [n], coef [n], entry_grad [n, k] and *norm are what mf_distill_grad needs.  grad [n, v] (or NULL;
+ * not with MF_SUM_NONE) receives the gradient for an incoming gradient of 1, while the logits are in
+ * the cache. */
 int mf_distill_loss(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld,
                     const void *values, int32_t values_type, const int64_t *indices,
                     const float *tail, int64_t k, float temperature, const float *weight,
-                    int32_t reduction, float *row_loss, float *ref, float *coef, float *entry_grad, float *loss, float *norm,
-                    void *stream);
-/* grad [n, v] of the logits: weight * norm * incoming[r * incoming_step] times the row loss's. */
+                    int32_t reduction, float *row_loss, float *ref, float *coef, float *entry_grad,
+                    float *loss, float *norm, void *grad, void *stream);
+/* grad [n, v] of the logits: weight * norm * incoming[r * incoming_step] times the row loss's.
+ * unless_one (incoming_step 0): grad holds the gradient for an incoming 1, so that one leaves it. */
 int mf_distill_grad(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld,
                     const int64_t *indices, int64_t k, float temperature, const float *weight,
                     const float *ref, const float *coef, const float *entry_grad, const float *norm,
-                    const float *incoming, int64_t incoming_step, void *grad, void *stream);
+                    const float *incoming, int64_t incoming_step, int32_t unless_one, void *grad,
+                    void *stream);
 
 #ifdef __cplusplus
 }

@@ -69,39 +69,89 @@ template <int WAVES> __device__ float block_sum(float v, float *scratch) {
 }
 
 // A row in 16-byte pieces at 16-byte addresses: piece i holds the classes i * P - off to
-// i * P - off + P - 1, the first and last pieces fewer where the row starts or ends inside them.
+// i * P - off + P - 1; pieces first to last - 1 are whole, and the one before or after them, where the row
+// starts or ends inside one, is read class by class. A row has at most 2^20 classes.
 template <typename T> struct Row {
+    static constexpr int P = PIECE<T>;
     const T *data;
-    i64 v;
-    int off;
-    i64 pieces;
-    __device__ __forceinline__ Row(const T *p, i64 classes) : data(p), v(classes) {
+    int v, off, pieces, first, last;
+    __device__ __forceinline__ Row(const T *p, i64 classes) : data(p), v(int(classes)) {
         off = int(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T));
-        pieces = (off + v + PIECE<T> - 1) / PIECE<T>;
+        pieces = (off + v + P - 1) / P;
+        first = off ? 1 : 0;
+        last = (off + v) / P;
     }
-    __device__ __forceinline__ bool whole(i64 i) const {
-        return i * PIECE<T> >= off && (i + 1) * PIECE<T> <= off + v;
+    // A whole piece's address: one 32-bit offset from the row's.
+    __device__ __forceinline__ v4u whole(int i) const {
+        return *reinterpret_cast<const v4u *>(reinterpret_cast<const char *>(data - off) + i * 16);
     }
-    // The piece's values, `fill` outside the row.
-    __device__ __forceinline__ void load(i64 i, float fill, float (&x)[PIECE<T>]) const {
-        const i64 first = i * PIECE<T> - off;
-        if (whole(i)) {
-            const Piece<T> piece = *reinterpret_cast<const Piece<T> *>(data + first);
+    // Any piece, `fill` outside the row.
+    __device__ __forceinline__ v4u piece(int i, T fill) const {
+        if (i >= first && i < last) return whole(i);
+        Piece<T> part;
 #pragma unroll
-            for (int j = 0; j < PIECE<T>; ++j) x[j] = float(piece.v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < PIECE<T>; ++j)
-                x[j] = first + j >= 0 && first + j < v ? float(data[first + j]) : fill;
+        for (int j = 0; j < P; ++j) {
+            const int index = i * P - off + j;
+            part.v[j] = index >= 0 && index < v ? data[index] : fill;
         }
+        return __builtin_bit_cast(v4u, part);
     }
 };
 
+template <typename T> __device__ __forceinline__ void unpack(v4u raw, float (&x)[PIECE<T>]) {
+    const Piece<T> p = __builtin_bit_cast(Piece<T>, raw);
+#pragma unroll
+    for (int j = 0; j < PIECE<T>; ++j) x[j] = float(p.v[j]);
+}
+
+// Calls f(i, values) for this thread's pieces from `start` on. Four loads are in flight: with one, a
+// compute unit's waves keep too few bytes under way to fill the memory's latency. Pieces that are not
+// whole come last.
+template <int THREADS, typename T, typename F>
+__device__ __forceinline__ void for_pieces(const Row<T> &row, int start, float fill, F f) {
+    constexpr int LOADS = 4;
+    float x[PIECE<T>];
+    int i = max(start, row.first) + int(threadIdx.x);
+    for (; i + (LOADS - 1) * THREADS < row.last; i += LOADS * THREADS) {
+        v4u raw[LOADS];
+#pragma unroll
+        for (int t = 0; t < LOADS; ++t) raw[t] = row.whole(i + t * THREADS);
+#pragma unroll
+        for (int t = 0; t < LOADS; ++t) {
+            unpack<T>(raw[t], x);
+            f(i + t * THREADS, x);
+        }
+    }
+    for (; i < row.last; i += THREADS) {
+        unpack<T>(row.whole(i), x);
+        f(i, x);
+    }
+    const int side = threadIdx.x == 0 ? 0 : row.pieces - 1;
+    if (threadIdx.x < 2 && side >= start && (side < row.first || side >= row.last) &&
+        (threadIdx.x == 0 || row.pieces > 1)) {
+        unpack<T>(row.piece(side, T(fill)), x);
+        f(side, x);
+    }
+}
+
+// The largest of a piece. (v_max3 as it is: fmaxf would first quiet every operand.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+template <int P> __device__ __forceinline__ float largest(const float (&x)[P], float top) {
+#pragma unroll
+    for (int j = 0; j < P; j += 2) top = max3(top, x[j], x[j + 1]);
+    return top;
+}
+
 // One bit for each class, in the order of the row's pieces.
 template <typename T>
-__device__ __forceinline__ u32 piece_bits(const u32 *bits, i64 i) {
-    constexpr int P = PIECE<T>;
-    return bits[i * P / 32] >> (i * P % 32) & ((1u << P) - 1u);
+__device__ __forceinline__ u32 piece_bits(const u32 *bits, int i) {
+    constexpr u32 P = PIECE<T>;
+    return bits[u32(i) * P / 32] >> (u32(i) * P % 32) & ((1u << P) - 1u);
 }
 
 struct DistillArgs {
@@ -117,6 +167,9 @@ struct DistillArgs {
     float *ref, *coef;       // [n]: a class outside the entries has the gradient
                              // exp2((s - ref) c) * coef (times T, weight and the incoming one)
     float *entry_grad;       // [n, k]: q - p
+    const float *norm;       // with a gradient: what the rows' weights are multiplied by
+    float inverse_n;         // the same where norm is nullptr
+    void *grad;              // [n, v]
 };
 
 // p d - p + q with d = log(p / q), as p (d + exp(-d) - 1) where that stays in range. d is formed
@@ -150,8 +203,46 @@ __device__ __forceinline__ bool mark_entries(const i64 *indices, i64 k, i64 v, i
     return __syncthreads_or(bad);
 }
 
-// One workgroup a row: one pass over the row for the classes outside the entries.
-template <typename T, int WAVES>
+// Writes a piece of the gradient; entries are left to the threads that hold them. `vec`: grad's pieces
+// lie at 16-byte addresses as the row's do.
+template <typename T>
+__device__ __forceinline__ void store_rest(T *grad, const Row<T> &row, int i, u32 marked, bool vec,
+                                           const float (&x)[PIECE<T>]) {
+    Piece<T> piece;
+#pragma unroll
+    for (int j = 0; j < PIECE<T>; ++j) piece.v[j] = T(x[j]);
+    if (marked == 0 && vec && i >= row.first && i < row.last) {
+        *reinterpret_cast<v4u *>(reinterpret_cast<char *>(grad - row.off) + i * 16) =
+            __builtin_bit_cast(v4u, piece);
+    } else {
+        const int first = i * PIECE<T> - row.off;
+#pragma unroll
+        for (int j = 0; j < PIECE<T>; ++j)
+            if (first + j >= 0 && first + j < row.v && !(marked >> j & 1u)) grad[first + j] = piece.v[j];
+    }
+}
+
+// The gradient of a row's classes outside its entries.
+template <typename T, int THREADS>
+__device__ __forceinline__ void write_rest(const Row<T> &row, const u32 *bits, float c, float ref,
+                                           float coef, T *grad) {
+    const bool vec = (reinterpret_cast<uintptr_t>(grad - row.off) & 15) == 0;
+    if (coef == 0.0f) {   // nothing flows back, whatever the logits are
+        const float zero[PIECE<T>] = {};
+        for (int i = threadIdx.x; i < row.pieces; i += THREADS)
+            store_rest(grad, row, i, piece_bits<T>(bits, i), vec, zero);
+        return;
+    }
+    for_pieces<THREADS>(row, 0, 0.0f, [&](int i, float (&x)[PIECE<T>]) {
+#pragma unroll
+        for (int j = 0; j < PIECE<T>; ++j) x[j] = power(x[j], ref, c) * coef;
+        store_rest(grad, row, i, piece_bits<T>(bits, i), vec, x);
+    });
+}
+
+// One workgroup a row: one pass over the row for the classes outside the entries, and with GRAD
+// another that writes the gradient for an incoming 1, which finds the row in the cache.
+template <typename T, int WAVES, bool GRAD>
 __global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
     extern __shared__ u32 bits[];
     __shared__ float scratch[2 * WAVES];
@@ -161,6 +252,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
     if (weight == 0.0f) {   // nothing of such a row is read
         for (i64 j = threadIdx.x; j < a.k; j += THREADS) a.entry_grad[r * a.k + j] = 0.0f;
         if (threadIdx.x == 0) a.row_loss[r] = a.ref[r] = a.coef[r] = 0.0f;
+        if (GRAD)
+            for (i64 i = threadIdx.x; i < a.v; i += THREADS) static_cast<T *>(a.grad)[r * a.v + i] = T(0.0f);
         return;
     }
     const T *s = static_cast<const T *>(a.logits) + r * a.ld;
@@ -178,21 +271,21 @@ __global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
                 teacher.add(value_at(a.values, a.values_type, first + j), c);
                 entries.add(float(s[indices[j]]), c);
             }
-    for (i64 i = threadIdx.x; i < row.pieces; i += THREADS) {
-        float x[PIECE<T>];
-        row.load(i, -INFINITY, x);
-        const u32 marked = piece_bits<T>(bits, i);
-        const float old = rest.m;
+    for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, float (&x)[PIECE<T>]) {
+        if (const u32 marked = piece_bits<T>(bits, i)) {
 #pragma unroll
-        for (int j = 0; j < PIECE<T>; ++j) {
-            if (marked >> j & 1u) x[j] = -INFINITY;
-            rest.m = fmaxf(rest.m, x[j]);
+            for (int j = 0; j < PIECE<T>; ++j)
+                if (marked >> j & 1u) x[j] = -INFINITY;
+        }
+        const float top = largest(x, rest.m);
+        if (top > rest.m) {
+            rest.s *= power(rest.m, top, c);
+            rest.m = top;
         }
         const float ref = rest.ref();
-        rest.s *= power(old, ref, c);
 #pragma unroll
         for (int j = 0; j < PIECE<T>; ++j) rest.s += power(x[j], ref, c);
-    }
+    });
     teacher = block_merge<WAVES>(teacher, c, scratch);
     entries = block_merge<WAVES>(entries, c, scratch);
     rest = block_merge<WAVES>(rest, c, scratch);
@@ -222,8 +315,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
         a.entry_grad[r * a.k + j] = grad;
     }
     loss = block_sum<WAVES>(loss, scratch);
-    if (threadIdx.x == 0) {
-        float coef = 0.0f;
+    float coef = 0.0f;
+    {   // the bucket of all other classes, by every thread
         if (bad) {
             loss = coef = NAN;
         } else if (!empty) {
@@ -235,21 +328,33 @@ __global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
             // Without any finite class outside the entries there is nothing to scale.
             coef = rest.s == 0.0f ? (p > 0.0f ? NAN : 0.0f) : scale - p / rest.s;
         }
+    }
+    if (threadIdx.x == 0) {
         a.row_loss[r] = loss * a.temperature * a.temperature;
         a.ref[r] = rest.ref();
         a.coef[r] = coef;
     }
+    if (GRAD) {
+        const float scale = 1.0f * weight * (a.norm ? *a.norm : a.inverse_n) * a.temperature;
+        T *grad = static_cast<T *>(a.grad) + r * a.v;
+        write_rest<T, THREADS>(row, bits, c, rest.ref(), coef * scale, grad);
+        for (i64 j = threadIdx.x; j < a.k; j += THREADS) {   // this thread's own entry_grad
+            const i64 index = indices[j];
+            if (index >= 0 && index < a.v)
+                grad[index] = T(bad ? NAN : scale == 0.0f ? 0.0f : a.entry_grad[r * a.k + j] * scale);
+        }
+    }
 }
 
 // sum(weight * loss) over the rows, divided by sum(weight) where `mean`, in a fixed order, in FP64;
-// norm = 1 / sum(weight) (0 where there is no weight) or 1.
+// norm = 1 / sum(weight) (0 where there is no weight) or 1. Without row_loss the norm alone.
 __global__ __launch_bounds__(256) void k_distill_total(const float *row_loss, const float *weight, i64 n,
                                                        bool mean, float *loss, float *norm) {
     __shared__ double part[2][256];
     double sum = 0.0, weights = 0.0;
     for (i64 r = threadIdx.x; r < n; r += 256) {
         const float w = weight ? weight[r] : 1.0f;
-        sum += double(w) * double(row_loss[r]);
+        if (row_loss) sum += double(w) * double(row_loss[r]);
         weights += w;
     }
     part[0][threadIdx.x] = sum;
@@ -264,7 +369,7 @@ __global__ __launch_bounds__(256) void k_distill_total(const float *row_loss, co
     if (threadIdx.x == 0) {
         const double total = part[1][0];
         const double scale = mean ? (total == 0.0 ? 0.0 : 1.0 / total) : 1.0;
-        *loss = total == 0.0 && mean ? 0.0f : float(part[0][0] * scale);
+        if (row_loss) *loss = total == 0.0 && mean ? 0.0f : float(part[0][0] * scale);
         *norm = float(scale);
     }
 }
@@ -278,32 +383,16 @@ struct DistillGradArgs {
     i64 incoming_step;
     i64 n, v, ld, k;
     float temperature;
+    bool unless_one;          // the gradient for an incoming 1 is there already
     void *grad;               // [n, v]
 };
-
-// Writes a piece of the gradient; entries are left to the threads that hold them.
-template <typename T>
-__device__ __forceinline__ void store_rest(T *grad, const Row<T> &row, i64 i, u32 marked,
-                                           const float (&x)[PIECE<T>]) {
-    const i64 first = i * PIECE<T> - row.off;
-    const bool vec = (reinterpret_cast<uintptr_t>(grad + first) & 15) == 0;
-    if (marked == 0 && vec && row.whole(i)) {
-        Piece<T> piece;
-#pragma unroll
-        for (int j = 0; j < PIECE<T>; ++j) piece.v[j] = T(x[j]);
-        *reinterpret_cast<Piece<T> *>(grad + first) = piece;
-    } else {
-#pragma unroll
-        for (int j = 0; j < PIECE<T>; ++j)
-            if (first + j >= 0 && first + j < row.v && !(marked >> j & 1u)) grad[first + j] = T(x[j]);
-    }
-}
 
 template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_distill_grad(const DistillGradArgs a) {
     extern __shared__ u32 bits[];
     constexpr int THREADS = 64 * WAVES;
     const i64 r = blockIdx.x;
+    if (a.unless_one && *a.incoming == 1.0f) return;
     const Row<T> row(static_cast<const T *>(a.logits) + r * a.ld, a.v);
     T *grad = static_cast<T *>(a.grad) + r * a.v;
     const i64 *indices = a.indices + r * a.k;
@@ -314,19 +403,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_distill_grad(const DistillGradAr
     const float c = LOG2E / a.temperature, ref = a.ref[r], coef = a.coef[r] * scale;
     const bool bad = mark_entries(indices, a.k, a.v, row.off, bits, (row.off + a.v + 31) / 32,
                                   THREADS);
-    for (i64 i = threadIdx.x; i < row.pieces; i += THREADS) {
-        float x[PIECE<T>];
-        if (coef == 0.0f) {   // nothing flows back, whatever the logits are
-#pragma unroll
-            for (int j = 0; j < PIECE<T>; ++j) x[j] = 0.0f;
-        } else {
-            row.load(i, 0.0f, x);
-#pragma unroll
-            for (int j = 0; j < PIECE<T>; ++j)
-                x[j] = power(x[j], ref, c) * coef;
-        }
-        store_rest(grad, row, i, piece_bits<T>(bits, i), x);
-    }
+    write_rest<T, THREADS>(row, bits, c, ref, coef, grad);
     for (i64 j = threadIdx.x; j < a.k; j += THREADS) {
         const i64 index = indices[j];
         if (index >= 0 && index < a.v) {
@@ -347,7 +424,7 @@ __device__ __forceinline__ u32 order_of(float x) {
     return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-__device__ __forceinline__ u64 key_of(float x, i64 index) {
+__device__ __forceinline__ u64 key_of(float x, int index) {
     return u64(order_of(x)) << 32 | (0xffffffffu - u32(index));
 }
 
@@ -361,99 +438,255 @@ struct TopArgs {
     float *tail;          // [n]
 };
 
-// Radix selection of the k-th largest key, eight bits at a time, then the selected keys in order and
-// the others' sum.
-template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_top_select(const TopArgs a) {
-    __shared__ u64 list[MOST_ENTRIES];
-    __shared__ u32 counts[256];
-    __shared__ u32 digit, remaining, found, last;
-    __shared__ float scratch[2 * WAVES];
-    constexpr int THREADS = 64 * WAVES;
-    const i64 r = blockIdx.x;
-    const T *s = static_cast<const T *>(a.logits) + r * a.ld;
-    const Row<T> row(s, a.v);
+constexpr int TOP_LIST = 2048;      // candidates of a row
+
+struct TopShared {
+    u64 list[TOP_LIST];
+    u32 ranks[TOP_LIST];
+    u64 bounds[16];
+    u32 counts[256];
+    u32 digit, remaining, found, last;
+    float scratch[32];
+};
+
+// The value of a key's logit, in FP32; NaN for the largest key.
+__device__ __forceinline__ float value_of(u64 key) {
+    const u32 order = u32(key >> 32);
+    return __uint_as_float(order >> 31 ? order ^ 0x80000000u : ~order);
+}
+
+// Lists a piece's classes from `bound` (of the value `least`) on, and adds the others' exp2(x c + b)
+// to the sum. A NaN that is not listed makes the sum one (with least = -inf every class's key is
+// compared, and a NaN that belongs there is listed).
+template <typename T>
+__device__ __forceinline__ void sift(const Row<T> &row, int i, const float (&x)[PIECE<T>], float least,
+                                     u64 bound, float c, float b, TopShared &sh, float &sum) {
+    constexpr int P = PIECE<T>;
+    if (largest(x, -INFINITY) >= least || i < row.first || i >= row.last) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int index = i * P - row.off + j;
+            if (index < 0 || index >= row.v) continue;
+            const u64 key = key_of(x[j], index);
+            if (key >= bound) {
+                const u32 at = atomicAdd(&sh.found, 1u);
+                if (at < u32(TOP_LIST)) sh.list[at] = key;
+            } else {
+                sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j) sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
+    }
+}
+
+// The smallest selected key by radix selection, eight bits a pass over the row: for rows with
+// more than TOP_LIST candidates.
+template <typename T, int THREADS>
+__device__ u64 exact_bound(const Row<T> &row, int k, TopShared &sh) {
     u64 prefix = 0;
-    if (threadIdx.x == 0) remaining = a.k;
-    int shift = 56;
-    for (;; shift -= 8) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.remaining = k;
+    for (int shift = 56;; shift -= 8) {
         __syncthreads();
-        for (int b = threadIdx.x; b < 256; b += THREADS) counts[b] = 0;
+        for (int b = threadIdx.x; b < 256; b += THREADS) sh.counts[b] = 0;
         __syncthreads();
-        for (i64 i = threadIdx.x; i < row.pieces; i += THREADS) {
-            float x[PIECE<T>];
-            row.load(i, 0.0f, x);
+        for_pieces<THREADS>(row, 0, 0.0f, [&](int i, float (&x)[PIECE<T>]) {
 #pragma unroll
             for (int j = 0; j < PIECE<T>; ++j) {
-                const i64 index = i * PIECE<T> - row.off + j;
+                const int index = i * PIECE<T> - row.off + j;
                 const u64 key = key_of(x[j], index);
-                if (index >= 0 && index < a.v &&
+                if (index >= 0 && index < row.v &&
                     (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8)))
-                    atomicAdd(&counts[key >> shift & 255u], 1u);
+                    atomicAdd(&sh.counts[key >> shift & 255u], 1u);
             }
-        }
+        });
         __syncthreads();
         if (threadIdx.x == 0) {   // the digit that holds the k-th largest
-            u32 left = remaining;
+            u32 left = sh.remaining;
             int d = 255;
-            while (counts[d] < left) left -= counts[d--];
-            digit = d;
-            remaining = left;
-            last = counts[d] == left;
+            while (sh.counts[d] < left) left -= sh.counts[d--];
+            sh.digit = d;
+            sh.remaining = left;
+            sh.last = sh.counts[d] == left;
         }
         __syncthreads();
-        prefix |= u64(digit) << shift;
-        if (last || shift == 0) break;
+        prefix |= u64(sh.digit) << shift;
+        if (sh.last || shift == 0) return prefix;
     }
-    // Every key from prefix on is selected: k of them.
-    int pow2 = 1;
-    while (pow2 < a.k) pow2 <<= 1;
-    for (int j = threadIdx.x; j < pow2; j += THREADS) list[j] = 0;
-    if (threadIdx.x == 0) found = 0;
+}
+
+// Every listed key's rank among the list, its comparisons shared by several threads.
+template <int THREADS> __device__ void rank_list(TopShared &sh, int found) {
+    for (int j = threadIdx.x; j < found; j += THREADS) sh.ranks[j] = 0;
     __syncthreads();
-    const float c = LOG2E / a.temperature;
-    LogSum rest;
-    for (i64 i = threadIdx.x; i < row.pieces; i += THREADS) {
-        float x[PIECE<T>];
-        row.load(i, -INFINITY, x);
+    const int parts = max(1, THREADS / found);
+    const int length = (found + parts - 1) / parts;
+    for (int e = threadIdx.x; e < found * parts; e += THREADS) {
+        const int j = e % found, from = e / found * length, to = min(from + length, found);
+        const u64 key = sh.list[j];
+        u32 above = 0;
+        for (int o = from; o < to; ++o) above += sh.list[o] > key;
+        if (parts == 1)
+            sh.ranks[j] = above;
+        else
+            atomicAdd(&sh.ranks[j], above);
+    }
+    __syncthreads();
+}
+
+// Sorts the list and leaves its first k keys; the others join the sum, in their order, because the
+// order in which they were listed changes from run to run.
+template <int THREADS>
+__device__ void keep_first(TopShared &sh, int k, float c, float b, float &sum) {
+    constexpr int EACH = TOP_LIST / THREADS;
+    const int found = int(sh.found);
+    rank_list<THREADS>(sh, found);
+    u64 keys[EACH];
+    u32 ranks[EACH];
 #pragma unroll
-        for (int j = 0; j < PIECE<T>; ++j) {
-            const i64 index = i * PIECE<T> - row.off + j;
-            if (index < 0 || index >= a.v) continue;
-            const u64 key = key_of(x[j], index);
-            if (key >= prefix) {
-                const u32 at = atomicAdd(&found, 1u);
-                if (at < u32(a.k)) list[at] = key;
-            } else {
-                rest.add(x[j], c);
-            }
-        }
+    for (int e = 0; e < EACH; ++e) {
+        const int j = threadIdx.x + e * THREADS;
+        keys[e] = j < found ? sh.list[j] : 0;
+        ranks[e] = j < found ? sh.ranks[j] : 0;
     }
     __syncthreads();
-    for (int size = 2; size <= pow2; size <<= 1)
-        for (int stride = size >> 1; stride; stride >>= 1) {
-            for (int j = threadIdx.x; j < pow2; j += THREADS) {
-                const int other = j ^ stride;
-                if (other > j) {
-                    const u64 x = list[j], y = list[other];
-                    if ((x < y) == ((j & size) == 0)) {
-                        list[j] = y;
-                        list[other] = x;
-                    }
-                }
-            }
-            __syncthreads();
-        }
-    for (int j = threadIdx.x; j < a.k; j += THREADS) {
-        const i64 index = i64(0xffffffffu - u32(list[j]));
-        a.indices[r * a.k + j] = index;
-        static_cast<T *>(a.values)[r * a.k + j] = s[index];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+        if (int(threadIdx.x) + e * THREADS < found) sh.list[ranks[e]] = keys[e];
+    if (threadIdx.x == 0) sh.found = min(found, k);
+    __syncthreads();
+    for (int j = k + threadIdx.x; j < found; j += THREADS)
+        sum += __builtin_amdgcn_exp2f(fmaf(value_of(sh.list[j]), c, b));
+    __syncthreads();
+}
+
+// One workgroup a row, one pass over it. Its first stretch (ITEMS pieces a thread, in registers) gives a
+// bound: of the largest classes of a wave's lanes the ceil(k / WAVES)-th largest, the smallest over
+// the waves; at least k classes lie at or above it. Those are listed, and the k-th of the list
+// is the bound for the rest of the row, of which it lists about k / (stretch) a class. A listed
+// class's rank is its place in the output. Keys hold the index, so ties do not lengthen the list; a
+// row that rises all along does, and takes exact_bound's passes over the cached row.
+// All classes that are not selected are summed relative to the first bound; where that overflows
+// or underflows, or the row holds a NaN, once more relative to their own maximum.
+template <typename T, int WAVES, int ITEMS>
+__global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
+    __shared__ TopShared sh;
+    constexpr int THREADS = 64 * WAVES, P = PIECE<T>;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const i64 r = blockIdx.x;
+    const Row<T> row(static_cast<const T *>(a.logits) + r * a.ld, a.v);
+    const float c = LOG2E / a.temperature;
+    if (threadIdx.x == 0) sh.found = 0;
+
+    // Kept packed: the empty asm keeps the compiler from holding the values unpacked as well, which
+    // takes twice the registers.
+    v4u first[ITEMS];
+    auto values = [&](int t, float (&x)[P]) {
+        asm volatile("" : "+v"(first[t]));
+        unpack<T>(first[t], x);
+    };
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) {
+        const int i = threadIdx.x + t * THREADS;
+        if (i < row.pieces) first[t] = row.piece(i, T(-INFINITY));
     }
-    rest = block_merge<WAVES>(rest, c, scratch);
-    if (threadIdx.x == 0)
-        a.tail[r] = rest.m == -INFINITY && rest.s == 0.0f
-                        ? -INFINITY
-                        : rest.ref() / a.temperature + __builtin_amdgcn_logf(rest.s) * LN2;
+    // The largest key of this thread (the first of equal ones), 0 for none.
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t)
+        if (int(threadIdx.x) + t * THREADS < row.pieces) {
+            float x[P];
+            values(t, x);
+            top = largest(x, top);
+        }
+    int at = -1;
+#pragma unroll
+    for (int t = ITEMS - 1; t >= 0; --t) {
+        const int i = threadIdx.x + t * THREADS;
+        if (i < row.pieces) {
+            float x[P];
+            values(t, x);
+            int where = -1;
+#pragma unroll
+            for (int j = P - 1; j >= 0; --j) where = x[j] == top ? j : where;
+            const int index = i * P - row.off + where;
+            if (where >= 0 && index >= 0 && index < row.v) at = index;
+        }
+    }
+    u64 best = at < 0 ? 0 : key_of(top, at);
+    for (int size = 2; size <= 64; size <<= 1)      // lanes in descending order
+        for (int stride = size >> 1; stride; stride >>= 1) {
+            const u64 other = __shfl_xor((unsigned long long)best, stride);
+            const bool larger = ((lane & size) == 0) == ((lane & stride) == 0);
+            best = larger ? max(best, other) : min(best, other);
+        }
+    const u64 mine = __shfl((unsigned long long)best, (a.k + WAVES - 1) / WAVES - 1);
+    if (lane == 0) sh.bounds[wave] = mine;
+    __syncthreads();
+    u64 bound = sh.bounds[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) bound = min(bound, sh.bounds[w]);
+
+    float least = bound ? value_of(bound) : -INFINITY;      // 0 lists everything
+    const float b = least == -INFINITY ? 0.0f : -least * c;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) {
+        const int i = threadIdx.x + t * THREADS;
+        if (i < row.pieces) {
+            float x[P];
+            values(t, x);
+            sift(row, i, x, least, bound, c, b, sh, sum);
+        }
+    }
+    // A NaN is found by the sum: it may be among the largest, which comparisons of values miss.
+    bool exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
+    if (!exact && row.pieces > ITEMS * THREADS) {
+        keep_first<THREADS>(sh, a.k, c, b, sum);
+        bound = sh.list[a.k - 1];
+        least = value_of(bound);
+        for_pieces<THREADS>(row, ITEMS * THREADS, -INFINITY, [&](int i, float (&x)[P]) {
+            sift(row, i, x, least, bound, c, b, sh, sum);
+        });
+        exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
+    }
+    if (exact) {
+        bound = exact_bound<T, THREADS>(row, a.k, sh);      // lists k classes
+        if (threadIdx.x == 0) sh.found = 0;
+        __syncthreads();
+        sum = 0.0f;
+        for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, float (&x)[P]) {
+            sift(row, i, x, -INFINITY, bound, c, b, sh, sum);
+        });
+        __syncthreads();
+    }
+    keep_first<THREADS>(sh, a.k, c, b, sum);
+    for (int j = threadIdx.x; j < a.k; j += THREADS) {
+        const int index = int(0xffffffffu - u32(sh.list[j]));
+        a.indices[r * a.k + j] = index;
+        static_cast<T *>(a.values)[r * a.k + j] = row.data[index];
+    }
+
+    sum = block_sum<WAVES>(sum, sh.scratch);
+    float tail = (__builtin_amdgcn_logf(sum) - b) * LN2;
+    if (a.k < a.v && !(sum > 0x1p-60f && sum < 0x1p60f && fabsf(b) < 0x1p60f)) {
+        const u64 last = sh.list[a.k - 1];
+        LogSum rest;
+        for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, float (&x)[P]) {
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const int index = i * P - row.off + j;
+                if (index >= 0 && index < row.v && key_of(x[j], index) < last) rest.add(x[j], c);
+            }
+        });
+        rest = block_merge<WAVES>(rest, c, sh.scratch);
+        tail = rest.m == -INFINITY && rest.s == 0.0f
+                   ? -INFINITY
+                   : rest.ref() / a.temperature + __builtin_amdgcn_logf(rest.s) * LN2;
+    }
+    if (threadIdx.x == 0) a.tail[r] = a.k < a.v ? tail : -INFINITY;
 }
 
 static int check_rows(const char *what, const void *logits, int32_t type, i64 n, i64 v, i64 ld, i64 k,
@@ -495,8 +728,17 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
     const TopArgs args{logits, n, v, ld, int(k), temperature, values, indices, tail};
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        hipLaunchKernelGGL((k_top_select<T, 16>), dim3(unsigned(n)), dim3(1024), 0,
-                           static_cast<hipStream_t>(stream), args);
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        // A wave needs a class in every lane for its bound, and no more than its 64. Where the
+        // rows fill the chip several times over, eight waves leave two workgroups to a compute unit.
+        const i64 pieces = v / PIECE<T>;
+        const auto fits = [&](int waves) { return pieces >= 64 * waves && k <= 64 * waves; };
+        if (n >= 512 && fits(8))
+            hipLaunchKernelGGL((k_top<T, 8, 16>), dim3(unsigned(n)), dim3(512), 0, s, args);
+        else if (fits(16) || k > 256)
+            hipLaunchKernelGGL((k_top<T, 16, 8>), dim3(unsigned(n)), dim3(1024), 0, s, args);
+        else
+            hipLaunchKernelGGL((k_top<T, 4, 8>), dim3(unsigned(n)), dim3(256), 0, s, args);
         return check_launch("top logits");
     });
 }
@@ -504,41 +746,50 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
 int mf_distill_loss(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld,
                     const void *values, int32_t values_type, const int64_t *indices,
                     const float *tail, int64_t k, float temperature, const float *weight,
-                    int32_t reduction, float *row_loss,
-                    float *ref, float *coef, float *entry_grad, float *loss, float *norm,
-                    void *stream) {
+                    int32_t reduction, float *row_loss, float *ref, float *coef, float *entry_grad,
+                    float *loss, float *norm, void *grad, void *stream) {
     const int status = check_rows("distillation", logits, type, n, v, ld, k, temperature);
     if (status) return status;
     if (!values || !known_type(values_type) || !indices || !row_loss || !ref || !coef || !entry_grad || reduction < 0 ||
-        reduction > 2 || (reduction != MF_SUM_NONE && (!loss || !norm)))
+        reduction > 2 || (reduction != MF_SUM_NONE && (!loss || !norm)) ||
+        (reduction == MF_SUM_NONE && grad))
         return fail(MF_E_INVALID, "invalid distillation arguments");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const DistillArgs args{logits, values, values_type, indices, tail, weight, n, v, ld, k,
-                           temperature, row_loss, ref, coef, entry_grad};
+    DistillArgs args{logits, values, values_type, indices, tail, weight, n, v, ld, k,
+                     temperature, row_loss, ref, coef, entry_grad};
+    const bool mean = reduction == MF_SUM_MEAN;
+    args.grad = grad;
+    args.inverse_n = mean ? float(1.0 / double(n)) : 1.0f;
+    if (grad && weight && mean) {
+        args.norm = norm;
+        hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(256), 0, s, nullptr, weight, n, true,
+                           nullptr, norm);
+    }
     const int launched = with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        const int lds = allow_lds(k_distill<T, ROW_WAVES>, mark_bytes(v));
+        auto kernel = grad ? k_distill<T, ROW_WAVES, true> : k_distill<T, ROW_WAVES, false>;
+        const int lds = allow_lds(kernel, mark_bytes(v));
         if (lds) return lds;
-        hipLaunchKernelGGL((k_distill<T, ROW_WAVES>), dim3(unsigned(n)), dim3(64 * ROW_WAVES),
-                           mark_bytes(v), s, args);
+        hipLaunchKernelGGL(kernel, dim3(unsigned(n)), dim3(64 * ROW_WAVES), mark_bytes(v), s, args);
         return check_launch("distillation loss");
     });
     if (launched || reduction == MF_SUM_NONE) return launched;
-    hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(256), 0, s, row_loss, weight, n,
-                       reduction == MF_SUM_MEAN, loss, norm);
+    hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(256), 0, s, row_loss, weight, n, mean, loss, norm);
     return check_launch("distillation total");
 }
 
 int mf_distill_grad(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld,
                     const int64_t *indices, int64_t k, float temperature, const float *weight,
                     const float *ref, const float *coef, const float *entry_grad, const float *norm,
-                    const float *incoming, int64_t incoming_step, void *grad, void *stream) {
+                    const float *incoming, int64_t incoming_step, int32_t unless_one, void *grad,
+                    void *stream) {
     const int status = check_rows("distillation gradient", logits, type, n, v, ld, k, temperature);
     if (status) return status;
-    if (!indices || !ref || !coef || !entry_grad || !incoming || !grad || incoming_step < 0)
+    if (!indices || !ref || !coef || !entry_grad || !incoming || !grad || incoming_step < 0 ||
+        (unless_one && incoming_step))
         return fail(MF_E_INVALID, "invalid distillation gradient arguments");
     const DistillGradArgs args{logits, indices, weight, ref, coef, entry_grad, norm, incoming,
-                               incoming_step, n, v, ld, k, temperature, grad};
+                               incoming_step, n, v, ld, k, temperature, unless_one != 0, grad};
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
         const int lds = allow_lds(k_distill_grad<T, ROW_WAVES>, mark_bytes(v));

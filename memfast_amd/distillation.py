@@ -58,24 +58,34 @@ def top_logits(logits, k, *, temperature=1.0):
 
 
 class _Distillation(torch.autograd.Function):
+    """A sum or mean computes its gradient with the loss, while a row is in the cache: for an
+    incoming gradient of 1, as a loss that is differentiated itself gets. The first backward hands
+    it out, computed again from the logits where the incoming gradient is another; further ones
+    through the same graph compute their own."""
+
     @staticmethod
     def forward(ctx, logits, values, indices, tail, weight, temperature, reduction):
-        row_loss, total, kept = hip.distill_loss(logits, values, indices, tail, temperature, weight,
-                                                 reduction)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, indices, weight, *kept)
-            ctx.temperature = temperature
-        if reduction != "none":
-            return total
-        return row_loss if weight is None else torch.where(weight == 0, 0.0, weight * row_loss)
+        row_loss, total, stats, grad = hip.distill_loss(
+            logits, values, indices, tail, temperature, weight, reduction, reduction != "none")
+        ctx.save_for_backward(logits, indices, weight, stats)
+        ctx.options, ctx.ready = (temperature, reduction), grad
+        return _weighted(row_loss, weight) if reduction == "none" else total
 
     @staticmethod
     @once_differentiable
     def backward(ctx, incoming):
-        logits, indices, weight, *kept = ctx.saved_tensors
-        grad = hip.distill_grad(logits, indices, ctx.temperature, weight, kept,
-                                incoming.to(torch.float32).contiguous())
-        return (grad,) + (None,) * 6
+        logits, indices, weight, stats = ctx.saved_tensors
+        temperature, reduction = ctx.options
+        ready, ctx.ready = ctx.ready, None
+        if incoming.dtype != torch.float32 or not incoming.is_contiguous():
+            incoming = incoming.to(torch.float32).contiguous()
+        grad = hip.distill_grad(logits, indices, temperature, weight, stats, reduction, incoming,
+                                ready)
+        return grad, None, None, None, None, None, None
+
+
+def _weighted(row_loss, weight):
+    return row_loss if weight is None else torch.where(weight == 0, 0.0, weight * row_loss)
 
 
 def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, weight=None,
@@ -127,14 +137,22 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
         zero = logits.sum(-1).float()
         return zero if reduction == "none" else zero.sum()
 
-    def per_row(value):
-        return None if value is None else value.detach().to(torch.float32).reshape(-1).contiguous()
-
+    rows = hip.rows_of(logits)
     entries = values.detach().reshape(-1, k).contiguous()
-    loss = _Distillation.apply(hip.rows_of(logits), entries,
-                               indices.to(torch.int64).reshape(-1, k).contiguous(), per_row(tail),
-                               per_row(weight), temperature, reduction)
+    indices = indices.reshape(-1, k).to(torch.int64).contiguous()
+    tail, weight = _per_row(tail), _per_row(weight)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        loss = _Distillation.apply(rows, entries, indices, tail, weight, temperature, reduction)
+    else:
+        row_loss, loss, _, _ = hip.distill_loss(rows, entries, indices, tail, temperature, weight,
+                                                reduction, False)
+        if reduction == "none":
+            loss = _weighted(row_loss, weight)
     return loss.reshape(lead) if reduction == "none" else loss
+
+
+def _per_row(value):
+    return None if value is None else value.detach().to(torch.float32).reshape(-1).contiguous()
 
 
 __all__ = ["top_logits", "distillation_loss"]

@@ -212,9 +212,9 @@ SIGNATURES = {
     "mf_mx_grad_bias": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P], ct.c_int),
     "mf_top_logits": ([_P, _I32, _I64, _I64, _I64, _I64, ct.c_float, _P, _P, _P, _P], ct.c_int),
     "mf_distill_loss": ([_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, ct.c_float, _P, _I32,
-                         _P, _P, _P, _P, _P, _P, _P], ct.c_int),
+                         _P, _P, _P, _P, _P, _P, _P, _P], ct.c_int),
     "mf_distill_grad": ([_P, _I32, _I64, _I64, _I64, _P, _I64, ct.c_float, _P, _P, _P, _P, _P, _P,
-                         _I64, _P, _P], ct.c_int),
+                         _I64, _I32, _P, _P], ct.c_int),
     "mf_rng_uniform": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
     "mf_rng_normal": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
 }
@@ -1437,10 +1437,11 @@ MX_SEGMENT, MX_SEGMENT_BYTES, MX_SEGMENT_SCALES = 256, 128, 8
 
 def rows_of(x):
     """``x`` [..., k] as a matrix whose rows are contiguous (a view where it has such a layout)."""
-    flat = x.reshape(-1, x.shape[-1])
-    if flat.stride(1) != 1 and flat.shape[1] > 1 or flat.stride(0) < flat.shape[1]:
-        flat = flat.contiguous()
-    return flat
+    flat = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    if flat.is_contiguous():
+        return flat
+    (row, column), width = flat.stride(), flat.shape[1]
+    return flat if (column == 1 or width == 1) and row >= width else flat.contiguous()
 
 
 def mx_empty(n, k, device):
@@ -1570,34 +1571,41 @@ def top_logits(logits, k, temperature):
     return values, indices, tail
 
 
-def distill_loss(logits, values, indices, tail, temperature, weight, reduction):
-    """Row losses [n], their sum or mean [] (None for "none"), and what ``distill_grad`` needs
-    (mf_distill_loss)."""
-    require_device(logits)
+def distill_loss(logits, values, indices, tail, temperature, weight, reduction, with_grad):
+    """Row losses [n], their sum or mean [] (None for "none"), what ``distill_grad`` needs, and
+    ``with_grad`` (a sum or mean) the gradient [n, v] for an incoming 1 (mf_distill_loss)."""
     n, v = logits.shape
     k = indices.shape[1]
-    stats = torch.empty(n * (3 + k) + 2, dtype=torch.float32, device=logits.device)
-    row_loss, ref, coef, entry_grad, total, norm = stats.split((n, n, n, n * k, 1, 1))
-    with _on(logits.device):
+    device = logits.device
+    # One allocation: total, norm, row losses, references, coefficients, entries' gradients.
+    stats = torch.empty(2 + n * (3 + k), dtype=torch.float32, device=device)
+    base = stats.data_ptr()
+    rows = base + 8
+    grad = torch.empty((n, v), dtype=logits.dtype, device=device) if with_grad else None
+    with _on(device):
         check(library().mf_distill_loss(
-            _ptr(logits), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), _ptr(values),
-            FLOAT_TYPES[values.dtype], _ptr(indices), _ptr(tail), k, temperature, _ptr(weight), REDUCTIONS[reduction],
-            _ptr(row_loss), _ptr(ref), _ptr(coef), _ptr(entry_grad), _ptr(total), _ptr(norm),
-            _stream(logits.device)), "distillation loss")
-    none = reduction == "none"
-    return row_loss, None if none else total.reshape(()), (ref, coef, entry_grad,
-                                                           None if none else norm)
+            logits.data_ptr(), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), values.data_ptr(),
+            FLOAT_TYPES[values.dtype], indices.data_ptr(), _ptr(tail), k, temperature, _ptr(weight),
+            REDUCTIONS[reduction], rows, rows + 4 * n, rows + 8 * n, rows + 12 * n, base, base + 4,
+            _ptr(grad), _stream(device)), "distillation loss")
+    if reduction == "none":
+        return stats[2:2 + n], None, stats, grad
+    return None, stats[0], stats, grad
 
 
-def distill_grad(logits, indices, temperature, weight, kept, incoming):
-    """The gradient [n, v] of ``distill_loss`` for the incoming gradient: one value, or one a row."""
+def distill_grad(logits, indices, temperature, weight, stats, reduction, incoming, grad=None):
+    """The gradient [n, v] of ``distill_loss`` for the incoming gradient: one value, or one a row.
+    ``grad``: the one that ``distill_loss`` gave, which an incoming 1 leaves."""
     n, v = logits.shape
-    ref, coef, entry_grad, norm = kept
-    grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+    base = stats.data_ptr()
+    ready = grad is not None
+    if not ready:
+        grad = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+    none = reduction == "none"
     with _on(logits.device):
         check(library().mf_distill_grad(
-            _ptr(logits), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), _ptr(indices),
-            indices.shape[1], temperature, _ptr(weight), _ptr(ref), _ptr(coef), _ptr(entry_grad),
-            _ptr(norm), _ptr(incoming), int(incoming.numel() > 1), _ptr(grad),
-            _stream(logits.device)), "distillation gradient")
+            logits.data_ptr(), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), indices.data_ptr(),
+            indices.shape[1], temperature, _ptr(weight), base + 8 + 4 * n, base + 8 + 8 * n,
+            base + 8 + 12 * n, None if none else base + 4, incoming.data_ptr(), int(none),
+            int(ready), grad.data_ptr(), _stream(logits.device)), "distillation gradient")
     return grad

@@ -37,20 +37,14 @@ class MXTensor:
     NaN).  rows is the product of the other dimensions."""
 
     def __init__(self, codes, scales, shape):
-        shape = torch.Size(shape)
+        self.shape = shape = torch.Size(shape)
         if not shape:
             raise ValueError("an MXTensor has at least one dimension")
         rows, segments = math.prod(shape[:-1]), -(-shape[-1] // hip.MX_SEGMENT)
-        for label, value, width in (("codes", codes, hip.MX_SEGMENT_BYTES * segments),
-                                    ("scales", scales, hip.MX_SEGMENT_SCALES * segments)):
-            if not isinstance(value, torch.Tensor) or value.dtype != torch.uint8:
-                raise TypeError(f"{label} must be a uint8 tensor")
-            if value.shape != (rows, width):
-                raise ValueError(f"{label} must have shape {(rows, width)}")
+        self.codes = _part("codes", codes, (rows, hip.MX_SEGMENT_BYTES * segments))
+        self.scales = _part("scales", scales, (rows, hip.MX_SEGMENT_SCALES * segments))
         if codes.device != scales.device:
             raise ValueError("codes and scales must use the same device")
-        self.codes, self.scales = (_aligned(v) for v in (codes, scales))
-        self.shape = shape
 
     @property
     def device(self):
@@ -66,9 +60,14 @@ class MXTensor:
         return f"MXTensor(shape={tuple(self.shape)}, device={self.device})"
 
 
-def _aligned(value):
-    """``value`` contiguous at a 16-byte address, as the kernels load it."""
-    value = value.contiguous()
+def _part(label, value, shape):
+    """``value``, checked, contiguous and at a 16-byte address, as the kernels load it."""
+    if not isinstance(value, torch.Tensor) or value.dtype != torch.uint8:
+        raise TypeError(f"{label} must be a uint8 tensor")
+    if value.shape != shape:
+        raise ValueError(f"{label} must have shape {shape}")
+    if not value.is_contiguous():
+        value = value.contiguous()
     return value if value.data_ptr() % 16 == 0 else value.clone()
 
 
@@ -124,12 +123,14 @@ def mx_linear(x, weight, bias=None):
         _check_floating("weight", weight)
     if bias is not None:
         _check_floating("bias", bias)
-    for label, value in (("weight", None if held else weight), ("bias", bias)):
-        if value is not None and value.dtype != x.dtype:
-            raise ValueError(f"x and {label} must have the same dtype")
-    for label, value in (("weight", weight), ("bias", bias)):
-        if value is not None and value.device != x.device:
-            raise ValueError(f"x and {label} must use the same device")
+    if not held and weight.dtype != x.dtype:
+        raise ValueError("x and weight must have the same dtype")
+    if bias is not None and bias.dtype != x.dtype:
+        raise ValueError("x and bias must have the same dtype")
+    if weight.device != x.device:
+        raise ValueError("x and weight must use the same device")
+    if bias is not None and bias.device != x.device:
+        raise ValueError("x and bias must use the same device")
     if x.ndim == 0 or len(weight.shape) != 2:
         raise ValueError("mx_linear takes x [..., k] and weight [o, k]")
     (o, k) = weight.shape
@@ -149,8 +150,14 @@ def mx_linear(x, weight, bias=None):
         codes, scales = hip.mx_quantize(hip.rows_of(weight.detach()))
     else:
         codes, scales, weight = weight.codes, weight.scales, None
-    bias = None if bias is None else bias.contiguous()
-    return _MXLinear.apply(hip.rows_of(x), weight, bias, codes, scales).reshape(shape)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    rows = hip.rows_of(x)
+    if torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in (x, weight, bias)):
+        y = _MXLinear.apply(rows, weight, bias, codes, scales)
+    else:
+        y = hip.mx_linear(rows, codes, scales, bias, False)[0]
+    return y if y.shape == shape else y.reshape(shape)
 
 
 __all__ = ["MXTensor", "mx_quantize", "mx_linear"]
