@@ -557,7 +557,7 @@ enum { MF_F32 = 0, MF_BF16 = 1, MF_F16 = 2 };
  * infinity and stands for NaN).  A value's code is x / 2^e rounded to nearest even on
  * {0, 0.5, 1, 1.5, 2, 3, 4, 6}, saturating at 6, with the sign in bit 3.  With S = ceil(k / 256), codes
  * are [n, 128 * S] bytes (the even value in the lower half of a byte) and scales [n, 8 * S]; codes past
- * k are 0.  codes 16-byte, scales 8-byte aligned.
+ * k are 0.  codes and scales are 16-byte aligned.
  *
  * x: [n, k], rows ldx values apart. */
 int mf_mx_quantize(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, uint8_t *codes,
@@ -565,31 +565,30 @@ int mf_mx_quantize(const void *x, int32_t type, int64_t n, int64_t k, int64_t ld
 /* out [n, k]: code * scale, rounded to the output's type. */
 int mf_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t k, void *out,
                      int32_t type, void *stream);
-/* out [n, o] = Q(x) W^T + bias (bias: o values of x's type, or NULL), FP32 sums; W [o, k] in codes.
- * xcodes and xscales receive Q(x), the scales segment by segment ([S, n, 8]), as mf_mx_grad_weight
- * takes them; where mf_mx_linear_sizes gives 0 bytes of codes they may be NULL and are not written
- * (`keep`: they always are). workspace: the bytes that it gives, 8-byte aligned.
- * n, o < 2^28, k < 2^24. */
-int mf_mx_linear_sizes(int32_t type, int64_t n, int64_t k, int64_t o, int32_t keep, int64_t *codes,
+/* out [n, o] = Q(x) W^T + bias (bias: o values of x's type, or NULL), FP32 sums.  W [o, k] is held in
+ * wcodes and wscales, or (weight != NULL: rows of x's type, ldw apart) quantized into them by the call.
+ * xcodes receives Q(x)'s codes.  The scales of an operand that the call quantizes go to wscales and
+ * xscales segment by segment, [S, n rounded up to even, 8], as mf_mx_grads takes them.
+ * mf_mx_linear_sizes gives the bytes of xcodes (0: neither xcodes nor xscales is written or needed,
+ * unless `keep`) and of the workspace; `held`: without weight.  Codes, scales and workspace are 16-byte
+ * aligned.  n, o < 2^28, k < 2^24. */
+int mf_mx_linear_sizes(int64_t n, int64_t k, int64_t o, int32_t held, int32_t keep, int64_t *xcodes,
                        int64_t *workspace);
-int mf_mx_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx,
-                 const uint8_t *wcodes, const uint8_t *wscales, int64_t o, const void *bias,
+int mf_mx_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, const void *weight,
+                 int64_t ldw, uint8_t *wcodes, uint8_t *wscales, int64_t o, const void *bias,
                  int32_t keep, uint8_t *xcodes, uint8_t *xscales, void *out, void *workspace,
                  int64_t bytes, void *stream);
 /* Gradients of mf_mx_linear straight through the quantizers, for dy [n, o] (rows ldy apart), FP32
- * sums: dx [n, k] = dy Q(W), dw [o, k] = dy^T Q(x), db [o] = column sums of dy.  They share a workspace
- * of mf_mx_grad_workspace bytes (16-byte aligned), one after the other on one stream: it holds the
- * 4-bit operand in BF16 and, where dy cannot be read in place, its BF16 terms.
- * n < 2^28, o <= 2^22, k < 2^24. */
-int mf_mx_grad_workspace(int32_t type, int64_t n, int64_t k, int64_t o, int64_t *bytes);
-int mf_mx_grad_input(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
-                     const uint8_t *wcodes, const uint8_t *wscales, int64_t k, void *dx,
-                     void *workspace, int64_t bytes, void *stream);
-int mf_mx_grad_weight(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
-                      const uint8_t *xcodes, const uint8_t *xscales, int64_t k, void *dw,
-                      void *workspace, int64_t bytes, void *stream);
-int mf_mx_grad_bias(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy, void *db,
-                    void *workspace, int64_t bytes, void *stream);
+ * sums: dx [n, k] = dy Q(W), dw [o, k] = dy^T Q(x), db [o] = column sums of dy; NULL for those that are
+ * not wanted.  wcodes and wscales are needed for dx (by_segment: the scales lie as mf_mx_linear
+ * writes them), xcodes and xscales for dw.  The workspace (mf_mx_grads_workspace bytes, 16-byte aligned)
+ * holds the 4-bit operands in BF16 and dy's BF16 terms.  n < 2^24, o <= 2^22, k < 2^24. */
+int mf_mx_grads_workspace(int32_t type, int64_t n, int64_t k, int64_t o, int32_t dx, int32_t dw,
+                          int32_t db, int64_t *bytes);
+int mf_mx_grads(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
+                const uint8_t *wcodes, const uint8_t *wscales, int32_t by_segment,
+                const uint8_t *xcodes, const uint8_t *xscales, int64_t k, void *dx, void *dw, void *db,
+                void *workspace, int64_t bytes, void *stream);
 
 /* ---- distillation from a teacher's top logits (distillation.hip) ---------- */
 /* The k largest of each row of logits [n, v] (rows ld apart), in descending order, the lowest index

@@ -104,32 +104,31 @@ template <typename T> __device__ __forceinline__ void unpack(v4u raw, float (&x)
     for (int j = 0; j < PIECE<T>; ++j) x[j] = float(p.v[j]);
 }
 
-// Calls f(i, values) for this thread's pieces from `start` on. Four loads are in flight: with one, a
-// compute unit's waves keep too few bytes under way to fill the memory's latency. Pieces that are not
-// whole come last.
+// Calls f(i, values) for this thread's pieces from `start` on: pieces i, i + THREADS, ... four at a
+// time, so that as many loads are in flight (with one, a compute unit's waves keep too few bytes under
+// way to fill the memory's latency), then singly. Pieces that are not whole come last.
 template <int THREADS, typename T, typename F>
 __device__ __forceinline__ void for_pieces(const Row<T> &row, int start, float fill, F f) {
     constexpr int LOADS = 4;
-    float x[PIECE<T>];
     int i = max(start, row.first) + int(threadIdx.x);
     for (; i + (LOADS - 1) * THREADS < row.last; i += LOADS * THREADS) {
         v4u raw[LOADS];
+        float x[LOADS][PIECE<T>];
 #pragma unroll
         for (int t = 0; t < LOADS; ++t) raw[t] = row.whole(i + t * THREADS);
 #pragma unroll
-        for (int t = 0; t < LOADS; ++t) {
-            unpack<T>(raw[t], x);
-            f(i + t * THREADS, x);
-        }
+        for (int t = 0; t < LOADS; ++t) unpack<T>(raw[t], x[t]);
+        f(i, x);
     }
+    float x[1][PIECE<T>];
     for (; i < row.last; i += THREADS) {
-        unpack<T>(row.whole(i), x);
+        unpack<T>(row.whole(i), x[0]);
         f(i, x);
     }
     const int side = threadIdx.x == 0 ? 0 : row.pieces - 1;
     if (threadIdx.x < 2 && side >= start && (side < row.first || side >= row.last) &&
         (threadIdx.x == 0 || row.pieces > 1)) {
-        unpack<T>(row.piece(side, T(fill)), x);
+        unpack<T>(row.piece(side, T(fill)), x[0]);
         f(side, x);
     }
 }
@@ -233,17 +232,21 @@ __device__ __forceinline__ void write_rest(const Row<T> &row, const u32 *bits, f
             store_rest(grad, row, i, piece_bits<T>(bits, i), vec, zero);
         return;
     }
-    for_pieces<THREADS>(row, 0, 0.0f, [&](int i, float (&x)[PIECE<T>]) {
+    for_pieces<THREADS>(row, 0, 0.0f, [&](int i, auto &x) {
+        constexpr int COUNT = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-        for (int j = 0; j < PIECE<T>; ++j) x[j] = power(x[j], ref, c) * coef;
-        store_rest(grad, row, i, piece_bits<T>(bits, i), vec, x);
+        for (int t = 0; t < COUNT; ++t) {
+#pragma unroll
+            for (int j = 0; j < PIECE<T>; ++j) x[t][j] = power(x[t][j], ref, c) * coef;
+            store_rest(grad, row, i + t * THREADS, piece_bits<T>(bits, i + t * THREADS), vec, x[t]);
+        }
     });
 }
 
 // One workgroup a row: one pass over the row for the classes outside the entries, and with GRAD
 // another that writes the gradient for an incoming 1, which finds the row in the cache.
 template <typename T, int WAVES, bool GRAD>
-__global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 4) void k_distill(const DistillArgs a) {
     extern __shared__ u32 bits[];
     __shared__ float scratch[2 * WAVES];
     constexpr int THREADS = 64 * WAVES;
@@ -271,20 +274,27 @@ __global__ __launch_bounds__(64 * WAVES) void k_distill(const DistillArgs a) {
                 teacher.add(value_at(a.values, a.values_type, first + j), c);
                 entries.add(float(s[indices[j]]), c);
             }
-    for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, float (&x)[PIECE<T>]) {
-        if (const u32 marked = piece_bits<T>(bits, i)) {
+    for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, auto &x) {
+        constexpr int COUNT = sizeof(x) / sizeof(x[0]);
+        float top = rest.m;
 #pragma unroll
-            for (int j = 0; j < PIECE<T>; ++j)
-                if (marked >> j & 1u) x[j] = -INFINITY;
+        for (int t = 0; t < COUNT; ++t) {
+            if (const u32 marked = piece_bits<T>(bits, i + t * THREADS)) {
+#pragma unroll
+                for (int j = 0; j < PIECE<T>; ++j)
+                    if (marked >> j & 1u) x[t][j] = -INFINITY;
+            }
+            top = largest(x[t], top);
         }
-        const float top = largest(x, rest.m);
         if (top > rest.m) {
             rest.s *= power(rest.m, top, c);
             rest.m = top;
         }
         const float ref = rest.ref();
 #pragma unroll
-        for (int j = 0; j < PIECE<T>; ++j) rest.s += power(x[j], ref, c);
+        for (int t = 0; t < COUNT; ++t)
+#pragma unroll
+            for (int j = 0; j < PIECE<T>; ++j) rest.s += power(x[t][j], ref, c);
     });
     teacher = block_merge<WAVES>(teacher, c, scratch);
     entries = block_merge<WAVES>(entries, c, scratch);
@@ -456,29 +466,27 @@ __device__ __forceinline__ float value_of(u64 key) {
 }
 
 // Lists a piece's classes from `bound` (of the value `least`) on, and adds the others' exp2(x c + b)
-// to the sum. A NaN that is not listed makes the sum one (with least = -inf every class's key is
-// compared, and a NaN that belongs there is listed).
+// to the sum. A NaN that is not listed makes the sum one (with least = -inf every piece's keys are
+// compared, and a NaN that belongs there is listed). Changes x.
 template <typename T>
-__device__ __forceinline__ void sift(const Row<T> &row, int i, const float (&x)[PIECE<T>], float least,
+__device__ __forceinline__ void sift(const Row<T> &row, int i, float (&x)[PIECE<T>], float least,
                                      u64 bound, float c, float b, TopShared &sh, float &sum) {
     constexpr int P = PIECE<T>;
     if (largest(x, -INFINITY) >= least || i < row.first || i >= row.last) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const int index = i * P - row.off + j;
-            if (index < 0 || index >= row.v) continue;
+            if (x[j] < least || index < 0 || index >= row.v) continue;
             const u64 key = key_of(x[j], index);
             if (key >= bound) {
                 const u32 at = atomicAdd(&sh.found, 1u);
                 if (at < u32(TOP_LIST)) sh.list[at] = key;
-            } else {
-                sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
+                x[j] = -INFINITY;       // adds nothing
             }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < P; ++j) sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
     }
+#pragma unroll
+    for (int j = 0; j < P; ++j) sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
 }
 
 // The smallest selected key by radix selection, eight bits a pass over the row: for rows with
@@ -492,15 +500,16 @@ __device__ u64 exact_bound(const Row<T> &row, int k, TopShared &sh) {
         __syncthreads();
         for (int b = threadIdx.x; b < 256; b += THREADS) sh.counts[b] = 0;
         __syncthreads();
-        for_pieces<THREADS>(row, 0, 0.0f, [&](int i, float (&x)[PIECE<T>]) {
+        for_pieces<THREADS>(row, 0, 0.0f, [&](int i, auto &x) {
+            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
 #pragma unroll
-            for (int j = 0; j < PIECE<T>; ++j) {
-                const int index = i * PIECE<T> - row.off + j;
-                const u64 key = key_of(x[j], index);
-                if (index >= 0 && index < row.v &&
-                    (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8)))
-                    atomicAdd(&sh.counts[key >> shift & 255u], 1u);
-            }
+                for (int j = 0; j < PIECE<T>; ++j) {
+                    const int index = (i + t * THREADS) * PIECE<T> - row.off + j;
+                    const u64 key = key_of(x[t][j], index);
+                    if (index >= 0 && index < row.v &&
+                        (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8)))
+                        atomicAdd(&sh.counts[key >> shift & 255u], 1u);
+                }
         });
         __syncthreads();
         if (threadIdx.x == 0) {   // the digit that holds the k-th largest
@@ -647,8 +656,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         keep_first<THREADS>(sh, a.k, c, b, sum);
         bound = sh.list[a.k - 1];
         least = value_of(bound);
-        for_pieces<THREADS>(row, ITEMS * THREADS, -INFINITY, [&](int i, float (&x)[P]) {
-            sift(row, i, x, least, bound, c, b, sh, sum);
+        for_pieces<THREADS>(row, ITEMS * THREADS, -INFINITY, [&](int i, auto &x) {
+#pragma unroll
+            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
+                sift(row, i + t * THREADS, x[t], least, bound, c, b, sh, sum);
         });
         exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
     }
@@ -657,8 +668,10 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         if (threadIdx.x == 0) sh.found = 0;
         __syncthreads();
         sum = 0.0f;
-        for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, float (&x)[P]) {
-            sift(row, i, x, -INFINITY, bound, c, b, sh, sum);
+        for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, auto &x) {
+#pragma unroll
+            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
+                sift(row, i + t * THREADS, x[t], -INFINITY, bound, c, b, sh, sum);
         });
         __syncthreads();
     }
@@ -674,12 +687,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     if (a.k < a.v && !(sum > 0x1p-60f && sum < 0x1p60f && fabsf(b) < 0x1p60f)) {
         const u64 last = sh.list[a.k - 1];
         LogSum rest;
-        for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, float (&x)[P]) {
+        for_pieces<THREADS>(row, 0, -INFINITY, [&](int i, auto &x) {
+            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
 #pragma unroll
-            for (int j = 0; j < P; ++j) {
-                const int index = i * P - row.off + j;
-                if (index >= 0 && index < row.v && key_of(x[j], index) < last) rest.add(x[j], c);
-            }
+                for (int j = 0; j < P; ++j) {
+                    const int index = (i + t * THREADS) * P - row.off + j;
+                    if (index >= 0 && index < row.v && key_of(x[t][j], index) < last)
+                        rest.add(x[t][j], c);
+                }
         });
         rest = block_merge<WAVES>(rest, c, sh.scratch);
         tail = rest.m == -INFINITY && rest.s == 0.0f

@@ -202,14 +202,14 @@ SIGNATURES = {
                            ct.c_int),
     "mf_mx_quantize": ([_P, _I32, _I64, _I64, _I64, _P, _P, _P], ct.c_int),
     "mf_mx_dequantize": ([_P, _P, _I64, _I64, _P, _I32, _P], ct.c_int),
-    "mf_mx_linear_sizes": ([_I32, _I64, _I64, _I64, _I32, ct.POINTER(_I64), ct.POINTER(_I64)],
+    "mf_mx_linear_sizes": ([_I64, _I64, _I64, _I32, _I32, ct.POINTER(_I64), ct.POINTER(_I64)],
                            ct.c_int),
-    "mf_mx_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P, _P, _P, _I64, _P],
-                     ct.c_int),
-    "mf_mx_grad_workspace": ([_I32, _I64, _I64, _I64, ct.POINTER(_I64)], ct.c_int),
-    "mf_mx_grad_input": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P], ct.c_int),
-    "mf_mx_grad_weight": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P], ct.c_int),
-    "mf_mx_grad_bias": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P], ct.c_int),
+    "mf_mx_linear": ([_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _I32, _P, _P, _P, _P,
+                      _I64, _P], ct.c_int),
+    "mf_mx_grads_workspace": ([_I32, _I64, _I64, _I64, _I32, _I32, _I32, ct.POINTER(_I64)],
+                              ct.c_int),
+    "mf_mx_grads": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _P, _I64, _P, _P, _P, _P, _I64,
+                     _P], ct.c_int),
     "mf_top_logits": ([_P, _I32, _I64, _I64, _I64, _I64, ct.c_float, _P, _P, _P, _P], ct.c_int),
     "mf_distill_loss": ([_P, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _I64, ct.c_float, _P, _I32,
                          _P, _P, _P, _P, _P, _P, _P, _P], ct.c_int),
@@ -1478,74 +1478,82 @@ def mx_dequantize(codes, scales, k, dtype):
 
 
 @lru_cache(maxsize=4096)
-def _mx_linear_sizes(kind, n, k, o, keep):
-    codes, work = _I64(), _I64()
-    check(library().mf_mx_linear_sizes(kind, n, k, o, keep, ct.byref(codes), ct.byref(work)),
+def _mx_linear_layout(n, k, o, held, keep):
+    """Bytes of an mx_linear call's parts in one block: where W's codes (not held), W's scales, Q(x)'s
+    codes, its scales and the workspace begin, and the end."""
+    xcodes, work = _I64(), _I64()
+    check(library().mf_mx_linear_sizes(n, k, o, held, keep, ct.byref(xcodes), ct.byref(work)),
           "microscaled product")
-    return codes.value, work.value
+    segments = -(-k // MX_SEGMENT)
+
+    def scales(rows):
+        return segments * (rows + rows % 2) * MX_SEGMENT_SCALES
+
+    sizes = (0 if held else o * segments * MX_SEGMENT_BYTES, 0 if held else scales(o), xcodes.value,
+             scales(n) if xcodes.value else 0, work.value)
+    starts = [0]
+    for size in sizes:
+        starts.append(starts[-1] + size)
+    return tuple(starts)
 
 
-def mx_linear(x, codes, scales, bias, keep):
-    """``Q(x) W^T + bias`` [n, o] (mf_mx_linear); with ``keep`` also the block of Q(x)'s codes
-    [n, 128 S] and scales [S, n, 8]."""
+def mx_linear(x, weight, codes, scales, bias, keep):
+    """``Q(x) W^T + bias`` [n, o] (mf_mx_linear) for ``weight`` [o, k], or for a W held in ``codes`` and
+    ``scales`` (``weight`` None). Also the block that holds what the call quantized, with ``keep``
+    Q(x) among it, for ``mx_grads``."""
     n, k = x.shape
-    o, kind = codes.shape[0], FLOAT_TYPES[x.dtype]
-    size, work = _mx_linear_sizes(kind, n, k, o, keep)
-    # One allocation: the codes, their scales (8 bytes for 128 of codes) and the workspace.
-    held = size + size // 16
-    block = torch.empty(held + work, dtype=torch.uint8, device=x.device) if held + work else None
-    base = block.data_ptr() if held + work else 0
+    held = weight is None
+    o = codes.shape[0] if held else weight.shape[0]
+    w0, ws0, x0, xs0, work0, end = _mx_linear_layout(n, k, o, held, keep)
+    block = torch.empty(end, dtype=torch.uint8, device=x.device) if end else None
+    base = block.data_ptr() if end else 0
     out = torch.empty((n, o), dtype=x.dtype, device=x.device)
+    quantized = xs0 > x0
     with _on(x.device):
         check(library().mf_mx_linear(
-            _ptr(x), kind, n, k, x.stride(0), _ptr(codes), _ptr(scales), o, _ptr(bias), keep,
-            base if size else None, base + size if size else None, _ptr(out),
-            base + held if work else None, work, _stream(x.device)), "microscaled product")
-    return out, block if keep else None
+            x.data_ptr(), FLOAT_TYPES[x.dtype], n, k, x.stride(0), _ptr(weight),
+            0 if held else weight.stride(0), codes.data_ptr() if held else base + w0,
+            scales.data_ptr() if held else base + ws0, o, _ptr(bias), keep,
+            base + x0 if quantized else None, base + xs0 if quantized else None, out.data_ptr(),
+            base + work0 if end > work0 else None, end - work0, _stream(x.device)),
+            "microscaled product")
+    return out, block
 
 
-def mx_grad_workspace(dy, k):
-    """The workspace that the gradients of ``dy`` [n, o] share."""
+def mx_grads(dy, k, codes, scales, block, want):
+    """(dx [n, k], dw [o, k], db [o]) of ``mx_linear`` for ``dy`` [n, o], None for those that ``want``
+    leaves out (mf_mx_grads). W is held in ``codes`` and ``scales``, or (None) in ``block``."""
+    n, o = dy.shape
+    kind, device = FLOAT_TYPES[dy.dtype], dy.device
+    held = codes is not None
+    wcodes = wscales = xcodes = xscales = None
+    if held:
+        wcodes, wscales = codes.data_ptr(), scales.data_ptr()
+    if block is not None:
+        w0, ws0, x0, xs0, _, _ = _mx_linear_layout(n, k, o, held, want[1])
+        base = block.data_ptr()
+        xcodes, xscales = base + x0, base + xs0
+        if not held:
+            wcodes, wscales = base + w0, base + ws0
+    dx = torch.empty((n, k), dtype=dy.dtype, device=device) if want[0] else None
+    dw = torch.empty((o, k), dtype=dy.dtype, device=device) if want[1] else None
+    db = torch.empty(o, dtype=dy.dtype, device=device) if want[2] else None
+    size = _mx_grads_workspace(kind, n, k, o, *want)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    with _on(device):
+        check(library().mf_mx_grads(
+            dy.data_ptr(), kind, n, o, dy.stride(0), wcodes, wscales, not held, xcodes, xscales, k,
+            _ptr(dx), _ptr(dw), _ptr(db), _ptr(work), size, _stream(device)),
+            "microscaled gradients")
+    return dx, dw, db
+
+
+@lru_cache(maxsize=4096)
+def _mx_grads_workspace(kind, n, k, o, dx, dw, db):
     size = _I64()
-    check(library().mf_mx_grad_workspace(FLOAT_TYPES[dy.dtype], dy.shape[0], k, dy.shape[1],
-                                         ct.byref(size)), "microscaled gradient workspace")
-    return torch.empty(size.value, dtype=torch.uint8, device=dy.device)
-
-
-def mx_grad_input(dy, codes, scales, k, workspace):
-    """``dy Q(W)`` [n, k] (mf_mx_grad_input)."""
-    n, o = dy.shape
-    dx = torch.empty((n, k), dtype=dy.dtype, device=dy.device)
-    with _on(dy.device):
-        check(library().mf_mx_grad_input(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0),
-                                         _ptr(codes), _ptr(scales), k, _ptr(dx), _ptr(workspace),
-                                         workspace.numel(), _stream(dy.device)),
-              "microscaled input gradient")
-    return dx
-
-
-def mx_grad_weight(dy, block, k, workspace):
-    """``dy^T Q(x)`` [o, k] (mf_mx_grad_weight) for the ``block`` that ``mx_linear`` kept."""
-    n, o = dy.shape
-    dw = torch.empty((o, k), dtype=dy.dtype, device=dy.device)
-    codes = n * -(-k // MX_SEGMENT) * MX_SEGMENT_BYTES
-    with _on(dy.device):
-        check(library().mf_mx_grad_weight(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0),
-                                          block.data_ptr(), block.data_ptr() + codes, k, _ptr(dw),
-                                          _ptr(workspace), workspace.numel(), _stream(dy.device)),
-              "microscaled weight gradient")
-    return dw
-
-
-def mx_grad_bias(dy, workspace):
-    """Column sums of ``dy`` [n, o] (mf_mx_grad_bias)."""
-    n, o = dy.shape
-    db = torch.empty(o, dtype=dy.dtype, device=dy.device)
-    with _on(dy.device):
-        check(library().mf_mx_grad_bias(_ptr(dy), FLOAT_TYPES[dy.dtype], n, o, dy.stride(0), _ptr(db),
-                                        _ptr(workspace), workspace.numel(), _stream(dy.device)),
-              "microscaled bias gradient")
-    return db
+    check(library().mf_mx_grads_workspace(kind, n, k, o, dx, dw, db, ct.byref(size)),
+          "microscaled gradient workspace")
+    return size.value
 
 
 # ---------------------------------------------------------------------------

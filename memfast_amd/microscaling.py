@@ -85,31 +85,22 @@ def mx_quantize(x):
 
 
 class _MXLinear(torch.autograd.Function):
-    """Product of Q(x) and a quantized weight.  ``weight`` is the tensor that ``codes`` and
-    ``scales`` were made of, or None for a weight that is held in codes alone."""
+    """Product of Q(x) and Q(weight), or of a weight held in ``codes`` and ``scales``."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, codes, scales):
-        keep = ctx.needs_input_grad
-        y, block = hip.mx_linear(x, codes, scales, bias, keep[1])
+        y, block = hip.mx_linear(x, weight, codes, scales, bias, ctx.needs_input_grad[1])
         ctx.width = x.shape[1]
-        ctx.save_for_backward(*((codes, scales) if keep[0] else (None, None)), block)
+        ctx.save_for_backward(codes, scales, block)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         codes, scales, block = ctx.saved_tensors
-        dy = hip.rows_of(dy)
-        work = hip.mx_grad_workspace(dy, ctx.width)
-        dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = hip.mx_grad_input(dy, codes, scales, ctx.width, work)
-        if ctx.needs_input_grad[1]:
-            dw = hip.mx_grad_weight(dy, block, ctx.width, work)
-        if ctx.needs_input_grad[2]:
-            db = hip.mx_grad_bias(dy, work)
-        return dx, dw, db, None, None
+        grads = hip.mx_grads(hip.rows_of(dy), ctx.width, codes, scales, block,
+                             ctx.needs_input_grad[:3])
+        return (*grads, None, None)
 
 
 def mx_linear(x, weight, bias=None):
@@ -146,17 +137,16 @@ def mx_linear(x, weight, bias=None):
         if not held:
             y = y + weight.sum(-1) * 0
         return y if bias is None else y + bias
-    if not held:
-        codes, scales = hip.mx_quantize(hip.rows_of(weight.detach()))
-    else:
-        codes, scales, weight = weight.codes, weight.scales, None
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
+    codes, scales = (weight.codes, weight.scales) if held else (None, None)
+    weight = None if held else hip.rows_of(weight)
     rows = hip.rows_of(x)
-    if torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or
+                                    bias is not None and bias.requires_grad):
         y = _MXLinear.apply(rows, weight, bias, codes, scales)
     else:
-        y = hip.mx_linear(rows, codes, scales, bias, False)[0]
+        y = hip.mx_linear(rows, weight, codes, scales, bias, False)[0]
     return y if y.shape == shape else y.reshape(shape)
 
 
