@@ -142,11 +142,15 @@ __device__ __forceinline__ v8bf transposed(const u8 *p, int four_rows) {
     return u.v;
 }
 
-// How far the 16-byte pieces of row r lie rotated in LDS, in rows of that many pieces: four
-// consecutive rows' reads of 64 bytes are then in different banks.
-template <int PIECES> __device__ __forceinline__ int rotation(int r) {
-    static_assert(PIECES == 8 || PIECES == 16 || PIECES == 32, "the rotation stays within the row");
-    return PIECES == 8 ? 4 * (r >> 1 & 1) : 4 * (r & 3);
+// Where piece p of row r of a tile with that many pieces a row lies in LDS, and the piece that lies at p:
+// moved on so that four consecutive rows' reads of 64 bytes are in different banks (rows of 384
+// bytes are half a turn of the banks apart from each other already).
+template <int PIECES> __device__ __forceinline__ int moved(int p, int r) {
+    static_assert(PIECES == 8 || PIECES == 16 || PIECES == 24 || PIECES == 32, "widths of tiles");
+    return (p + (PIECES == 8 ? 4 * (r >> 1 & 1) : 4 * (r & 3))) % PIECES;
+}
+template <int PIECES> __device__ __forceinline__ int moved_back(int p, int r) {
+    return (p + PIECES - (PIECES == 8 ? 4 * (r >> 1 & 1) : 4 * (r & 3))) % PIECES;
 }
 
 // Tile `block` of out[m, c] = sum_t sum_d A_t[m, d] B[d, c], WM x WC waves of TM x TC tiles of 32 x 32,
@@ -176,32 +180,36 @@ __device__ __forceinline__ void grad_tile(const GradArgs &a, u32 block, u8 *stag
         } else if (at < A_BYTES) {
             constexpr int PIECES = BM / 8;
             const int piece = at / 16 + lane, r = piece / PIECES;
-            const int p = piece % PIECES ^ rotation<PIECES>(r);
+            const int p = moved_back<PIECES>(piece % PIECES, r);
             offset[i] = u32(r * a.lda * 2) + u32(min(m0 + p * 8, a.width - 8) - m0) * 2;
         } else {
             constexpr int PIECES = BC / 8;
             const int piece = (at - A_BYTES) / 16 + lane, r = piece / PIECES;
-            offset[i] = u32(r * a.ldb * 2) + u32((piece % PIECES ^ rotation<PIECES>(r)) * 16);
+            const int p = moved_back<PIECES>(piece % PIECES, r);
+            offset[i] = u32(r * a.ldb * 2) + u32(min(c0 + p * 8, a.ldb - 8) - c0) * 2;
         }
     }
     const u32 lds = lds_address(staged);
     const i64 steps = (a.depth + GRAD_STEP - 1) / GRAD_STEP, stages = steps * a.terms;
-    int term = a.terms - 1;     // the smallest terms first
-    i64 step = 0;               // of the next copy
+    // The next copy's tiles; the smallest terms come first.
+    const i64 a_step = (DEPTH_ROWS ? GRAD_STEP * a.lda : GRAD_STEP) * 2, b_step = GRAD_STEP * a.ldb * 2;
+    const u8 *at_a0 = reinterpret_cast<const u8 *>(a.a + (a.terms - 1) * a.plane +
+                                                   (DEPTH_ROWS ? m0 : m0 * a.lda));
+    const u8 *at_b0 = reinterpret_cast<const u8 *>(a.b + c0);
+    i64 step = 0;
     auto copy = [&](int buffer) {
-        const bf16 *plane = a.a + term * a.plane;
-        const u8 *a0 = reinterpret_cast<const u8 *>(
-            DEPTH_ROWS ? plane + step * GRAD_STEP * a.lda + m0 : plane + m0 * a.lda + step * GRAD_STEP);
-        const u8 *b0 = reinterpret_cast<const u8 *>(a.b + step * GRAD_STEP * a.ldb + c0);
 #pragma unroll
         for (int i = 0; i < COPIES; ++i) {
             const int at = (first_copy + i) * 1024;
-            lds_dma_16((at < A_BYTES ? a0 : b0) + offset[i],
+            lds_dma_16((at < A_BYTES ? at_a0 : at_b0) + offset[i],
                        __builtin_amdgcn_readfirstlane(lds + buffer * STAGE + at));
         }
+        at_a0 += a_step;
+        at_b0 += b_step;
         if (++step == steps) {
             step = 0;
-            --term;
+            at_a0 -= steps * a_step + a.plane * 2;
+            at_b0 -= steps * b_step;
         }
     };
 
@@ -212,7 +220,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs &a, u32 block, u8 *stag
     auto turned_at = [&](int col, auto width) {
         constexpr int PIECES = decltype(width)::value / 8;
         const int r = 8 * half + (i16 >> 2), piece = (col + 16 * side) / 8 + (i16 & 3) / 2;
-        return r * PIECES * 16 + (piece ^ rotation<PIECES>(r)) * 16 + (i16 & 1) * 8;
+        return r * PIECES * 16 + moved<PIECES>(piece, r) * 16 + (i16 & 1) * 8;
     };
     const std::integral_constant<int, BM> bm{};
     const std::integral_constant<int, BC> bc{};
@@ -233,15 +241,9 @@ __device__ __forceinline__ void grad_tile(const GradArgs &a, u32 block, u8 *stag
             wait_stage<(STAGES - 2) * COPIES>();
         else
             wait_stage<0>();
-        if (next < stages) {
-            copy(filling);
-            ++next;
-            filling = filling + 1 == STAGES ? 0 : filling + 1;
-        }
         const u8 *tile = staged + reading * STAGE;
         reading = reading + 1 == STAGES ? 0 : reading + 1;
-#pragma unroll
-        for (int s = 0; s < GRAD_STEP / 16; ++s) {
+        auto multiply = [&](int s) {
             v8bf fa[TM], fb[TC];
 #pragma unroll
             for (int i = 0; i < TM; ++i)
@@ -258,7 +260,14 @@ __device__ __forceinline__ void grad_tile(const GradArgs &a, u32 block, u8 *stag
                 for (int j = 0; j < TC; ++j)
                     acc[i][j] =
                         __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        };
+        if (next < stages) {
+            copy(filling);
+            ++next;
+            filling = filling + 1 == STAGES ? 0 : filling + 1;
         }
+#pragma unroll
+        for (int s = 0; s < GRAD_STEP / 16; ++s) multiply(s);
     }
     T *out = static_cast<T *>(a.out);
 #pragma unroll
@@ -322,15 +331,14 @@ struct GradSpace {
     }
 };
 
-static i64 grad_tiles(const GradArgs &a, i64 edge) {
-    return (a.rows + edge - 1) / edge * ((a.cols + edge - 1) / edge);
+static i64 grad_tiles(const GradArgs &a, i64 bm, i64 bc) {
+    return (a.rows + bm - 1) / bm * ((a.cols + bc - 1) / bc);
 }
 
 template <typename T, bool DEPTH_ROWS, int WM, int WC, int TM, int TC, int STAGES>
 static int launch_grad_tile(const GradArgs &args, hipStream_t s) {
     constexpr int BM = 32 * WM * TM, BC = 32 * WC * TC, LDS = STAGES * (BM + BC) * GRAD_STEP * 2;
-    static_assert(BM == BC && BC <= SEG, "square tiles within the padding of the rows");
-    const i64 tiles = grad_tiles(args, BM);
+    const i64 tiles = grad_tiles(args, BM, BC);
     if (tiles > i64(1) << 30) return fail(MF_E_UNSUPPORTED, "gradient too large");
     auto kernel = k_mx_grad<T, DEPTH_ROWS, WM, WC, TM, TC, STAGES>;
     if (const int status = allow_lds(kernel, LDS)) return status;
@@ -338,24 +346,31 @@ static int launch_grad_tile(const GradArgs &args, hipStream_t s) {
     return check_launch("microscaled gradient");
 }
 
-// The largest tile of which every compute unit gets one (us, 64 x 64 / 128 x 128 / 256 x 256, n x k x o): dw of
-// 2048 x 11008 x 4096 402 / 258 / 183, dx of it 363 / 282 / 218, dx of 2048 x 4096 x 11008
-// 349 / 206 / 266, dx of 512 x 1024 x 1024 8 / 15 / 30. Few small tiles wait for their copies: a third
-// stage takes dx of 128 x 4096 x 4096 from 34 to 24 us; in the larger ones it costs a second
-// workgroup (282 -> 321 us).
+// The tile whose rounds over the 256 compute units take the least: a round of 256 x 256 takes 123 us
+// at a depth of 4096, one of 192 x 256 0.75 and one of 128 x 128 (two a compute unit) 0.63 of that. us,
+// 256 x 256 / 192 x 256 / 128 x 128, n x k x o: dx of 2048 x 11008 x 4096 (344 / 473 / 1376 tiles) 223 / 189 / 273, dw
+// of it 189 / 211 / 255, dx of 2048 x 4096 x 11008 265 / 222 / 204, dx of 4096^3 126 / 172 / 164.
+// Where 128 x 128 leaves compute units without a tile, 64 x 64: dx of 512 x 1024 x 1024 8 against 15 us. Few
+// small tiles wait for their copies: a third stage takes dx of 128 x 4096 x 4096 from 34 to 24 us; in
+// the larger ones it costs the second workgroup (282 -> 321 us).
 template <typename T, bool DEPTH_ROWS> static int launch_grad(const GradArgs &args, hipStream_t s) {
-    if (grad_tiles(args, 256) >= 256) return launch_grad_tile<T, DEPTH_ROWS, 4, 2, 2, 4, 2>(args, s);
-    if (grad_tiles(args, 128) >= 256) return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 2, 2, 2>(args, s);
-    return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 1, 1, 3>(args, s);
+    if (grad_tiles(args, 128, 128) < 256) return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 1, 1, 3>(args, s);
+    const auto rounds = [](i64 tiles, i64 at_once) { return (tiles + at_once - 1) / at_once; };
+    const i64 large = rounds(grad_tiles(args, 256, 256), 256) * 100;
+    const i64 middle = rounds(grad_tiles(args, 192, 256), 256) * 75;
+    const i64 small = rounds(grad_tiles(args, 128, 128), 512) * 63;
+    if (large <= middle && large <= small) return launch_grad_tile<T, DEPTH_ROWS, 4, 2, 2, 4, 2>(args, s);
+    if (middle <= small) return launch_grad_tile<T, DEPTH_ROWS, 2, 4, 3, 2, 2>(args, s);
+    return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 2, 2, 2>(args, s);
 }
 
 template <typename T> static int launch_both(const GradArgs &dx, const GradArgs &dw, hipStream_t s) {
-    const i64 tiles = grad_tiles(dx, 64);
+    const i64 tiles = grad_tiles(dx, 64, 64);
     constexpr int STAGES = 3, LDS = STAGES * 128 * GRAD_STEP * 2;
-    if (grad_tiles(dx, 128) < 256 && grad_tiles(dw, 128) < 256) {
+    if (grad_tiles(dx, 128, 128) < 256 && grad_tiles(dw, 128, 128) < 256) {
         auto kernel = k_mx_grads<T, 2, 2, 1, 1, STAGES>;
         if (const int status = allow_lds(kernel, LDS)) return status;
-        hipLaunchKernelGGL(kernel, dim3(unsigned(tiles + grad_tiles(dw, 64))), dim3(256), LDS, s, dx, dw,
+        hipLaunchKernelGGL(kernel, dim3(unsigned(tiles + grad_tiles(dw, 64, 64))), dim3(256), LDS, s, dx, dw,
                            u32(tiles));
         return check_launch("microscaled gradients");
     }

@@ -72,8 +72,13 @@ class _Distillation(torch.autograd.Function):
         return _weighted(row_loss, weight) if reduction == "none" else total
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, incoming):
+        if torch.is_grad_enabled():     # create_graph: the gradient is not differentiable
+            return once_differentiable(_Distillation._grad)(ctx, incoming)
+        return _Distillation._grad(ctx, incoming)
+
+    @staticmethod
+    def _grad(ctx, incoming):
         logits, indices, weight, stats = ctx.saved_tensors
         temperature, reduction = ctx.options
         ready, ctx.ready = ctx.ready, None
@@ -138,8 +143,8 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
         return zero if reduction == "none" else zero.sum()
 
     rows = hip.rows_of(logits)
-    entries = values.detach().reshape(-1, k).contiguous()
-    indices = indices.reshape(-1, k).to(torch.int64).contiguous()
+    entries = _matrix(values, k)
+    indices = _matrix(indices if indices.dtype == torch.int64 else indices.to(torch.int64), k)
     tail, weight = _per_row(tail), _per_row(weight)
     if torch.is_grad_enabled() and logits.requires_grad:
         loss = _Distillation.apply(rows, entries, indices, tail, weight, temperature, reduction)
@@ -151,8 +156,14 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
     return loss.reshape(lead) if reduction == "none" else loss
 
 
+def _matrix(value, k):
+    return value if value.ndim == 2 and value.is_contiguous() else value.reshape(-1, k).contiguous()
+
+
 def _per_row(value):
-    return None if value is None else value.detach().to(torch.float32).reshape(-1).contiguous()
+    if value is None or value.dtype == torch.float32 and value.ndim == 1 and value.is_contiguous():
+        return value
+    return value.detach().to(torch.float32).reshape(-1).contiguous()
 
 
 __all__ = ["top_logits", "distillation_loss"]

@@ -90,17 +90,20 @@ class _MXLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, codes, scales):
         y, block = hip.mx_linear(x, weight, codes, scales, bias, ctx.needs_input_grad[1])
-        ctx.width = x.shape[1]
-        ctx.save_for_backward(codes, scales, block)
+        ctx.width, ctx.operands = x.shape[1], (codes, scales, block)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        codes, scales, block = ctx.saved_tensors
-        grads = hip.mx_grads(hip.rows_of(dy), ctx.width, codes, scales, block,
-                             ctx.needs_input_grad[:3])
-        return (*grads, None, None)
+        if torch.is_grad_enabled():     # create_graph: the gradients are not differentiable
+            return once_differentiable(_MXLinear._grads)(ctx, dy)
+        return _MXLinear._grads(ctx, dy)
+
+    @staticmethod
+    def _grads(ctx, dy):
+        codes, scales, block = ctx.operands
+        return (*hip.mx_grads(hip.rows_of(dy), ctx.width, codes, scales, block,
+                              ctx.needs_input_grad[:3]), None, None)
 
 
 def mx_linear(x, weight, bias=None):

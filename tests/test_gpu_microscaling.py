@@ -324,3 +324,11 @@ def test_held_weight_from_its_parts(hip_device):
         memfast.mx_linear(x.cpu(), t)
     with pytest.raises(ValueError, match="per output"):
         memfast.mx_linear(x, t, x[0])
+
+
+def test_gradients_are_not_differentiable(hip_device):
+    x, w = (data(64, 64, torch.float32, hip_device, s).requires_grad_(True) for s in (1, 2))
+    dx, = torch.autograd.grad(memfast.mx_linear(x, w).square().sum(), x, create_graph=True)
+    assert dx.shape == x.shape
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
