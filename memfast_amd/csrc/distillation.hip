@@ -455,7 +455,7 @@ struct TopArgs {
 constexpr int TOP_LIST = 2048;      // candidates of a row
 
 struct TopShared {
-    u64 list[TOP_LIST];
+    u64 list[TOP_LIST];     // in whole steps of rank_list
     u32 ranks[TOP_LIST];
     u64 bounds[16];
     u32 counts[256];
@@ -469,12 +469,31 @@ __device__ __forceinline__ float value_of(u64 key) {
     return __uint_as_float(order >> 31 ? order ^ 0x80000000u : ~order);
 }
 
+// A thread's listed key is held back until it has another: most have none or one, and those go into the
+// list together, with one atomic a wave, instead of one wait for the LDS each.
+__device__ __forceinline__ void list_key(TopShared &sh, u64 key) {
+    const u32 at = atomicAdd(&sh.found, 1u);
+    if (at < u32(TOP_LIST)) sh.list[at] = key;
+}
+
+__device__ __forceinline__ void list_pending(TopShared &sh, u64 &pending) {
+    const u64 mask = __ballot(pending != 0);
+    if (mask == 0) return;
+    u32 first = 0;
+    if ((threadIdx.x & 63) == 0) first = atomicAdd(&sh.found, u32(__popcll(mask)));
+    first = __builtin_amdgcn_readfirstlane(first);
+    const u32 at = first + __builtin_amdgcn_mbcnt_hi(u32(mask >> 32), __builtin_amdgcn_mbcnt_lo(u32(mask), 0));
+    if (pending != 0 && at < u32(TOP_LIST)) sh.list[at] = pending;
+    pending = 0;
+}
+
 // Lists a piece's classes from `bound` (of the value `least`) on, and adds the others' exp2(x c + b)
 // to the sum. A NaN that is not listed makes the sum one (with least = -inf every piece's keys are
 // compared, and a NaN that belongs there is listed). Changes x.
 template <typename T>
 __device__ __forceinline__ void sift(const Row<T> &row, int i, float (&x)[PIECE<T>], float least,
-                                     u64 bound, float c, float b, TopShared &sh, float &sum) {
+                                     u64 bound, float c, float b, TopShared &sh, u64 &pending,
+                                     float &sum) {
     constexpr int P = PIECE<T>;
     if (largest(x, -INFINITY) >= least || i < row.first || i >= row.last) {
 #pragma unroll
@@ -483,8 +502,8 @@ __device__ __forceinline__ void sift(const Row<T> &row, int i, float (&x)[PIECE<
             if (x[j] < least || index < 0 || index >= row.v) continue;
             const u64 key = key_of(x[j], index);
             if (key >= bound) {
-                const u32 at = atomicAdd(&sh.found, 1u);
-                if (at < u32(TOP_LIST)) sh.list[at] = key;
+                if (pending != 0) list_key(sh, pending);
+                pending = key;
                 x[j] = -INFINITY;       // adds nothing
             }
         }
@@ -530,23 +549,48 @@ __device__ u64 exact_bound(const Row<T> &row, int k, TopShared &sh) {
     }
 }
 
-// Every listed key's rank among the list, its comparisons shared by several threads.
+// Every listed key's rank among the list, its comparisons shared by several threads, eight at a time.
 template <int THREADS> __device__ void rank_list(TopShared &sh, int found) {
+    constexpr int STEP = 8;
+    const int steps = (found + STEP - 1) / STEP;
     for (int j = threadIdx.x; j < found; j += THREADS) sh.ranks[j] = 0;
+    for (int j = found + threadIdx.x; j < steps * STEP; j += THREADS) sh.list[j] = 0;   // above nothing
     __syncthreads();
-    const int parts = max(1, THREADS / found);
-    const int length = (found + parts - 1) / parts;
+    const int parts = max(1, min(THREADS / found, steps));
+    const int length = (steps + parts - 1) / parts;
     for (int e = threadIdx.x; e < found * parts; e += THREADS) {
-        const int j = e % found, from = e / found * length, to = min(from + length, found);
+        const int j = e % found, from = e / found * length, to = min(from + length, steps);
         const u64 key = sh.list[j];
         u32 above = 0;
-        for (int o = from; o < to; ++o) above += sh.list[o] > key;
+        for (int o = from; o < to; ++o)
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) above += sh.list[o * STEP + i] > key;
         if (parts == 1)
             sh.ranks[j] = above;
         else
             atomicAdd(&sh.ranks[j], above);
     }
     __syncthreads();
+}
+
+// The q-th largest key of the wave's lanes, bit by bit; 0 where fewer lanes have one. Keys differ but
+// for zeros, and the bits of an index above the 20th are ones.
+__device__ __forceinline__ u64 nth_of_wave(u64 key, int q) {
+    u64 mask = ~u64(0), prefix = 0;
+    int left = q;
+    for (int bit = 63; bit >= 0; --bit) {
+        const u64 ones = __ballot(key >> bit & 1) & mask;
+        const int count = __popcll(ones);
+        if (count >= left) {
+            mask = ones;
+            prefix |= u64(1) << bit;
+        } else {
+            left -= count;
+            mask &= ~ones;
+        }
+        if (__popcll(mask) == 1) return __shfl((unsigned long long)key, __ffsll((unsigned long long)mask) - 1);
+    }
+    return prefix;
 }
 
 // Sorts the list and leaves its first k keys; the others join the sum, in their order, because the
@@ -605,37 +649,33 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         const int i = threadIdx.x + t * THREADS;
         if (i < row.pieces) first[t] = row.template piece<true>(i, T(-INFINITY));
     }
-    // The largest key of this thread (the first of equal ones), 0 for none.
+    // The largest key of this thread (the first of equal ones), 0 for none: its piece, then its place there.
     float top = -INFINITY;
+    v4u holder = first[0];
+    int at = 0;
 #pragma unroll
     for (int t = 0; t < ITEMS; ++t)
         if (int(threadIdx.x) + t * THREADS < row.pieces) {
             float x[P];
             values(t, x);
-            top = largest(x, top);
+            const float m = largest(x, -INFINITY);
+            if (m > top) {
+                top = m;
+                holder = first[t];
+                at = t;
+            }
         }
-    int at = -1;
+    u64 best = 0;
+    {
+        float x[P];
+        unpack<T>(holder, x);
+        int where = -1;
 #pragma unroll
-    for (int t = ITEMS - 1; t >= 0; --t) {
-        const int i = threadIdx.x + t * THREADS;
-        if (i < row.pieces) {
-            float x[P];
-            values(t, x);
-            int where = -1;
-#pragma unroll
-            for (int j = P - 1; j >= 0; --j) where = x[j] == top ? j : where;
-            const int index = i * P - row.off + where;
-            if (where >= 0 && index >= 0 && index < row.v) at = index;
-        }
+        for (int j = P - 1; j >= 0; --j) where = x[j] == top ? j : where;
+        const int i = threadIdx.x + at * THREADS, index = i * P - row.off + where;
+        if (i < row.pieces && where >= 0 && index >= 0 && index < row.v) best = key_of(top, index);
     }
-    u64 best = at < 0 ? 0 : key_of(top, at);
-    for (int size = 2; size <= 64; size <<= 1)      // lanes in descending order
-        for (int stride = size >> 1; stride; stride >>= 1) {
-            const u64 other = __shfl_xor((unsigned long long)best, stride);
-            const bool larger = ((lane & size) == 0) == ((lane & stride) == 0);
-            best = larger ? max(best, other) : min(best, other);
-        }
-    const u64 mine = __shfl((unsigned long long)best, (a.k + WAVES - 1) / WAVES - 1);
+    const u64 mine = nth_of_wave(best, (a.k + WAVES - 1) / WAVES);
     if (lane == 0) sh.bounds[wave] = mine;
     __syncthreads();
     u64 bound = sh.bounds[0];
@@ -645,15 +685,17 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     float least = bound ? value_of(bound) : -INFINITY;      // 0 lists everything
     const float b = least == -INFINITY ? 0.0f : -least * c;
     float sum = 0.0f;
+    u64 pending = 0;
 #pragma unroll
     for (int t = 0; t < ITEMS; ++t) {
         const int i = threadIdx.x + t * THREADS;
         if (i < row.pieces) {
             float x[P];
             values(t, x);
-            sift(row, i, x, least, bound, c, b, sh, sum);
+            sift(row, i, x, least, bound, c, b, sh, pending, sum);
         }
     }
+    list_pending(sh, pending);
     // A NaN is found by the sum: it may be among the largest, which comparisons of values miss.
     bool exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
     if (!exact && row.pieces > ITEMS * THREADS) {
@@ -663,8 +705,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         for_pieces<THREADS, true>(row, ITEMS * THREADS, -INFINITY, [&](int i, auto &x) {
 #pragma unroll
             for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
-                sift(row, i + t * THREADS, x[t], least, bound, c, b, sh, sum);
+                sift(row, i + t * THREADS, x[t], least, bound, c, b, sh, pending, sum);
         });
+        list_pending(sh, pending);
         exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
     }
     if (exact) {
@@ -675,8 +718,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         for_pieces<THREADS, false>(row, 0, -INFINITY, [&](int i, auto &x) {
 #pragma unroll
             for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
-                sift(row, i + t * THREADS, x[t], -INFINITY, bound, c, b, sh, sum);
+                sift(row, i + t * THREADS, x[t], -INFINITY, bound, c, b, sh, pending, sum);
         });
+        list_pending(sh, pending);
         __syncthreads();
     }
     keep_first<THREADS>(sh, a.k, c, b, sum);
@@ -748,14 +792,19 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
         hipStream_t s = static_cast<hipStream_t>(stream);
-        // A wave needs a class in every lane for its bound, and no more than its 64. Where the
-        // rows fill the chip several times over, eight waves leave two workgroups to a compute unit.
+        // A wave needs a class in every lane for its bound, and no more than its 64. Few rows take
+        // sixteen waves each. Where the rows fill the chip several times over, eight waves leave room
+        // for two or three workgroups on a compute unit, and one lists while others load; the longer
+        // stretch pays where the short one would list many classes (us, 2048 x 128000 BF16, 8 / 16 pieces: k =
+        // 64 168 / 185, k = 250 407 / 309; 64 rows, 8 / 16 waves 36 / 28).
         const i64 pieces = v / PIECE<T>;
         const auto fits = [&](int waves) { return pieces >= 64 * waves && k <= 64 * waves; };
-        if (n >= 512 && fits(8))
+        if (n >= 512 && fits(8) && k * v <= 256 * 4096 * PIECE<T>)
+            hipLaunchKernelGGL((k_top<T, 8, 8>), dim3(unsigned(n)), dim3(512), 0, s, args);
+        else if (n >= 512 && fits(8))
             hipLaunchKernelGGL((k_top<T, 8, 16>), dim3(unsigned(n)), dim3(512), 0, s, args);
         else if (fits(16) || k > 256)
-            hipLaunchKernelGGL((k_top<T, 16, 8>), dim3(unsigned(n)), dim3(1024), 0, s, args);
+            hipLaunchKernelGGL((k_top<T, 16, 16>), dim3(unsigned(n)), dim3(1024), 0, s, args);
         else
             hipLaunchKernelGGL((k_top<T, 4, 8>), dim3(unsigned(n)), dim3(256), 0, s, args);
         return check_launch("top logits");
