@@ -57,14 +57,26 @@ template <int WAVES> __device__ LogSum block_merge(LogSum v, float c, float *scr
     return all;
 }
 
-template <int WAVES> __device__ float block_sum(float v, float *scratch) {
+template <int WAVES, typename V> __device__ V block_sum(V v, float *scratch) {
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    V *part = reinterpret_cast<V *>(scratch);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    V all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all += part[w];
+    return all;
+}
+
+template <int WAVES> __device__ float block_max(float v, float *scratch) {
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
     __syncthreads();
-    float all = 0.0f;
+    float all = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) all += scratch[w];
+    for (int w = 0; w < WAVES; ++w) all = fmaxf(all, scratch[w]);
     return all;
 }
 
@@ -173,11 +185,10 @@ struct DistillArgs {
     void *grad;              // [n, v]
 };
 
-// p d - p + q with d = log(p / q), as p (d + exp(-d) - 1) where that stays in range. d is formed
-// and expanded in 64 bits: its terms cancel to the order of d^2, and there are k + 1 of them a row.
-__device__ __forceinline__ float bucket_loss(float p, float q, double d) {
-    if (p == 0.0f) return q;
-    return d > -8.0 ? p * float(d + expm1(-d)) : p * float(d) + (q - p);
+// p d - p + q with d = log(p / q), as p (d + exp(-d) - 1) where that stays in range.
+__device__ __forceinline__ double bucket_loss(double p, double q, double d) {
+    if (p == 0.0) return q;
+    return d > -8.0 ? p * (d + expm1(-d)) : p * d + (q - p);
 }
 
 __device__ __forceinline__ float value_at(const void *values, int type, i64 i) {
@@ -252,7 +263,7 @@ __device__ __forceinline__ void write_rest(const Row<T> &row, const u32 *bits, f
 template <typename T, int WAVES, bool GRAD>
 __global__ __launch_bounds__(64 * WAVES, 5) void k_distill(const DistillArgs a) {
     extern __shared__ u32 bits[];
-    __shared__ float scratch[2 * WAVES];
+    __shared__ __align__(16) float scratch[2 * WAVES];     // two floats or one double a wave
     constexpr int THREADS = 64 * WAVES;
     const i64 r = blockIdx.x;
     const float weight = a.weight ? a.weight[r] : 1.0f;
@@ -271,13 +282,7 @@ __global__ __launch_bounds__(64 * WAVES, 5) void k_distill(const DistillArgs a) 
     const bool bad = mark_entries(indices, a.k, a.v, row.off, bits, (row.off + a.v + 31) / 32,
                                   THREADS);
 
-    LogSum teacher, entries, rest;
-    if (!bad)
-        for (i64 j = threadIdx.x; j < a.k; j += THREADS)
-            if (indices[j] >= 0) {
-                teacher.add(value_at(a.values, a.values_type, first + j), c);
-                entries.add(float(s[indices[j]]), c);
-            }
+    LogSum rest;
     for_pieces<THREADS, !GRAD>(row, 0, -INFINITY, [&](int i, auto &x) {
         constexpr int COUNT = sizeof(x) / sizeof(x[0]);
         float top = rest.m;
@@ -300,51 +305,65 @@ __global__ __launch_bounds__(64 * WAVES, 5) void k_distill(const DistillArgs a) 
 #pragma unroll
             for (int j = 0; j < PIECE<T>; ++j) rest.s += power(x[t][j], ref, c);
     });
-    teacher = block_merge<WAVES>(teacher, c, scratch);
-    entries = block_merge<WAVES>(entries, c, scratch);
     rest = block_merge<WAVES>(rest, c, scratch);
 
-    const float tail = a.tail ? a.tail[r] * a.temperature : -INFINITY;   // as a logit
-    const bool empty = teacher.m == -INFINITY && teacher.s == 0.0f && tail == -INFINITY;
-    teacher.add(tail, c);
-    LogSum all = rest;
-    all.merge(entries.m, entries.s, c);
-    const float t0 = teacher.ref(), z0 = all.ref();
-    // log(p / q) = ((t - t0) - (z - z0)) / T - shift.
+    // The entries and the buckets, k + 1 values a row, are taken in 64 bits: near its teacher, a
+    // student's gradient is a small difference of q and p.
     const double cold = 1.0 / double(a.temperature);
-    const double shift = log(double(teacher.s)) - log(double(all.s));
-    float loss = 0.0f;
+    const float tail = a.tail ? a.tail[r] * a.temperature : -INFINITY;   // as a logit
+    float most_t = tail, most_z = rest.m;
+    for (i64 j = threadIdx.x; j < a.k; j += THREADS)
+        if (!bad && indices[j] >= 0) {
+            most_t = fmaxf(most_t, value_at(a.values, a.values_type, first + j));
+            most_z = fmaxf(most_z, float(s[indices[j]]));
+        }
+    most_t = block_max<WAVES>(most_t, scratch);
+    most_z = block_max<WAVES>(most_z, scratch);
+    // What exponents are taken from; -inf stands for values that are all -inf.
+    const double t0 = most_t == -INFINITY ? 0.0 : double(most_t);
+    const double z0 = most_z == -INFINITY ? 0.0 : double(most_z);
+    double teacher = 0.0, student = 0.0;
+    for (i64 j = threadIdx.x; j < a.k; j += THREADS)
+        if (!bad && indices[j] >= 0) {
+            teacher += exp((double(value_at(a.values, a.values_type, first + j)) - t0) * cold);
+            student += exp((double(float(s[indices[j]])) - z0) * cold);
+        }
+    teacher = block_sum<WAVES>(teacher, scratch);
+    student = block_sum<WAVES>(student, scratch);
+    const double tail_mass = exp((double(tail) - t0) * cold);
+    const double rest_scale = exp((double(rest.ref()) - z0) * cold);
+    teacher += tail_mass;
+    student += rest_scale * double(rest.s);
+    const bool empty = most_t == -INFINITY && teacher == 0.0;
+    // log(p / q) = ((t - t0) - (z - z0)) / T - shift.
+    const double shift = log(teacher) - log(student);
+    double loss = 0.0;
     for (i64 j = threadIdx.x; j < a.k; j += THREADS) {
         float grad = 0.0f;
         if (bad) {
             grad = NAN;
         } else if (indices[j] >= 0 && !empty) {
-            const float t = value_at(a.values, a.values_type, first + j);
-            const float z = float(s[indices[j]]);
-            const float p = power(t, t0, c) / teacher.s;
-            const float q = power(z, z0, c) / all.s;
-            loss += bucket_loss(p, q, ((double(t) - t0) - (double(z) - z0)) * cold - shift);
-            grad = q - p;
+            const double t = (double(value_at(a.values, a.values_type, first + j)) - t0) * cold;
+            const double z = (double(float(s[indices[j]])) - z0) * cold;
+            const double p = exp(t) / teacher, q = exp(z) / student;
+            loss += bucket_loss(p, q, t - z - shift);
+            grad = float(q - p);
         }
         a.entry_grad[r * a.k + j] = grad;
     }
     loss = block_sum<WAVES>(loss, scratch);
     float coef = 0.0f;
-    {   // the bucket of all other classes, by every thread
-        if (bad) {
-            loss = coef = NAN;
-        } else if (!empty) {
-            const float p = power(tail, t0, c) / teacher.s;
-            const float scale = power(rest.ref(), z0, c) / all.s;
-            const float q = rest.s * scale;
-            const double student = (double(rest.ref()) - z0) * cold + log(double(rest.s));
-            loss += bucket_loss(p, q, (double(tail) - t0) * cold - student - shift);
-            // Without any finite class outside the entries there is nothing to scale.
-            coef = rest.s == 0.0f ? (p > 0.0f ? NAN : 0.0f) : scale - p / rest.s;
-        }
+    if (bad) {                  // and the bucket of all other classes, by every thread
+        loss = coef = NAN;
+    } else if (!empty) {
+        const double p = tail_mass / teacher, scale = rest_scale / student, sum = double(rest.s);
+        const double z = (double(rest.ref()) - z0) * cold + log(sum);
+        loss += bucket_loss(p, sum * scale, (double(tail) - t0) * cold - z - shift);
+        // Without any finite class outside the entries there is nothing to scale.
+        coef = sum == 0.0 ? (p > 0.0 ? NAN : 0.0f) : float(scale - p / sum);
     }
     if (threadIdx.x == 0) {
-        a.row_loss[r] = loss * a.temperature * a.temperature;
+        a.row_loss[r] = float(loss * a.temperature * a.temperature);
         a.ref[r] = rest.ref();
         a.coef[r] = coef;
     }
@@ -460,7 +479,7 @@ struct TopShared {
     u64 bounds[16];
     u32 counts[256];
     u32 digit, remaining, found, last;
-    float scratch[32];
+    alignas(16) float scratch[32];
 };
 
 // The value of a key's logit, in FP32; NaN for the largest key.

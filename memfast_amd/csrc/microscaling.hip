@@ -92,11 +92,11 @@ struct MxArgs {
 };
 
 // ---- few rows --------------------------------------------------------------
-// Up to 64 rows of x: the weight's bytes bound it, so each is loaded once, straight into the operand
+// Few rows of x: the weight's bytes bound it, so each is loaded once, straight into the operand
 // registers. A workgroup takes 16 rows of W; its eight waves split the segments and add their
 // sums in LDS in the order of the waves. QUANTIZE: the workgroup quantizes x into LDS itself, while
 // its first weights are on their way, which saves a launch; else Q(x) is read from the cache.
-constexpr int FEW_WAVES = 8, FEW_TILE = 16;
+constexpr int FEW_WAVES = 8, FEW_TILE = 16, AHEAD = 2;
 
 __device__ __forceinline__ v4f mfma_few(v4u a, v4u b, v4f c, u32 sa, u32 sb) {
     const v8i av = {int(a.x), int(a.y), int(a.z), int(a.w), 0, 0, 0, 0};
@@ -124,14 +124,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_mx_few(const MxArgs a) {
     const i64 o = min(o0 + row, a.o - 1);
     const u8 *wc = a.wc + o * a.segs * SEG_BYTES + block * 16, *ws = a.ws.data + o * a.ws.row;
 
-    v4u w[2];
-    v2u sw;
-    auto load_weight = [&](i64 s) {
-        w[0] = *reinterpret_cast<const v4u *>(wc + s * SEG_BYTES);
-        w[1] = *reinterpret_cast<const v4u *>(wc + s * SEG_BYTES + 64);
-        sw = *reinterpret_cast<const v2u *>(ws + s * a.ws.seg);
+    // AHEAD segments of the weight are under way: a compute unit's waves then keep more bytes in flight
+    // for the memory's latency.
+    v4u w[AHEAD][2];
+    v2u sw[AHEAD];
+    auto load_weight = [&](int slot, i64 s) {
+        if (s < last) {
+            w[slot][0] = *reinterpret_cast<const v4u *>(wc + s * SEG_BYTES);
+            w[slot][1] = *reinterpret_cast<const v4u *>(wc + s * SEG_BYTES + 64);
+            sw[slot] = *reinterpret_cast<const v2u *>(ws + s * a.ws.seg);
+        }
     };
-    if (first < last) load_weight(first);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load_weight(i, first + i);
 
     const i64 pitch = few_pitch(a.segs);
     u8 *const staged_scales = staged + a.n * pitch;
@@ -153,24 +158,32 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_mx_few(const MxArgs a) {
     }
 
     v4f acc[NT] = {};
-    for (i64 s = first; s < last; ++s) {
-        const v4u w0 = w[0], w1 = w[1];
-        const v2u scale = sw;
-        if (s + 1 < last) load_weight(s + 1);
-        const u32 sw0 = scale.x >> (8 * block), sw1 = scale.y >> (8 * block);
+    auto multiply = [&](int slot, i64 s) {
+        v4u x0[NT], x1[NT];
+        v2u sx[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const i64 r = min(i64(16 * t + row), a.n - 1);
             const u8 *xc = QUANTIZE ? staged + r * pitch : a.xc + r * a.segs * SEG_BYTES;
             const u8 *xs = QUANTIZE ? staged_scales + (r * a.segs + s) * SEG_SCALES
                                     : a.xs.data + r * a.xs.row + s * a.xs.seg;
-            const v4u x0 = *reinterpret_cast<const v4u *>(xc + s * SEG_BYTES + block * 16);
-            const v4u x1 = *reinterpret_cast<const v4u *>(xc + s * SEG_BYTES + 64 + block * 16);
-            const v2u sx = *reinterpret_cast<const v2u *>(xs);
-            acc[t] = mfma_few(x0, w0, acc[t], sx.x >> (8 * block), sw0);
-            acc[t] = mfma_few(x1, w1, acc[t], sx.y >> (8 * block), sw1);
+            x0[t] = *reinterpret_cast<const v4u *>(xc + s * SEG_BYTES + block * 16);
+            x1[t] = *reinterpret_cast<const v4u *>(xc + s * SEG_BYTES + 64 + block * 16);
+            sx[t] = *reinterpret_cast<const v2u *>(xs);
         }
-    }
+        const v4u w0 = w[slot][0], w1 = w[slot][1];
+        const u32 sw0 = sw[slot].x >> (8 * block), sw1 = sw[slot].y >> (8 * block);
+        load_weight(slot, s + AHEAD);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            acc[t] = mfma_few(x0[t], w0, acc[t], sx[t].x >> (8 * block), sw0);
+            acc[t] = mfma_few(x1[t], w1, acc[t], sx[t].y >> (8 * block), sw1);
+        }
+    };
+    for (i64 s = first; s < last; s += AHEAD)
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (s + i < last) multiply(i, s + i);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -347,27 +360,29 @@ struct ProductPlan {
     bool quantize;   // Q(x) goes through memory
 };
 
-constexpr i64 FEW_ROWS = 64;
-constexpr i64 FEW_QUANTIZE = 32768;   // values of x that every workgroup may quantize again
+// k_mx_few reads Q(x) again for every 16 rows of W, k_mx_tile waits longer where it has few tiles (us, few /
+// tiles, n x k x o): 16 x 4096 x 11008 9.7 / 9.3, 24 of them 12.0 / 9.4, 64 21.6 / 9.8; 24 x 11008 x 4096
+// 10.3 / 18.9, 64 of them 16.9 / 19.2, 64 x 4096 x 4096 8.0 / 8.8.
+constexpr i64 FEW_ROWS = 64, FEW_ROWS_WIDE = 16, WIDE = 8192;
+// Values of x that every workgroup may quantize again: 1 x 4096 x 11008 7.5 us against 8.1 and a launch of 3,
+// 8 x 4096 x 11008 13.2 against 8.7 and 3.
+constexpr i64 FEW_QUANTIZE = 16384;
 
-static ProductPlan plan_product(i64 n, i64 k, bool keep) {
-    const bool few = n <= FEW_ROWS;
+static ProductPlan plan_product(i64 n, i64 k, i64 o, bool keep) {
+    const bool few = n <= (o < WIDE ? FEW_ROWS : FEW_ROWS_WIDE);
     return {few, keep || !few || n > 16 || n * segments(k) * SEG > FEW_QUANTIZE};
 }
 
-template <typename T> static int launch_few(const MxArgs &args, const ProductPlan &plan, hipStream_t s) {
-    const dim3 grid(unsigned((args.o + FEW_TILE - 1) / FEW_TILE)), block(64 * FEW_WAVES);
-    if (!plan.quantize)
-        hipLaunchKernelGGL((k_mx_few<T, 1, true>), grid, block, few_lds(args.n, args.segs), s, args);
-    else if (args.n <= 16)
-        hipLaunchKernelGGL((k_mx_few<T, 1, false>), grid, block, 0, s, args);
-    else if (args.n <= 32)
-        hipLaunchKernelGGL((k_mx_few<T, 2, false>), grid, block, 0, s, args);
-    else if (args.n <= 48)
-        hipLaunchKernelGGL((k_mx_few<T, 3, false>), grid, block, 0, s, args);
-    else
-        hipLaunchKernelGGL((k_mx_few<T, 4, false>), grid, block, 0, s, args);
+template <typename T, int NT, bool QUANTIZE> static int launch_few_as(const MxArgs &args, hipStream_t s) {
+    hipLaunchKernelGGL((k_mx_few<T, NT, QUANTIZE>), dim3(unsigned((args.o + FEW_TILE - 1) / FEW_TILE)),
+                       dim3(64 * FEW_WAVES), QUANTIZE ? few_lds(args.n, args.segs) : 0, s, args);
     return check_launch("microscaled product");
+}
+
+template <typename T> static int launch_few(const MxArgs &args, const ProductPlan &plan, hipStream_t s) {
+    if (!plan.quantize) return launch_few_as<T, 1, true>(args, s);
+    if (args.n <= 16) return launch_few_as<T, 1, false>(args, s);
+    return args.n <= 32 ? launch_few_as<T, 2, false>(args, s) : launch_few_as<T, 4, false>(args, s);
 }
 
 template <typename T, int WN, int WO, int TN, int TO, int STAGES>
@@ -396,6 +411,9 @@ template <typename T> static int launch_tiles(const MxArgs &args, hipStream_t s)
         return launch_tile<T, 2, 4, 2, 2, 2>(args, s);
     }
     if (tiles(128, 128) >= 256) return launch_tile<T, 2, 2, 2, 2, 2>(args, s);
+    // With a tile or less for each compute unit, more stages stand in for other workgroups: 64 x 4096 x
+    // 11008 14.7 / 9.8 us with two / four.
+    if (tiles(64, 64) <= 256) return launch_tile<T, 2, 2, 1, 1, 4>(args, s);
     return launch_tile<T, 2, 2, 1, 1, 2>(args, s);
 }
 
@@ -441,7 +459,7 @@ int mf_mx_linear_sizes(int64_t n, int64_t k, int64_t o, int32_t held, int32_t ke
                        int64_t *workspace) {
     if (!xcodes || !workspace || !sizes_ok(n, k) || !sizes_ok(o, k))
         return fail(MF_E_INVALID, "invalid microscaled product sizes");
-    const ProductPlan plan = plan_product(n, k, keep);
+    const ProductPlan plan = plan_product(n, k, o, keep);
     *xcodes = plan.quantize ? n * segments(k) * SEG_BYTES : 0;
     *workspace = held && !plan.few ? even(o) * segments(k) * SEG_SCALES : 0;
     return MF_OK;
@@ -454,7 +472,7 @@ int mf_mx_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx,
     if (!known_type(type) || !sizes_ok(n, k) || !out || !x || (n > 1 && ldx < k) ||
         !operand_ok(weight ? weight : wcodes, o, k, weight ? ldw : k, wcodes, wscales))
         return fail(MF_E_INVALID, "invalid microscaled product arguments");
-    const ProductPlan plan = plan_product(n, k, keep);
+    const ProductPlan plan = plan_product(n, k, o, keep);
     const i64 segs = segments(k);
     const bool turn = !weight && !plan.few;
     if (plan.quantize && !operand_ok(x, n, k, ldx, xcodes, xscales))
