@@ -218,8 +218,9 @@ __device__ __forceinline__ v16f mfma_step(v4u a, v4u b, v16f c, u32 sa, u32 sb) 
 
 // WN x WO waves of TN x TO tiles of 32 x 32. A stage is one segment of every row of the tile (128 bytes of
 // codes and 8 of scales), copied to LDS without passing through registers, STAGES - 1 stages ahead of
-// the matrix cores. The 16-byte pieces of row r lie rotated by r & 7, so that the eight rows
-// that a read serves at once are in different banks.
+// the matrix cores. The 16-byte pieces of row r lie at p ^ (r / 2 & 7): the sixteen rows that a read serves
+// at once, two to the 256 bytes of the banks, are then in different ones (p ^ (r & 7) has pairs of them
+// meet: 78 against 70 us at 2048 x 4096 x 11008).
 template <typename T, int WN, int WO, int TN, int TO, int STAGES>
 __global__ __launch_bounds__(64 * WN * WO) void k_mx_tile(const MxArgs a) {
     constexpr int BN = 32 * WN * TN, BO = 32 * WO * TO, ROWS = BN + BO, WAVES = WN * WO;
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(64 * WN * WO) void k_mx_tile(const MxArgs a) {
     for (int i = 0; i < COPIES; ++i) {
         const int r = (first_copy + i) * 8 + (lane >> 3);
         const i64 at = r < BN ? min(i64(r), a.n - n0 - 1) : min(i64(r - BN), a.o - o0 - 1);
-        offset[i] = u32(at * pitch) + u32(((lane & 7) ^ (lane >> 3)) * 16);
+        offset[i] = u32(at * pitch) + u32(((lane ^ r >> 1) & 7) * 16);
     }
     // Two rows' scales a lane; the even pitch of a segment holds the second of the last pair.
     const bool copies_scales = __builtin_amdgcn_readfirstlane(wave) < SCALE_COPIES;
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(64 * WN * WO) void k_mx_tile(const MxArgs a) {
                 *reinterpret_cast<const v2u *>(scales + (wo + 32 * j) * SEG_SCALES), half);
         auto step = [&](auto number) {
             constexpr int STEP = decltype(number)::value;
-            const int piece = ((2 * STEP + half) ^ (row & 7)) * 16;
+            const int piece = ((2 * STEP + half) ^ (row >> 1 & 7)) * 16;
             v4u fx[TN], fw[TO];
 #pragma unroll
             for (int i = 0; i < TN; ++i)
@@ -399,10 +400,10 @@ static int launch_tile(const MxArgs &args, hipStream_t s) {
 
 template <typename T> static int launch_tiles(const MxArgs &args, hipStream_t s) {
     // The largest tile of which every compute unit gets one (us, 64 x 64 / 128 x 128 / 128 x 256):
-    // 2048 x 11008 x 4096 86 / 60 / 56, 300 x 4096 x 4096 11.4 / 15.6 / 20.3, 777 x 1500 x 1111
-    // 5.7 / 9.3 / 11.2. A 256 x 256 tile is 1.17 times as fast as two of 128 x 256 (43 against 50 us at
-    // 4096^3) where it does not leave more of the last round empty (81 against 73 us at
-    // 2048 x 4096 x 11008). A third stage costs the second workgroup of a compute unit: 74 against 60 us.
+    // 2048 x 11008 x 4096 86 / 58 / 54, 777 x 1500 x 1111 5.7 / 9.2 / 11.0. A 256 x 256 tile is 1.14 times
+    // as fast as two of 128 x 256 (43 against 49 us at 4096^3) where it does not leave more of the last
+    // round empty (77 against 70 us at 2048 x 4096 x 11008). A third stage takes 128 x 256 from 54 to 55 us,
+    // and 128 x 128 the second workgroup of a compute unit: from 60 to 74 us.
     const auto tiles = [&](i64 bn, i64 bo) { return (args.n + bn - 1) / bn * ((args.o + bo - 1) / bo); };
     const auto rounds = [&](i64 bn, i64 bo) { return (tiles(bn, bo) + 255) / 256; };
     if (tiles(128, 256) >= 256) {

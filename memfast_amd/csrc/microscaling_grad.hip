@@ -174,9 +174,9 @@ __device__ __forceinline__ void grad_tile(const GradArgs &a, u32 block, u8 *stag
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
         const int at = (first_copy + i) * 1024;
-        if (at < A_BYTES && !DEPTH_ROWS) {      // rows of 64 values, 8 pieces rotated by the row
+        if (at < A_BYTES && !DEPTH_ROWS) {      // rows of 64 values, 8 pieces at p ^ (r / 2 & 7)
             const int piece = at / 16 + lane, r = piece >> 3;
-            offset[i] = u32(min(i64(r), a.rows - m0 - 1) * a.lda * 2) + u32(((piece ^ r) & 7) * 16);
+            offset[i] = u32(min(i64(r), a.rows - m0 - 1) * a.lda * 2) + u32(((piece ^ r >> 1) & 7) * 16);
         } else if (at < A_BYTES) {
             constexpr int PIECES = BM / 8;
             const int piece = at / 16 + lane, r = piece / PIECES;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs &a, u32 block, u8 *stag
                 fa[i] = DEPTH_ROWS
                             ? transposed(tile + at_a[i] + s * 16 * BM * 2, 4 * BM * 2)
                             : *reinterpret_cast<const v8bf *>(
-                                  tile + at_a[i] + ((2 * s + half) ^ (lane & 7)) * 16);
+                                  tile + at_a[i] + ((2 * s + half) ^ (lane >> 1 & 7)) * 16);
 #pragma unroll
             for (int j = 0; j < TC; ++j)
                 fb[j] = transposed(tile + at_b[j] + s * 16 * BC * 2, 4 * BC * 2);
@@ -346,10 +346,10 @@ static int launch_grad_tile(const GradArgs &args, hipStream_t s) {
     return check_launch("microscaled gradient");
 }
 
-// The tile whose rounds over the 256 compute units take the least: a round of 256 x 256 takes 123 us
-// at a depth of 4096, one of 192 x 256 0.75 and one of 128 x 128 (two a compute unit) 0.63 of that. us,
-// 256 x 256 / 192 x 256 / 128 x 128, n x k x o: dx of 2048 x 11008 x 4096 (344 / 473 / 1376 tiles) 223 / 189 / 273, dw
-// of it 189 / 211 / 255, dx of 2048 x 4096 x 11008 265 / 222 / 204, dx of 4096^3 126 / 172 / 164.
+// The tile whose rounds over the 256 compute units take the least: a round of 256 x 256 takes 117 us
+// at a depth of 4096, one of 192 x 256 0.75 and one of 128 x 128 (two a compute unit) 0.65 of that. us,
+// 256 x 256 / 192 x 256 / 128 x 128, n x k x o: dx of 2048 x 11008 x 4096 (344 / 473 / 1376 tiles) 220 / 187 / 268, dw
+// of it 187 / 206 / 251, dx of 2048 x 4096 x 11008 264 / 220 / 198, dx of 4096^3 116 / 162 / 159.
 // Where 128 x 128 leaves compute units without a tile, 64 x 64: dx of 512 x 1024 x 1024 8 against 15 us. Few
 // small tiles wait for their copies: a third stage takes dx of 128 x 4096 x 4096 from 34 to 24 us; in
 // the larger ones it costs the second workgroup (282 -> 321 us).
@@ -358,7 +358,7 @@ template <typename T, bool DEPTH_ROWS> static int launch_grad(const GradArgs &ar
     const auto rounds = [](i64 tiles, i64 at_once) { return (tiles + at_once - 1) / at_once; };
     const i64 large = rounds(grad_tiles(args, 256, 256), 256) * 100;
     const i64 middle = rounds(grad_tiles(args, 192, 256), 256) * 75;
-    const i64 small = rounds(grad_tiles(args, 128, 128), 512) * 63;
+    const i64 small = rounds(grad_tiles(args, 128, 128), 512) * 65;
     if (large <= middle && large <= small) return launch_grad_tile<T, DEPTH_ROWS, 4, 2, 2, 4, 2>(args, s);
     if (middle <= small) return launch_grad_tile<T, DEPTH_ROWS, 2, 4, 3, 2, 2>(args, s);
     return launch_grad_tile<T, DEPTH_ROWS, 2, 2, 2, 2, 2>(args, s);
