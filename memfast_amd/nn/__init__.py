@@ -3,6 +3,7 @@
 from .conversion import convert_model, reset_read_events
 from .convolution import AnalogConv2d
 from .linear import AnalogLinear
+from .microscaled import MXLinear
 from .modules import Conv2d, Linear
 from .recurrent import AnalogGRU, AnalogGRUCell, AnalogRNN, AnalogRNNCell
 from .training import TrainableAnalogConv2d, TrainableAnalogLinear
@@ -13,5 +14,5 @@ HATConv2d = TrainableAnalogConv2d
 __all__ = [
     "Linear", "Conv2d", "AnalogLinear", "AnalogConv2d", "TrainableAnalogLinear",
     "TrainableAnalogConv2d", "HATLinear", "HATConv2d", "AnalogRNNCell", "AnalogRNN",
-    "AnalogGRUCell", "AnalogGRU", "convert_model", "reset_read_events",
+    "AnalogGRUCell", "AnalogGRU", "convert_model", "reset_read_events", "MXLinear",
 ]
