@@ -102,23 +102,38 @@ template <typename T> struct Row {
     // Any piece, `fill` outside the row.
     template <bool ONCE> __device__ __forceinline__ v4u piece(int i, T fill) const {
         if (i >= first && i < last) return whole<ONCE>(i);
-        Piece<T> part;
+        v4u part{};
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const int index = i * P - off + j;
-            part.v[j] = index >= 0 && index < v ? data[index] : fill;
+            const T x = index >= 0 && index < v ? data[index] : fill;
+            if constexpr (P == 4)
+                part[j] = __builtin_bit_cast(u32, x);
+            else
+                part[j / 2] |= u32(__builtin_bit_cast(unsigned short, x)) << 16 * (j % 2);
         }
-        return __builtin_bit_cast(v4u, part);
+        return part;
     }
 };
 
 template <typename T> __device__ __forceinline__ void unpack(v4u raw, float (&x)[PIECE<T>]) {
-    const Piece<T> p = __builtin_bit_cast(Piece<T>, raw);
+    // (By shifts: arrays of 16-bit values that live across branches go through memory.)
 #pragma unroll
-    for (int j = 0; j < PIECE<T>; ++j) x[j] = float(p.v[j]);
+    for (int j = 0; j < PIECE<T>; ++j) {
+        if constexpr (PIECE<T> == 4)
+            x[j] = __uint_as_float(raw[j]);
+        else
+            x[j] = float(__builtin_bit_cast(T, static_cast<unsigned short>(raw[j / 2] >> 16 * (j % 2))));
+    }
 }
 
-// Calls f(i, values) for this thread's pieces from `start` on: pieces i, i + THREADS, ... four at a
+template <typename T, int COUNT>
+__device__ __forceinline__ void unpack(const v4u (&raw)[COUNT], float (&x)[COUNT][PIECE<T>]) {
+#pragma unroll
+    for (int t = 0; t < COUNT; ++t) unpack<T>(raw[t], x[t]);
+}
+
+// Calls f(i, raw) for this thread's pieces from `start` on: pieces i, i + THREADS, ... four at a
 // time, so that as many loads are in flight (with one, a compute unit's waves keep too few bytes under
 // way to fill the memory's latency), then singly. Pieces that are not whole come last.
 template <int THREADS, bool ONCE, typename T, typename F>
@@ -127,23 +142,20 @@ __device__ __forceinline__ void for_pieces(const Row<T> &row, int start, float f
     int i = max(start, row.first) + int(threadIdx.x);
     for (; i + (LOADS - 1) * THREADS < row.last; i += LOADS * THREADS) {
         v4u raw[LOADS];
-        float x[LOADS][PIECE<T>];
 #pragma unroll
         for (int t = 0; t < LOADS; ++t) raw[t] = row.template whole<ONCE>(i + t * THREADS);
-#pragma unroll
-        for (int t = 0; t < LOADS; ++t) unpack<T>(raw[t], x[t]);
-        f(i, x);
+        f(i, raw);
     }
-    float x[1][PIECE<T>];
+    v4u raw[1];
     for (; i < row.last; i += THREADS) {
-        unpack<T>(row.template whole<ONCE>(i), x[0]);
-        f(i, x);
+        raw[0] = row.template whole<ONCE>(i);
+        f(i, raw);
     }
     const int side = threadIdx.x == 0 ? 0 : row.pieces - 1;
     if (threadIdx.x < 2 && side >= start && (side < row.first || side >= row.last) &&
         (threadIdx.x == 0 || row.pieces > 1)) {
-        unpack<T>(row.template piece<ONCE>(side, T(fill)), x[0]);
-        f(side, x);
+        raw[0] = row.template piece<ONCE>(side, T(fill));
+        f(side, raw);
     }
 }
 
@@ -247,8 +259,10 @@ __device__ __forceinline__ void write_rest(const Row<T> &row, const u32 *bits, f
             store_rest(grad, row, i, piece_bits<T>(bits, i), vec, zero);
         return;
     }
-    for_pieces<THREADS, true>(row, 0, 0.0f, [&](int i, auto &x) {
-        constexpr int COUNT = sizeof(x) / sizeof(x[0]);
+    for_pieces<THREADS, true>(row, 0, 0.0f, [&](int i, auto &raw) {
+        constexpr int COUNT = sizeof(raw) / sizeof(raw[0]);
+        float x[COUNT][PIECE<T>];
+        unpack<T>(raw, x);
 #pragma unroll
         for (int t = 0; t < COUNT; ++t) {
 #pragma unroll
@@ -283,8 +297,10 @@ __global__ __launch_bounds__(64 * WAVES, 5) void k_distill(const DistillArgs a) 
                                   THREADS);
 
     LogSum rest;
-    for_pieces<THREADS, !GRAD>(row, 0, -INFINITY, [&](int i, auto &x) {
-        constexpr int COUNT = sizeof(x) / sizeof(x[0]);
+    for_pieces<THREADS, !GRAD>(row, 0, -INFINITY, [&](int i, auto &raw) {
+        constexpr int COUNT = sizeof(raw) / sizeof(raw[0]);
+        float x[COUNT][PIECE<T>];
+        unpack<T>(raw, x);
         float top = rest.m;
 #pragma unroll
         for (int t = 0; t < COUNT; ++t) {
@@ -506,35 +522,80 @@ __device__ __forceinline__ void list_pending(TopShared &sh, u64 &pending) {
     pending = 0;
 }
 
-// Lists a piece's classes from `bound` (of the value `least`) on, and adds the others' exp2(x c + b)
-// to the sum. A NaN that is not listed makes the sum one (with least = -inf every piece's keys are
-// compared, and a NaN that belongs there is listed). Changes x.
-template <typename T>
-__device__ __forceinline__ void sift(const Row<T> &row, int i, float (&x)[PIECE<T>], float least,
-                                     u64 bound, float c, float b, TopShared &sh, u64 &pending,
-                                     float &sum) {
-    constexpr int P = PIECE<T>;
-    if (largest(x, -INFINITY) >= least || i < row.first || i >= row.last) {
+// What a thread has found in its pieces. A piece with a class from `least` on, the value of the key
+// `bound`, is held back whole and looked into when the thread meets another or at the end: most of a
+// wave's pieces have such a class in some lane, and going through the classes of each of them took twice
+// the instructions of all the rest.
+template <typename T> struct Sift {
+    static constexpr int P = PIECE<T>;
+    float c, b;
+    float least;
+    u64 bound;
+    float sum = 0.0f;       // of exp2(x c + b) over what is not listed
+    v4u held{};
+    int at = -1;            // which piece is held
+    u64 pending = 0;        // a key that is not yet in the list
+
+    // Pieces i, i + step, ... before `end`; those of a row's edges, which the caller knows, are held.
+    // A NaN in a piece that is not held makes the sum one.
+    template <int COUNT>
+    __device__ __forceinline__ void add(const Row<T> &row, TopShared &sh, v4u (&raw)[COUNT], int i,
+                                        int step, int end) {
+        u32 hold = 0;
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const int index = i * P - row.off + j;
-            if (x[j] < least || index < 0 || index >= row.v) continue;
-            const u64 key = key_of(x[j], index);
-            if (key >= bound) {
-                if (pending != 0) list_key(sh, pending);
-                pending = key;
-                x[j] = -INFINITY;       // adds nothing
+        for (int t = 0; t < COUNT; ++t) {
+            float x[P], part = 0.0f;
+            // (Unpacked one after the other: all of them at once take twice the registers.)
+            asm volatile("" : "+v"(raw[t]));
+            unpack<T>(raw[t], x);
+#pragma unroll
+            for (int j = 0; j < P; ++j) part += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
+            const int piece = i + t * step;
+            if (piece < end) {
+                const bool in = largest(x, -INFINITY) >= least || piece < row.first || piece >= row.last;
+                hold |= in ? 1u << t : 0u;
+                sum += in ? 0.0f : part;
             }
         }
-    }
+        for (; hold; hold &= hold - 1) {
+            if (at >= 0) look(row, sh);
+            const int t = __ffs(hold) - 1;
+            held = raw[0];
 #pragma unroll
-    for (int j = 0; j < P; ++j) sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
-}
+            for (int o = 1; o < COUNT; ++o) held = t == o ? raw[o] : held;
+            at = i + t * step;
+        }
+    }
+    // Lists the classes of the held piece from `bound` on and adds the others. A NaN is listed.
+    __device__ __forceinline__ void look(const Row<T> &row, TopShared &sh) {
+        float x[P];
+        unpack<T>(held, x);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            bool listed = false;
+            if (!(x[j] < least)) {
+                const int index = at * P - row.off + j;
+                const u64 key = key_of(x[j], index);
+                if (index >= 0 && index < row.v && key >= bound) {
+                    if (pending != 0) list_key(sh, pending);
+                    pending = key;
+                    listed = true;
+                }
+            }
+            if (!listed) sum += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
+        }
+        at = -1;
+    }
+    __device__ __forceinline__ void finish(const Row<T> &row, TopShared &sh) {
+        if (at >= 0) look(row, sh);
+        list_pending(sh, pending);
+    }
+};
 
 // The smallest selected key by radix selection, eight bits a pass over the row: for rows with
 // more than TOP_LIST candidates.
 template <typename T, int THREADS>
-__device__ u64 exact_bound(const Row<T> &row, int k, TopShared &sh) {
+__device__ u64 exact_bound(const Row<T> row, int k, TopShared &sh) {
     u64 prefix = 0;
     __syncthreads();
     if (threadIdx.x == 0) sh.remaining = k;
@@ -542,16 +603,20 @@ __device__ u64 exact_bound(const Row<T> &row, int k, TopShared &sh) {
         __syncthreads();
         for (int b = threadIdx.x; b < 256; b += THREADS) sh.counts[b] = 0;
         __syncthreads();
-        for_pieces<THREADS, false>(row, 0, 0.0f, [&](int i, auto &x) {
-            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
+        for_pieces<THREADS, false>(row, 0, 0.0f, [&](int i, auto &raw) {
+#pragma unroll
+            for (int t = 0; t < int(sizeof(raw) / sizeof(raw[0])); ++t) {
+                float x[PIECE<T>];
+                unpack<T>(raw[t], x);
 #pragma unroll
                 for (int j = 0; j < PIECE<T>; ++j) {
                     const int index = (i + t * THREADS) * PIECE<T> - row.off + j;
-                    const u64 key = key_of(x[t][j], index);
+                    const u64 key = key_of(x[j], index);
                     if (index >= 0 && index < row.v &&
                         (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8)))
                         atomicAdd(&sh.counts[key >> shift & 255u], 1u);
                 }
+            }
         });
         __syncthreads();
         if (threadIdx.x == 0) {   // the digit that holds the k-th largest
@@ -639,13 +704,16 @@ __device__ void keep_first(TopShared &sh, int k, float c, float b, float &sum) {
 }
 
 // One workgroup a row, one pass over it. Its first stretch (ITEMS pieces a thread, in registers) gives a
-// bound: of the largest classes of a wave's lanes the ceil(k / WAVES)-th largest, the smallest over
+// bound: of the largest classes of a wave's lanes the ceil(k / waves)-th largest, the smallest over
 // the waves; at least k classes lie at or above it. Those are listed, and the k-th of the list
 // is the bound for the rest of the row, of which it lists about k / (stretch) a class. A listed
 // class's rank is its place in the output. Keys hold the index, so ties do not lengthen the list; a
 // row that rises all along does, and takes exact_bound's passes over the cached row.
 // All classes that are not selected are summed relative to the first bound; where that overflows
 // or underflows, or the row holds a NaN, once more relative to their own maximum.
+// What it costs beyond the bytes (106 us at a copy's rate for 2048 x 128000 BF16, measured 132: 4.0 TB/s) are
+// the exponentials, a quarter of the vector units' rate, and the phases in which a workgroup ranks and
+// loads nothing, which the others on its compute unit fill.
 template <typename T, int WAVES, int ITEMS>
 __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     __shared__ TopShared sh;
@@ -694,54 +762,75 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         const int i = threadIdx.x + at * THREADS, index = i * P - row.off + where;
         if (i < row.pieces && where >= 0 && index >= 0 && index < row.v) best = key_of(top, index);
     }
-    const u64 mine = nth_of_wave(best, (a.k + WAVES - 1) / WAVES);
-    if (lane == 0) sh.bounds[wave] = mine;
-    __syncthreads();
-    u64 bound = sh.bounds[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) bound = min(bound, sh.bounds[w]);
-
-    float least = bound ? value_of(bound) : -INFINITY;      // 0 lists everything
-    const float b = least == -INFINITY ? 0.0f : -least * c;
-    float sum = 0.0f;
-    u64 pending = 0;
-#pragma unroll
-    for (int t = 0; t < ITEMS; ++t) {
-        const int i = threadIdx.x + t * THREADS;
-        if (i < row.pieces) {
-            float x[P];
-            values(t, x);
-            sift(row, i, x, least, bound, c, b, sh, pending, sum);
-        }
+    const int full = min(WAVES, row.pieces / 64);       // waves with a piece in every lane
+    const bool bounded = a.k <= 64 * full;
+    if (bounded && wave < full) {
+        const u64 mine = nth_of_wave(best, (a.k + full - 1) / full);
+        if (lane == 0) sh.bounds[wave] = mine;
     }
-    list_pending(sh, pending);
-    // A NaN is found by the sum: it may be among the largest, which comparisons of values miss.
-    bool exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
-    if (!exact && row.pieces > ITEMS * THREADS) {
-        keep_first<THREADS>(sh, a.k, c, b, sum);
-        bound = sh.list[a.k - 1];
-        least = value_of(bound);
-        for_pieces<THREADS, true>(row, ITEMS * THREADS, -INFINITY, [&](int i, auto &x) {
+    __syncthreads();
+    u64 bound = bounded ? sh.bounds[0] : 0;
 #pragma unroll
-            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
-                sift(row, i + t * THREADS, x[t], least, bound, c, b, sh, pending, sum);
-        });
-        list_pending(sh, pending);
-        exact = __syncthreads_or(sum != sum) || sh.found > u32(TOP_LIST);
+    for (int w = 1; w < WAVES; ++w)
+        if (bounded && w < full) bound = min(bound, sh.bounds[w]);
+
+    const float least = bound ? value_of(bound) : -INFINITY;      // 0 lists everything
+    const float b = least == -INFINITY ? 0.0f : -least * c;
+    Sift<T> sift{c, b, least, bound};
+    // All pieces together where rows fill the chip (133 against 152 us for 2048 x 128000 BF16), four at a
+    // time for few rows (15.0 against 16.4 us for 1 x 50001 FP32).
+    constexpr int LOADS = 4, TOGETHER = WAVES < 16 ? ITEMS : LOADS;
+#pragma unroll
+    for (int t = 0; t < ITEMS; t += TOGETHER)
+        sift.add(row, sh, reinterpret_cast<v4u (&)[TOGETHER]>(first[t]), threadIdx.x + t * THREADS,
+                 THREADS, row.pieces);
+    sift.finish(row, sh);
+    // A NaN is found by the sum: it may be among the largest, which comparisons of values miss.
+    bool exact = __syncthreads_or(sift.sum != sift.sum) || sh.found > u32(TOP_LIST);
+    if (!exact && row.pieces > ITEMS * THREADS) {
+        keep_first<THREADS>(sh, a.k, c, b, sift.sum);
+        sift.bound = sh.list[a.k - 1];
+        sift.least = value_of(sift.bound);
+        if (threadIdx.x == 0 && row.last < row.pieces) {
+            sift.held = row.template piece<true>(row.last, T(-INFINITY));
+            sift.at = row.last;
+        }
+        for (int i = ITEMS * THREADS + threadIdx.x; i < row.last; i += LOADS * THREADS) {
+            v4u raw[LOADS]{};
+#pragma unroll
+            for (int t = 0; t < LOADS; ++t)
+                if (i + t * THREADS < row.last) raw[t] = row.template whole<true>(i + t * THREADS);
+            sift.add(row, sh, raw, i, THREADS, row.last);
+        }
+        sift.finish(row, sh);
+        exact = __syncthreads_or(sift.sum != sift.sum) || sh.found > u32(TOP_LIST);
     }
     if (exact) {
-        bound = exact_bound<T, THREADS>(row, a.k, sh);      // lists k classes
+        const Row<T> again = row;
+        bound = exact_bound<T, THREADS>(again, a.k, sh);      // lists k classes
         if (threadIdx.x == 0) sh.found = 0;
         __syncthreads();
-        sum = 0.0f;
-        for_pieces<THREADS, false>(row, 0, -INFINITY, [&](int i, auto &x) {
+        float others = 0.0f;
+        for_pieces<THREADS, false>(again, 0, -INFINITY, [&](int i, auto &raw) {
 #pragma unroll
-            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
-                sift(row, i + t * THREADS, x[t], -INFINITY, bound, c, b, sh, pending, sum);
+            for (int t = 0; t < int(sizeof(raw) / sizeof(raw[0])); ++t) {
+                float x[P];
+                unpack<T>(raw[t], x);
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    const int index = (i + t * THREADS) * P - again.off + j;
+                    const u64 key = key_of(x[j], index);
+                    if (index >= 0 && index < again.v && key >= bound)
+                        list_key(sh, key);
+                    else
+                        others += __builtin_amdgcn_exp2f(fmaf(x[j], c, b));
+                }
+            }
         });
-        list_pending(sh, pending);
+        sift.sum = others;
         __syncthreads();
     }
+    float sum = sift.sum;
     keep_first<THREADS>(sh, a.k, c, b, sum);
     for (int j = threadIdx.x; j < a.k; j += THREADS) {
         const int index = int(0xffffffffu - u32(sh.list[j]));
@@ -753,15 +842,19 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     float tail = (__builtin_amdgcn_logf(sum) - b) * LN2;
     if (a.k < a.v && !(sum > 0x1p-60f && sum < 0x1p60f && fabsf(b) < 0x1p60f)) {
         const u64 last = sh.list[a.k - 1];
+        const Row<T> again = row;
         LogSum rest;
-        for_pieces<THREADS, false>(row, 0, -INFINITY, [&](int i, auto &x) {
-            for (int t = 0; t < int(sizeof(x) / sizeof(x[0])); ++t)
+        for_pieces<THREADS, false>(again, 0, -INFINITY, [&](int i, auto &raw) {
+#pragma unroll
+            for (int t = 0; t < int(sizeof(raw) / sizeof(raw[0])); ++t) {
+                float x[P];
+                unpack<T>(raw[t], x);
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
-                    const int index = (i + t * THREADS) * P - row.off + j;
-                    if (index >= 0 && index < row.v && key_of(x[t][j], index) < last)
-                        rest.add(x[t][j], c);
+                    const int index = (i + t * THREADS) * P - again.off + j;
+                    if (index >= 0 && index < again.v && key_of(x[j], index) < last) rest.add(x[j], c);
                 }
+            }
         });
         rest = block_merge<WAVES>(rest, c, sh.scratch);
         tail = rest.m == -INFINITY && rest.s == 0.0f
@@ -811,21 +904,24 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
         hipStream_t s = static_cast<hipStream_t>(stream);
-        // A wave needs a class in every lane for its bound, and no more than its 64. Few rows take
-        // sixteen waves each. Where the rows fill the chip several times over, eight waves leave room
-        // for two or three workgroups on a compute unit, and one lists while others load; the longer
-        // stretch pays where the short one would list many classes (us, 2048 x 128000 BF16, 8 / 16 pieces: k =
-        // 64 168 / 185, k = 250 407 / 309; 64 rows, 8 / 16 waves 36 / 28).
+        // Few rows take sixteen waves each (us, 64 x 128000 BF16, k = 64, 4 / 8 / 16 waves: 49 / 30 / 27). Where the
+        // rows fill the chip, small workgroups let some list while others load; a longer stretch and more
+        // waves pay where the bound would list many classes, and a wave's bound is near the
+        // row's while k is at most half its lanes times the waves (us, 2048 rows BF16, four waves of 8 and
+        // 16 pieces / eight of 16: 16000 classes, k = 64 41 / 44 / 68; 128000, k = 64 206 / 132 / 141; 128000,
+        // k = 128 380 / 195 / 174).
         const i64 pieces = v / PIECE<T>;
-        const auto fits = [&](int waves) { return pieces >= 64 * waves && k <= 64 * waves; };
-        if (n >= 512 && fits(8) && k * v <= 256 * 4096 * PIECE<T>)
-            hipLaunchKernelGGL((k_top<T, 8, 8>), dim3(unsigned(n)), dim3(512), 0, s, args);
-        else if (n >= 512 && fits(8))
-            hipLaunchKernelGGL((k_top<T, 8, 16>), dim3(unsigned(n)), dim3(512), 0, s, args);
-        else if (fits(16) || k > 256)
-            hipLaunchKernelGGL((k_top<T, 16, 16>), dim3(unsigned(n)), dim3(1024), 0, s, args);
+        const auto launch = [&](auto kernel, int waves) {
+            hipLaunchKernelGGL(kernel, dim3(unsigned(n)), dim3(64 * waves), 0, s, args);
+        };
+        if (n < 512 ? pieces >= 1024 || k > 128 : k > 256)
+            launch(k_top<T, 16, 16>, 16);
+        else if (k <= 128 && pieces <= 4 * 64 * 8)
+            launch(k_top<T, 4, 8>, 4);
+        else if (k <= 128 && k * v <= 256 * 4096 * PIECE<T>)
+            launch(k_top<T, 4, 16>, 4);
         else
-            hipLaunchKernelGGL((k_top<T, 4, 8>), dim3(unsigned(n)), dim3(256), 0, s, args);
+            launch(k_top<T, 8, 16>, 8);
         return check_launch("top logits");
     });
 }
