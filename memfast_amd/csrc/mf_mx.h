@@ -30,7 +30,9 @@ struct Scales {
 };
 
 __host__ inline Scales scales_by_row(const u8 *data, i64 segs) { return {data, segs * SEG_SCALES, SEG_SCALES}; }
-__host__ inline Scales scales_by_segment(const u8 *data, i64 n) { return {data, SEG_SCALES, even(n) * SEG_SCALES}; }
+__host__ inline Scales scales_by_segment(const u8 *data, i64 n) {
+    return {data, SEG_SCALES, even(n) * SEG_SCALES};
+}
 
 // ---- values ----------------------------------------------------------------
 // Eight values of a row from column c; zero from column k on.
