@@ -41,6 +41,8 @@ def distill(steps=40, batch=64, features=256, hidden=512, classes=1000, k=16, te
     """The losses of ``steps`` updates of the analog student."""
     torch.manual_seed(seed)
     original = classifier(features, hidden, classes).to(device)
+    with torch.no_grad():       # logits as far apart as a trained network's
+        original[-1].weight.mul_(12)
     teacher = microscaled(original)
     # The student starts away from the teacher: its weights were lost in part.
     student = copy.deepcopy(original)
