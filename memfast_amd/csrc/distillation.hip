@@ -351,7 +351,9 @@ __global__ __launch_bounds__(64 * WAVES, 5) void k_distill(const DistillArgs a) 
     teacher = block_sum<WAVES>(teacher, scratch);
     student = block_sum<WAVES>(student, scratch);
     const double tail_mass = exp((double(tail) - t0) * cold);
-    const double rest_scale = exp((double(rest.ref()) - z0) * cold);
+    // 0 where nothing is left outside the entries: ref() is then no logit's value, and may be so far above
+    // z0 that the exponential is infinite.
+    const double rest_scale = rest.s == 0.0f ? 0.0 : exp((double(rest.ref()) - z0) * cold);
     teacher += tail_mass;
     student += rest_scale * double(rest.s);
     const bool empty = most_t == -INFINITY && teacher == 0.0;
