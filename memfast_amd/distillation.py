@@ -65,11 +65,11 @@ class _Distillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, values, indices, tail, weight, temperature, reduction):
-        row_loss, total, stats, grad = hip.distill_loss(
+        loss, stats, grad = hip.distill_loss(
             logits, values, indices, tail, temperature, weight, reduction, reduction != "none")
         ctx.save_for_backward(logits, indices, weight, stats)
         ctx.options, ctx.ready = (temperature, reduction), grad
-        return _weighted(row_loss, weight) if reduction == "none" else total
+        return _weighted(loss, weight) if reduction == "none" else loss
 
     @staticmethod
     def backward(ctx, incoming):
@@ -149,10 +149,9 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
     if torch.is_grad_enabled() and logits.requires_grad:
         loss = _Distillation.apply(rows, entries, indices, tail, weight, temperature, reduction)
     else:
-        row_loss, loss, _, _ = hip.distill_loss(rows, entries, indices, tail, temperature, weight,
-                                                reduction, False)
+        loss = hip.distill_loss(rows, entries, indices, tail, temperature, weight, reduction, False)[0]
         if reduction == "none":
-            loss = _weighted(row_loss, weight)
+            loss = _weighted(loss, weight)
     return loss.reshape(lead) if reduction == "none" else loss
 
 

@@ -1580,25 +1580,27 @@ def top_logits(logits, k, temperature):
 
 
 def distill_loss(logits, values, indices, tail, temperature, weight, reduction, with_grad):
-    """Row losses [n], their sum or mean [] (None for "none"), what ``distill_grad`` needs, and
+    """The rows' losses [n] ("none", not weighted), their sum or mean [], what ``distill_grad`` needs, and
     ``with_grad`` (a sum or mean) the gradient [n, v] for an incoming 1 (mf_distill_loss)."""
     n, v = logits.shape
     k = indices.shape[1]
     device = logits.device
-    # One allocation: total, norm, row losses, references, coefficients, entries' gradients.
-    stats = torch.empty(2 + n * (3 + k), dtype=torch.float32, device=device)
-    base = stats.data_ptr()
-    rows = base + 8
+    # The loss is a tensor of its own, which a caller may change in place or keep. One allocation for
+    # the rest: norm, references, coefficients, entries' gradients, row losses that are summed.
+    none = reduction == "none"
+    loss = torch.empty(n if none else (), dtype=torch.float32, device=device)
+    stats = torch.empty(1 + n * ((2 if none else 3) + k), dtype=torch.float32, device=device)
+    norm = stats.data_ptr()
+    refs = norm + 4
+    rows = loss.data_ptr() if none else refs + 4 * n * (2 + k)
     grad = torch.empty((n, v), dtype=logits.dtype, device=device) if with_grad else None
     with _on(device):
         check(library().mf_distill_loss(
             logits.data_ptr(), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), values.data_ptr(),
             FLOAT_TYPES[values.dtype], indices.data_ptr(), _ptr(tail), k, temperature, _ptr(weight),
-            REDUCTIONS[reduction], rows, rows + 4 * n, rows + 8 * n, rows + 12 * n, base, base + 4,
-            _ptr(grad), _stream(device)), "distillation loss")
-    if reduction == "none":
-        return stats[2:2 + n], None, stats, grad
-    return None, stats[0], stats, grad
+            REDUCTIONS[reduction], rows, refs, refs + 4 * n, refs + 8 * n,
+            None if none else loss.data_ptr(), norm, _ptr(grad), _stream(device)), "distillation loss")
+    return loss, stats, grad
 
 
 def distill_grad(logits, indices, temperature, weight, stats, reduction, incoming, grad=None):
@@ -1613,7 +1615,7 @@ def distill_grad(logits, indices, temperature, weight, stats, reduction, incomin
     with _on(logits.device):
         check(library().mf_distill_grad(
             logits.data_ptr(), FLOAT_TYPES[logits.dtype], n, v, logits.stride(0), indices.data_ptr(),
-            indices.shape[1], temperature, _ptr(weight), base + 8 + 4 * n, base + 8 + 8 * n,
-            base + 8 + 12 * n, None if none else base + 4, incoming.data_ptr(), int(none),
+            indices.shape[1], temperature, _ptr(weight), base + 4, base + 4 + 4 * n, base + 4 + 8 * n,
+            None if none else base, incoming.data_ptr(), int(none),
             int(ready), grad.data_ptr(), _stream(logits.device)), "distillation gradient")
     return grad

@@ -57,3 +57,47 @@ def test_all_classes_are_entries(hip_device, shift, temperature):
     for tail in (None, rest):
         loss, grad = check_loss(s, values, indices, tail, temperature=temperature)
         assert bool(torch.isfinite(loss)) and bool(torch.isfinite(grad).all())
+
+
+# ---------------------------------------------------------------------------
+# A loss that is changed in place or kept
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_losses_can_be_changed_in_place(hip_device, reduction, weighted):
+    """Divided by a number of accumulation steps and joined by another loss, as training loops do."""
+    n = 5
+    s = logits(n, 700, torch.float32, hip_device)
+    values, indices, rest = teacher_of(s, 6, 1.0)
+    options = dict(reduction=reduction)
+    if weighted:
+        options["weight"] = torch.tensor([1.0, 0.0, 2.0, 0.5, 1.0], device=hip_device)
+
+    def gradient(in_place):
+        leaf = s.clone().requires_grad_(True)
+        loss = memfast.distillation_loss(leaf, values, indices, rest, **options)
+        other = 0.1 * leaf.square().mean()
+        if in_place:
+            loss /= 4
+            loss += other
+        else:
+            loss = loss / 4 + other
+        loss.sum().backward()
+        return loss.detach(), leaf.grad
+
+    for here, there in zip(gradient(True), gradient(False)):
+        assert torch.equal(here, there)
+    # Without a gradient too; what a caller does to a loss reaches no other result.
+    loss = memfast.distillation_loss(s, values, indices, rest, **options)
+    kept = loss.clone()
+    loss.zero_()
+    assert torch.equal(memfast.distillation_loss(s, values, indices, rest, **options), kept)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_kept_losses_hold_no_other_memory(hip_device, reduction):
+    s = logits(40, 300, torch.float32, hip_device)
+    values, indices, rest = teacher_of(s, 20, 1.0)
+    for leaf in (s, s.clone().requires_grad_(True)):
+        loss = memfast.distillation_loss(leaf, values, indices, rest, reduction=reduction).detach()
+        assert loss.untyped_storage().nbytes() == 4 * loss.numel()
