@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import hip
-from .microscaling import _check_floating
+from .microscaling import _check_floating, _refuse_tangents
 
 MOST_ENTRIES, MOST_CLASSES = 1024, 1 << 20
 
@@ -107,7 +107,7 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
 
     ``weight`` [...] weighs the rows (bool or floating; a row of weight 0 is not read).
     ``reduction``: "mean" (over the weights' sum; 0 if that is 0), "sum" or "none".  The loss is FP32;
-    gradients reach ``logits`` alone."""
+    gradients reach ``logits`` alone.  An operand with a tangent of forward mode is refused."""
     _check_logits(logits)
     _check_floating("values", values)
     temperature = _check_temperature(temperature)
@@ -137,6 +137,7 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
                          ("weight", weight)):
         if value is not None and value.device != logits.device:
             raise ValueError(f"logits and {label} must use the same device")
+    _refuse_tangents("distillation_loss", logits, values, tail, weight)
     hip.require_device(logits)
     if logits.numel() == 0:
         zero = logits.sum(-1).float()

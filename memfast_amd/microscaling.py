@@ -17,6 +17,7 @@ shows as NaN in the result and raises nothing.
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import hip
@@ -58,6 +59,16 @@ class MXTensor:
 
     def __repr__(self):
         return f"MXTensor(shape={tuple(self.shape)}, device={self.device})"
+
+
+def _refuse_tangents(name, *operands):
+    """The operators have no forward-mode derivative: an operand with a tangent is refused, as the
+    autograd functions do where some operand wants a gradient."""
+    if getattr(forward_ad, "_current_level", 0) < 0:     # outside forward mode, the usual case
+        return
+    for value in operands:
+        if isinstance(value, torch.Tensor) and forward_ad.unpack_dual(value).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _part(label, value, shape):
@@ -110,7 +121,7 @@ def mx_linear(x, weight, bias=None):
     """``Q(x) Q(weight)^T + bias`` for ``x`` [..., k] and ``weight`` [o, k], in x's dtype.
 
     ``weight`` is an MXTensor, or a tensor of x's dtype that is quantized in the call and gets a
-    gradient.  ``bias`` [o] has x's dtype."""
+    gradient.  ``bias`` [o] has x's dtype.  An operand with a tangent of forward mode is refused."""
     _check_floating("x", x)
     held = isinstance(weight, MXTensor)
     if not held:
@@ -132,6 +143,7 @@ def mx_linear(x, weight, bias=None):
         raise ValueError("x and weight have incompatible reduction dimensions")
     if bias is not None and bias.shape != (o,):
         raise ValueError("bias must have one value per output")
+    _refuse_tangents("mx_linear", x, weight, bias)
     hip.require_device(x)
     shape = x.shape[:-1] + (o,)
     if x.numel() == 0 or o == 0:
