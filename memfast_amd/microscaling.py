@@ -101,7 +101,9 @@ class _MXLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, codes, scales):
         y, block = hip.mx_linear(x, weight, codes, scales, bias, ctx.needs_input_grad[1])
-        ctx.width, ctx.operands = x.shape[1], (codes, scales, block)
+        ctx.width = x.shape[1]
+        # A held weight's gradients need none of what the call quantized.
+        ctx.save_for_backward(codes, scales, block if codes is None else None)
         return y
 
     @staticmethod
@@ -112,7 +114,7 @@ class _MXLinear(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, dy):
-        codes, scales, block = ctx.operands
+        codes, scales, block = ctx.saved_tensors
         return (*hip.mx_grads(hip.rows_of(dy), ctx.width, codes, scales, block,
                               ctx.needs_input_grad[:3]), None, None)
 
