@@ -1433,6 +1433,7 @@ __all__ = [
 # ---------------------------------------------------------------------------
 FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # MF_F32, MF_BF16, MF_F16
 MX_SEGMENT, MX_SEGMENT_BYTES, MX_SEGMENT_SCALES = 256, 128, 8
+MX_GRAD_ROWS, MX_GRAD_OUTPUTS = (1 << 24) - 1, 1 << 22      # what mf_mx_grads takes
 
 
 def rows_of(x):

@@ -123,7 +123,8 @@ def mx_linear(x, weight, bias=None):
     """``Q(x) Q(weight)^T + bias`` for ``x`` [..., k] and ``weight`` [o, k], in x's dtype.
 
     ``weight`` is an MXTensor, or a tensor of x's dtype that is quantized in the call and gets a
-    gradient.  ``bias`` [o] has x's dtype.  An operand with a tangent of forward mode is refused."""
+    gradient.  ``bias`` [o] has x's dtype.  Rows of x and o are below 2**28 and k below 2**24; where a
+    gradient is wanted, x has at most 2**24 - 1 rows and o is at most 2**22.  An operand with a tangent of forward mode is refused."""
     _check_floating("x", x)
     held = isinstance(weight, MXTensor)
     if not held:
@@ -156,11 +157,15 @@ def mx_linear(x, weight, bias=None):
         return y if bias is None else y + bias
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
+    recorded = torch.is_grad_enabled() and (x.requires_grad or not held and weight.requires_grad or
+                                            bias is not None and bias.requires_grad)
+    if recorded and (x.numel() // k > hip.MX_GRAD_ROWS or o > hip.MX_GRAD_OUTPUTS):
+        raise NotImplementedError(f"gradients of more than {hip.MX_GRAD_ROWS} rows or "
+                                  f"{hip.MX_GRAD_OUTPUTS} outputs")
     codes, scales = (weight.codes, weight.scales) if held else (None, None)
     weight = None if held else hip.rows_of(weight)
     rows = hip.rows_of(x)
-    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or
-                                    bias is not None and bias.requires_grad):
+    if recorded:
         y = _MXLinear.apply(rows, weight, bias, codes, scales)
     else:
         y = hip.mx_linear(rows, weight, codes, scales, bias, False)[0]

@@ -95,3 +95,24 @@ def test_checkpointed_products(hip_device):
         x.grad = w.grad = None
         y.backward(dy)
         assert torch.equal(x.grad, expected[0]) and torch.equal(w.grad, expected[1])
+
+
+def test_sizes_without_a_backward_are_refused_before_the_forward(hip_device):
+    """The gradients take fewer rows and outputs than the product."""
+    rows, outputs = 1 << 24, (1 << 22) + 1
+    many = torch.ones(1, 1, dtype=torch.bfloat16, device=hip_device)
+    w = torch.full((1, 1), 2.0, dtype=torch.bfloat16, device=hip_device)
+    for x, weight in ((many.expand(rows, 1), w), (many, w.expand(outputs, 1)),
+                      (many.expand(rows, 1), memfast.mx_quantize(w))):
+        y = memfast.mx_linear(x, weight)
+        assert bool((y == 2).all())
+        with torch.no_grad():
+            assert memfast.mx_linear(x.detach().requires_grad_(True), weight).shape == y.shape
+        with pytest.raises(NotImplementedError, match="gradients of more than"):
+            memfast.mx_linear(x.detach().requires_grad_(True), weight)
+    x = many.expand(rows - 1, 1).contiguous().requires_grad_(True)
+    dx, = torch.autograd.grad(memfast.mx_linear(x, w).sum(), x)
+    assert bool((dx == 2).all())
+    w = w.expand(outputs - 1, 1).contiguous().requires_grad_(True)
+    dw, = torch.autograd.grad(memfast.mx_linear(many, w).sum(), w)
+    assert bool((dw == 1).all())
