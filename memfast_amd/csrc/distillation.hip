@@ -852,6 +852,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
         const u64 last = sh.list[a.k - 1];
         const Row<T> again = row;
         LogSum rest;
+        bool infinite = false, nan = false;
         for_pieces<THREADS, false>(again, 0, -INFINITY, [&](int i, auto &raw) {
 #pragma unroll
             for (int t = 0; t < int(sizeof(raw) / sizeof(raw[0])); ++t) {
@@ -860,14 +861,23 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
 #pragma unroll
                 for (int j = 0; j < P; ++j) {
                     const int index = (i + t * THREADS) * P - again.off + j;
-                    if (index >= 0 && index < again.v && key_of(x[j], index) < last) rest.add(x[j], c);
+                    if (index < 0 || index >= again.v || key_of(x[j], index) >= last) continue;
+                    infinite = infinite || x[j] == INFINITY;
+                    nan = nan || x[j] != x[j];
+                    rest.add(x[j], c);
                 }
             }
         });
         rest = block_merge<WAVES>(rest, c, sh.scratch);
-        tail = rest.m == -INFINITY && rest.s == 0.0f
-                   ? -INFINITY
-                   : rest.ref() / a.temperature + __builtin_amdgcn_logf(rest.s) * LN2;
+        // A +inf makes the tail +inf, where the sum relative to it is NaN; a NaN makes it NaN.
+        infinite = __syncthreads_or(infinite);
+        nan = __syncthreads_or(nan);
+        if (infinite && !nan)
+            tail = INFINITY;
+        else if (rest.m == -INFINITY && rest.s == 0.0f)
+            tail = -INFINITY;
+        else
+            tail = rest.ref() / a.temperature + __builtin_amdgcn_logf(rest.s) * LN2;
     }
     if (threadIdx.x == 0) a.tail[r] = a.k < a.v ? tail : -INFINITY;
 }

@@ -101,3 +101,33 @@ def test_kept_losses_hold_no_other_memory(hip_device, reduction):
     for leaf in (s, s.clone().requires_grad_(True)):
         loss = memfast.distillation_loss(leaf, values, indices, rest, reduction=reduction).detach()
         assert loss.untyped_storage().nbytes() == 4 * loss.numel()
+
+
+# ---------------------------------------------------------------------------
+# Infinities among the others
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("v,k", [(2, 1), (9, 2), (3001, 2), (3001, 64), (40000, 1), (70003, 129)])
+@pytest.mark.parametrize("repeats", [1, 200])
+def test_the_tail_of_infinite_logits(hip_device, kind, v, k, repeats):
+    """log(sum(exp)) of others with +inf among them is +inf, with NaN it is NaN, and beside
+    an infinity that is selected, or -inf, it is as finite as without."""
+    s = torch.zeros(6, v)
+    at = torch.arange(v)
+    s[0] = torch.where(at >= v - (k + 1), math.inf, 0.0)      # one more than is selected
+    s[1] = torch.where(at < k + 1, math.inf, -math.inf)
+    s[2] = math.inf
+    s[3] = torch.where(at % 2 == 0, math.nan, math.inf) if 2 * k < v else math.nan
+    s[4] = torch.where(at < k, math.inf, 0.0)                 # all of them are selected
+    s[5] = torch.where(at < k, math.nan, math.inf)            # every NaN is
+    s = s.to(TYPES[kind]).to(hip_device).repeat(repeats, 1)
+    values, indices, tail = memfast.top_logits(s, k, temperature=2.0)
+    rows = s[:6].cpu().double()
+    ordered, order = torch.sort(rows, dim=1, descending=True, stable=True)
+    assert torch.equal(indices.cpu(), order[:, :k].repeat(repeats, 1))
+    expected = torch.logsumexp(ordered[:, k:] / 2.0, 1)
+    assert torch.equal(expected[:3], torch.full((3,), math.inf, dtype=torch.float64))
+    got = tail.cpu().double().reshape(repeats, 6)
+    assert torch.equal(got[:, [0, 1, 2, 5]], expected[[0, 1, 2, 5]].expand(repeats, 4))
+    assert bool(expected[3].isnan()) and bool(got[:, 3].isnan().all())
+    assert bool(((got[:, 4] - expected[4]).abs() <= 2.0**-17 + 2.0**-22 * expected[4].abs()).all())
