@@ -594,7 +594,7 @@ int mf_mx_grads(const void *dy, int32_t type, int64_t n, int64_t o, int64_t ldy,
 /* The k largest of each row of logits [n, v] (rows ld apart), in descending order, the lowest index
  * first among equal ones (NaN counts as the largest, -0 as 0): values [n, k] of the logits' type, indices
  * [n, k], and tail [n] = log(sum(exp(logits / temperature))) of the row's other logits (-inf where
- * there is none).  k <= 1024, v <= 2^20. */
+ * there is none).  k <= 1024, v <= 2^20.  Temperatures are FP32's normal numbers, here and below. */
 int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_t ld, int64_t k,
                   float temperature, void *values, int64_t *indices, float *tail, void *stream);
 

@@ -882,10 +882,11 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     if (threadIdx.x == 0) a.tail[r] = a.k < a.v ? tail : -INFINITY;
 }
 
+// (log2(e) / T is finite from FLT_MIN on.)
 static int check_rows(const char *what, const void *logits, int32_t type, i64 n, i64 v, i64 ld, i64 k,
                       float temperature) {
     if (!logits || !known_type(type) || n < 1 || v < 1 || k < 1 || k > v || (n > 1 && ld < v) ||
-        !(temperature > 0.0f) || !(temperature <= FLT_MAX) || !aligned(logits, type_bytes(type)))
+        !(temperature >= FLT_MIN) || !(temperature <= FLT_MAX) || !aligned(logits, type_bytes(type)))
         return fail(MF_E_INVALID, "invalid %s arguments", what);
     if (v > MOST_CLASSES || n > i64(1) << 30)
         return fail(MF_E_UNSUPPORTED, "%s takes at most %lld classes", what, (long long)MOST_CLASSES);

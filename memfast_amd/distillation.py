@@ -6,10 +6,8 @@ largest logits per row and the logarithm of the mass of all others, and ``distil
 the student's loss against them, with its gradient.
 
 Both run in one pass over the logits each way, hold their sums in FP32 and read nothing back
-to the host; a row whose indices are wrong has a NaN loss.
+to the host; a row whose indices are wrong has a NaN loss.  Temperatures are normal numbers of FP32.
 """
-
-import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -18,13 +16,15 @@ from . import hip
 from .microscaling import _check_floating, _refuse_tangents
 
 MOST_ENTRIES, MOST_CLASSES = 1024, 1 << 20
+# 1 / T is formed in FP32: below its smallest normal number it would be infinite.
+LEAST_TEMPERATURE, MOST_TEMPERATURE = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _check_temperature(temperature):
     if isinstance(temperature, bool) or not isinstance(temperature, (int, float)):
         raise TypeError("temperature must be a number")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("temperature must be positive and finite")
+    if not LEAST_TEMPERATURE <= temperature <= MOST_TEMPERATURE:
+        raise ValueError("temperature must be a positive normal number of float32")
     return float(temperature)
 
 

@@ -131,3 +131,14 @@ def test_the_tail_of_infinite_logits(hip_device, kind, v, k, repeats):
     assert torch.equal(got[:, [0, 1, 2, 5]], expected[[0, 1, 2, 5]].expand(repeats, 4))
     assert bool(expected[3].isnan()) and bool(got[:, 3].isnan().all())
     assert bool(((got[:, 4] - expected[4]).abs() <= 2.0**-17 + 2.0**-22 * expected[4].abs()).all())
+
+
+def test_the_smallest_temperature(hip_device):
+    """At 2**-126 the largest class has all the mass, and exponents stay finite."""
+    temperature = 2.0**-126
+    s = torch.arange(8.0, device=hip_device)[None] / 4
+    values, indices, tail = memfast.top_logits(s, 2, temperature=temperature)
+    assert indices.tolist() == [[7, 6]] and float(tail) == 1.25 * 2.0**126
+    s = s * 2.0**-126
+    values, indices, tail = memfast.top_logits(s, 2, temperature=temperature)
+    check_loss(s, values, indices, temperature=temperature)
