@@ -195,6 +195,7 @@ struct DistillArgs {
     const float *norm;       // with a gradient: what the rows' weights are multiplied by
     float inverse_n;         // the same where norm is nullptr
     void *grad;              // [n, v]
+    i64 first;               // row of the launch's first workgroup
 };
 
 // p d - p + q with d = log(p / q), as p (d + exp(-d) - 1) where that stays in range.
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(64 * WAVES, 5) void k_distill(const DistillArgs a) 
     extern __shared__ u32 bits[];
     __shared__ __align__(16) float scratch[2 * WAVES];     // two floats or one double a wave
     constexpr int THREADS = 64 * WAVES;
-    const i64 r = blockIdx.x;
+    const i64 r = a.first + blockIdx.x;
     const float weight = a.weight ? a.weight[r] : 1.0f;
     if (weight == 0.0f) {   // nothing of such a row is read
         for (i64 j = threadIdx.x; j < a.k; j += THREADS) a.entry_grad[r * a.k + j] = 0.0f;
@@ -440,6 +441,7 @@ struct DistillGradArgs {
     float temperature;
     bool unless_one;          // the gradient for an incoming 1 is there already
     void *grad;               // [n, v]
+    i64 first;                // row of the launch's first workgroup
 };
 
 // The gradient for another incoming value, from the row's reference and coefficient: one pass, bound by
@@ -448,7 +450,7 @@ template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_distill_grad(const DistillGradArgs a) {
     extern __shared__ u32 bits[];
     constexpr int THREADS = 64 * WAVES;
-    const i64 r = blockIdx.x;
+    const i64 r = a.first + blockIdx.x;
     if (a.unless_one && *a.incoming == 1.0f) return;
     const Row<T> row(static_cast<const T *>(a.logits) + r * a.ld, a.v);
     T *grad = static_cast<T *>(a.grad) + r * a.v;
@@ -493,6 +495,7 @@ struct TopArgs {
     void *values;         // [n, k]
     i64 *indices;         // [n, k]
     float *tail;          // [n]
+    i64 first;            // row of the launch's first workgroup
 };
 
 constexpr int TOP_LIST = 2048;      // candidates of a row
@@ -727,7 +730,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     __shared__ TopShared sh;
     constexpr int THREADS = 64 * WAVES, P = PIECE<T>;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const i64 r = blockIdx.x;
+    const i64 r = a.first + blockIdx.x;
     const Row<T> row(static_cast<const T *>(a.logits) + r * a.ld, a.v);
     const float c = LOG2E / a.temperature;
     if (threadIdx.x == 0) sh.found = 0;
@@ -889,13 +892,26 @@ static int check_rows(const char *what, const void *logits, int32_t type, i64 n,
         !(temperature >= FLT_MIN) || !(temperature <= FLT_MAX) || !aligned(logits, type_bytes(type)))
         return fail(MF_E_INVALID, "invalid %s arguments", what);
     if (v > MOST_CLASSES || n > i64(1) << 30)
-        return fail(MF_E_UNSUPPORTED, "%s takes at most %lld classes", what, (long long)MOST_CLASSES);
+        return fail(MF_E_UNSUPPORTED, "%s takes at most %lld classes and %lld rows", what,
+                    (long long)MOST_CLASSES, (long long)(i64(1) << 30));
     if (k > MOST_ENTRIES)
         return fail(MF_E_UNSUPPORTED, "%s takes at most %d entries a row", what, MOST_ENTRIES);
     return MF_OK;
 }
 
 constexpr int ROW_WAVES = 8;
+
+// Launches a workgroup a row. A launch has fewer than 2^32 threads, so more rows take several.
+template <typename K, typename A>
+static int launch_rows(const char *what, K kernel, A args, int waves, size_t lds, hipStream_t s) {
+    constexpr i64 ROWS = i64(1) << 21;      // of at most 1024 threads
+    for (args.first = 0; args.first < args.n; args.first += ROWS) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(std::min(ROWS, args.n - args.first))), dim3(64 * waves), lds,
+                           s, args);
+        if (const int status = check_launch(what)) return status;
+    }
+    return MF_OK;
+}
 
 static size_t mark_bytes(i64 v) { return size_t((v + 8 + 31) / 32 * 4); }
 
@@ -922,7 +938,6 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
     const TopArgs args{logits, n, v, ld, int(k), temperature, values, indices, tail};
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        hipStream_t s = static_cast<hipStream_t>(stream);
         // Few rows take sixteen waves each (us, 64 x 128000 BF16, k = 64, 4 / 8 / 16 waves: 49 / 30 / 27).
         // Where the rows fill the chip, small workgroups let some list while others load; a longer
         // stretch and more waves pay where the bound would list many classes, and a wave's bound is near
@@ -931,17 +946,12 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
         // 128000, k = 128 380 / 195 / 174).
         const i64 pieces = v / PIECE<T>;
         const auto launch = [&](auto kernel, int waves) {
-            hipLaunchKernelGGL(kernel, dim3(unsigned(n)), dim3(64 * waves), 0, s, args);
+            return launch_rows("top logits", kernel, args, waves, 0, static_cast<hipStream_t>(stream));
         };
-        if (n < 512 ? pieces >= 1024 || k > 128 : k > 256)
-            launch(k_top<T, 16, 16>, 16);
-        else if (k <= 128 && pieces <= 4 * 64 * 8)
-            launch(k_top<T, 4, 8>, 4);
-        else if (k <= 128 && k * v <= 256 * 4096 * PIECE<T>)
-            launch(k_top<T, 4, 16>, 4);
-        else
-            launch(k_top<T, 8, 16>, 8);
-        return check_launch("top logits");
+        if (n < 512 ? pieces >= 1024 || k > 128 : k > 256) return launch(k_top<T, 16, 16>, 16);
+        if (k <= 128 && pieces <= 4 * 64 * 8) return launch(k_top<T, 4, 8>, 4);
+        if (k <= 128 && k * v <= 256 * 4096 * PIECE<T>) return launch(k_top<T, 4, 16>, 4);
+        return launch(k_top<T, 8, 16>, 8);
     });
 }
 
@@ -972,8 +982,7 @@ int mf_distill_loss(const void *logits, int32_t type, int64_t n, int64_t v, int6
         auto kernel = grad ? k_distill<T, ROW_WAVES, true> : k_distill<T, ROW_WAVES, false>;
         const int lds = allow_lds(kernel, mark_bytes(v));
         if (lds) return lds;
-        hipLaunchKernelGGL(kernel, dim3(unsigned(n)), dim3(64 * ROW_WAVES), mark_bytes(v), s, args);
-        return check_launch("distillation loss");
+        return launch_rows("distillation loss", kernel, args, ROW_WAVES, mark_bytes(v), s);
     });
     if (launched || reduction == MF_SUM_NONE) return launched;
     hipLaunchKernelGGL(k_distill_total, dim3(1), dim3(256), 0, s, row_loss, weight, n, mean, loss, norm);
@@ -996,9 +1005,8 @@ int mf_distill_grad(const void *logits, int32_t type, int64_t n, int64_t v, int6
         using T = decltype(zero);
         const int lds = allow_lds(k_distill_grad<T, ROW_WAVES>, mark_bytes(v));
         if (lds) return lds;
-        hipLaunchKernelGGL((k_distill_grad<T, ROW_WAVES>), dim3(unsigned(n)), dim3(64 * ROW_WAVES),
-                           mark_bytes(v), static_cast<hipStream_t>(stream), args);
-        return check_launch("distillation gradient");
+        return launch_rows("distillation gradient", k_distill_grad<T, ROW_WAVES>, args, ROW_WAVES, mark_bytes(v),
+                           static_cast<hipStream_t>(stream));
     });
 }
 

@@ -142,3 +142,39 @@ def test_the_smallest_temperature(hip_device):
     s = s * 2.0**-126
     values, indices, tail = memfast.top_logits(s, 2, temperature=temperature)
     check_loss(s, values, indices, temperature=temperature)
+
+
+# ---------------------------------------------------------------------------
+# More rows than one launch takes
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_rows_past_a_launch(hip_device, reduction):
+    """2**24 + 7 rows, one workgroup each: their threads pass 2**32. Every row has the bits of the
+    same row among a few."""
+    n, v, k, period = (1 << 24) + 7, 3, 1, 16
+    say("rows", n, reduction)
+    few = logits(period, v, torch.bfloat16, hip_device)
+    many = few.repeat(-(-n // period), 1)[:n]
+
+    def equal_rows(got, expected):
+        whole = n // period * period
+        assert torch.equal(got[:whole].reshape(-1, period, *got.shape[1:]),
+                           expected.expand(n // period, *expected.shape))
+        assert torch.equal(got[whole:], expected[:n - whole])
+
+    top = memfast.top_logits(many, k)
+    expected = memfast.top_logits(few, k)
+    for a, b in zip(top, expected):
+        equal_rows(a, b)
+    teacher = [t.roll(1, 0) for t in expected]
+    teachers = [t.repeat(-(-n // period), *[1] * (t.ndim - 1))[:n] for t in teacher]
+    results = [loss_and_gradient(rows, *t, reduction=reduction)
+               for rows, t in ((many, teachers), (few, teacher))]
+    equal_rows(results[0][1], results[1][1])
+    if reduction == "none":
+        equal_rows(results[0][0], results[1][0])
+    else:
+        rows = memfast.distillation_loss(few, *teacher, reduction="none").double()
+        total = rows.sum() * (n // period) + rows[:n % period].sum()
+        # FP64 sums, rounded once.
+        assert abs(float(results[0][0]) - float(total)) <= 2.0**-23 * float(total)
