@@ -370,12 +370,14 @@ struct ProductPlan {
 // tiles, n x k x o): 16 x 4096 x 11008 9.7 / 9.3, 24 of them 12.0 / 9.4, 64 21.6 / 9.8; 24 x 11008 x 4096
 // 10.3 / 18.9, 64 of them 16.9 / 19.2, 64 x 4096 x 4096 8.0 / 8.8.
 constexpr i64 FEW_ROWS = 64, FEW_ROWS_WIDE = 16, WIDE = 8192;
+// A launch has fewer than 2^32 threads; k_mx_few takes 32 an output.
+constexpr i64 FEW_OUTPUTS = i64(1) << 26;
 // Values of x that every workgroup may quantize again: 1 x 4096 x 11008 7.5 us against 8.1 and a launch of 3,
 // 8 x 4096 x 11008 13.2 against 8.7 and 3.
 constexpr i64 FEW_QUANTIZE = 16384;
 
 static ProductPlan plan_product(i64 n, i64 k, i64 o, bool keep) {
-    const bool few = n <= (o < WIDE ? FEW_ROWS : FEW_ROWS_WIDE);
+    const bool few = n <= (o < WIDE ? FEW_ROWS : FEW_ROWS_WIDE) && o <= FEW_OUTPUTS;
     return {few, keep || !few || n > 16 || n * segments(k) * SEG > FEW_QUANTIZE};
 }
 
