@@ -95,7 +95,10 @@ __device__ __forceinline__ u32 codes8(const float (&v)[8], u32 byte) {
     return byte == NAN_BYTE ? 0u : word;
 }
 
-// Eight codes as BF16, exactly: two significant bits, and the scales are BF16's own exponents.
+// Eight codes as BF16, exactly: two significant bits, and the scales are BF16's own exponents. The instruction
+// takes its scale's exponent field, so that byte 0, which the quantizer does not write, is 2^-127 here
+// as in the scaled product (measured: every byte gives the same value in both). Where a code times
+// byte 253 or 254 passes FP32's range it is infinite here.
 __device__ __forceinline__ v8bf expand8(u32 word, u32 byte) {
     if (byte == NAN_BYTE) {
         const bf16 nan = bf16(__uint_as_float(0x7fc00000u));

@@ -35,7 +35,9 @@ class MXTensor:
 
     ``codes`` is uint8 [rows, 128 * S] with S = ceil(k / 256), two codes a byte, the even value in
     the lower half, codes past k zero; ``scales`` is uint8 [rows, 8 * S], e + 127 of each block (255:
-    NaN).  rows is the product of the other dimensions."""
+    NaN; not in blocks past k).  rows is the product of the other dimensions.  Codes from elsewhere
+    may have any e from -127 on; a value beyond FP32's range (e of 126 and 127) is infinite in
+    ``dequantize`` and in gradients."""
 
     def __init__(self, codes, scales, shape):
         self.shape = shape = torch.Size(shape)
