@@ -915,15 +915,6 @@ static int launch_rows(const char *what, K kernel, A args, int waves, size_t lds
 
 static size_t mark_bytes(i64 v) { return size_t((v + 8 + 31) / 32 * 4); }
 
-// Dynamic LDS above 64 KiB has to be asked for once per kernel and device.
-template <typename K> static int allow_lds(K kernel, size_t bytes) {
-    if (bytes <= 48 << 10) return MF_OK;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-    return e == hipSuccess ? MF_OK : fail(MF_E_RESOURCE, "LDS of %zu bytes: %s", bytes,
-                                          hipGetErrorString(e));
-}
-
 }  // namespace mf
 
 using namespace mf;

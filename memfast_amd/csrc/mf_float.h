@@ -1,5 +1,5 @@
-// The floating types that the microscaled and distillation kernels read and write, and loads and
-// stores of whole 16-byte pieces of them.
+// The floating types that the microscaled and distillation kernels read and write, loads and stores of
+// whole 16-byte pieces of them, and what their host sides share.
 #pragma once
 
 #include "mf_device.h"
@@ -41,5 +41,16 @@ __host__ inline bool known_type(int32_t type) { return type >= MF_F32 && type <=
 int fail(int code, const char *fmt, ...);
 int check_launch(const char *what);
 bool aligned(const void *p, uintptr_t bytes);
+
+// Dynamic LDS that passes 64 KiB, with up to 16 KiB of the kernel's own beside it, has to be asked for: on
+// the kernel's current device, so at every launch.
+template <typename K> __host__ int allow_lds(K kernel, i64 bytes) {
+    if (bytes <= 48 << 10) return MF_OK;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    return e == hipSuccess
+               ? MF_OK
+               : fail(MF_E_RESOURCE, "LDS of %lld bytes: %s", (long long)bytes, hipGetErrorString(e));
+}
 
 }  // namespace mf

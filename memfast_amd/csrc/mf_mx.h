@@ -159,14 +159,4 @@ __device__ __forceinline__ u32 lds_address(const u8 *p) {
     return u32(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) u8 *)p));
 }
 
-// LDS above 64 KiB has to be asked for.
-template <typename K> __host__ int allow_lds(K kernel, i64 bytes) {
-    if (bytes <= 64 << 10) return MF_OK;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-    return e == hipSuccess
-               ? MF_OK
-               : fail(MF_E_RESOURCE, "LDS of %lld bytes: %s", (long long)bytes, hipGetErrorString(e));
-}
-
 }  // namespace mf
