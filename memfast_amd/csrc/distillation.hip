@@ -229,7 +229,7 @@ __device__ __forceinline__ bool mark_entries(const i64 *indices, i64 k, i64 v, i
 }
 
 // Writes a piece of the gradient; entries are left to the threads that hold them. `vec`: grad's pieces
-// lie at 16-byte addresses as the row's do.
+// lie at 16-byte addresses as the row's do. (Else, as with a part of a wider matrix's columns, single stores.)
 template <typename T>
 __device__ __forceinline__ void store_rest(T *grad, const Row<T> &row, int i, u32 marked, bool vec,
                                            const float (&x)[PIECE<T>]) {
@@ -445,7 +445,8 @@ struct DistillGradArgs {
 };
 
 // The gradient for another incoming value, from the row's reference and coefficient: one pass, bound by
-// its bytes (2048 x 128000 BF16 213 us, 1.05 GB at 4.9 TB/s).
+// its bytes (2048 x 128000 BF16 213 us, 1.05 GB at 4.9 TB/s). After a sum or mean it writes what k_distill
+// wrote for 1 a second time: forward and backward of a loss times 0.5 465 us, against 260 of the loss itself.
 template <typename T, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_distill_grad(const DistillGradArgs a) {
     extern __shared__ u32 bits[];
@@ -714,17 +715,20 @@ __device__ void keep_first(TopShared &sh, int k, float c, float b, float &sum) {
     __syncthreads();
 }
 
-// One workgroup a row, one pass over it. Its first stretch (ITEMS pieces a thread, in registers) gives a
-// bound: of the largest classes of a wave's lanes the ceil(k / waves)-th largest, the smallest over
-// the waves; at least k classes lie at or above it. Those are listed, and the k-th of the list
-// is the bound for the rest of the row, of which it lists about k / (stretch) a class. A listed
-// class's rank is its place in the output. Keys hold the index, so ties do not lengthen the list; a
-// row that rises all along does, and takes exact_bound's passes over the cached row.
+// One workgroup a row, as a rule one pass over it. Its first stretch (ITEMS pieces a thread, in registers)
+// gives a bound: of the largest classes of a wave's lanes the ceil(k / waves)-th largest, the smallest over
+// the waves; at least k classes lie at or above it. Those are listed, and the k-th of the list is the bound
+// for the rest of the row, of which it lists about k / (stretch) a class. A listed class's rank is its
+// place in the output. Keys hold the index, so ties do not lengthen the list; a row that rises all along
+// does, and takes exact_bound's passes over the cached row. So do ordinary rows of large k: the bound comes
+// from one class a lane, and where k nears the lanes it is their least, above which lie more classes than
+// the list holds. 2048 x 128000 BF16 (us): k = 128 170, 250 248, 512 462, 700 750, and from about 820 on,
+// with the exact passes, 1950 to 2180.
 // All classes that are not selected are summed relative to the first bound; where that overflows
 // or underflows, or the row holds a NaN, once more relative to their own maximum.
-// What it costs beyond the bytes (106 us at a copy's rate for 2048 x 128000 BF16, measured 132: 4.0 TB/s) are
-// the exponentials, a quarter of the vector units' rate, and the phases in which a workgroup ranks and
-// loads nothing, which the others on its compute unit fill.
+// What it costs beyond the bytes (106 us at a copy's rate for 2048 x 128000 BF16, measured 132: 4.0 TB/s;
+// a few more under the profiler) are the exponentials, a quarter of the vector units' rate, and the phases in
+// which a workgroup ranks and loads nothing, which the others on its compute unit fill.
 template <typename T, int WAVES, int ITEMS>
 __global__ __launch_bounds__(64 * WAVES, 4) void k_top(const TopArgs a) {
     __shared__ TopShared sh;
@@ -929,12 +933,13 @@ int mf_top_logits(const void *logits, int32_t type, int64_t n, int64_t v, int64_
     const TopArgs args{logits, n, v, ld, int(k), temperature, values, indices, tail};
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        // Few rows take sixteen waves each (us, 64 x 128000 BF16, k = 64, 4 / 8 / 16 waves: 49 / 30 / 27).
+        // Few rows take sixteen waves each (us, 64 x 128000 BF16, k = 64, 4 / 8 / 16 waves: 49 / 30 / 27), of
+        // which a compute unit holds one workgroup: 256 rows 30, 300 rows 49, 511 rows 56 and 512 57.
         // Where the rows fill the chip, small workgroups let some list while others load; a longer
         // stretch and more waves pay where the bound would list many classes, and a wave's bound is near
         // the row's while k is at most half its lanes times the waves (us, 2048 rows BF16, four waves of 8
         // and of 16 pieces / eight of 16: 16000 classes, k = 64 41 / 44 / 68; 128000, k = 64 206 / 132 / 141;
-        // 128000, k = 128 380 / 195 / 174).
+        // 128000, k = 128 380 / 195 / 174; between them k * v is drawn from these alone).
         const i64 pieces = v / PIECE<T>;
         const auto launch = [&](auto kernel, int waves) {
             return launch_rows("top logits", kernel, args, waves, 0, static_cast<hipStream_t>(stream));
@@ -996,8 +1001,8 @@ int mf_distill_grad(const void *logits, int32_t type, int64_t n, int64_t v, int6
         using T = decltype(zero);
         const int lds = allow_lds(k_distill_grad<T, ROW_WAVES>, mark_bytes(v));
         if (lds) return lds;
-        return launch_rows("distillation gradient", k_distill_grad<T, ROW_WAVES>, args, ROW_WAVES, mark_bytes(v),
-                           static_cast<hipStream_t>(stream));
+        return launch_rows("distillation gradient", k_distill_grad<T, ROW_WAVES>, args, ROW_WAVES,
+                           mark_bytes(v), static_cast<hipStream_t>(stream));
     });
 }
 

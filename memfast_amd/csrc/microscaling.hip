@@ -98,7 +98,8 @@ struct MxArgs {
 // sums in LDS in the order of the waves. QUANTIZE: the workgroup quantizes x into LDS itself, while
 // its first weights are on their way, which saves a launch; else Q(x) is read from the cache. Where W
 // is not much larger, a wave's chain of two or three segments, its launch and the sums bound it: 1 x 4096 x
-// 11008 BF16 7.7 us (24 MB of weight, 3.1 TB/s), 24 x 11008 x 4096 10.5 us.
+// 11008 BF16 7.7 us (24 MB of weight, 3.1 TB/s). With more rows it is also what every workgroup reads of Q(x):
+// 24 x 11008 x 4096 10.5 us, 36 MB of x from the caches beside 24 MB of W; 64 rows 17 us, 96 MB of it.
 constexpr int FEW_WAVES = 8, FEW_TILE = 16, AHEAD = 2;
 
 __device__ __forceinline__ v4f mfma_few(v4u a, v4u b, v4f c, u32 sa, u32 sb) {
@@ -366,9 +367,10 @@ struct ProductPlan {
     bool quantize;   // Q(x) goes through memory
 };
 
-// k_mx_few reads Q(x) again for every 16 rows of W, k_mx_tile waits longer where it has few tiles (us, few /
-// tiles, n x k x o): 16 x 4096 x 11008 9.7 / 9.3, 24 of them 12.0 / 9.4, 64 21.6 / 9.8; 24 x 11008 x 4096
-// 10.3 / 18.9, 64 of them 16.9 / 19.2, 64 x 4096 x 4096 8.0 / 8.8.
+// k_mx_few reads Q(x) again for every 16 rows of W, k_mx_tile waits longer where it has few tiles (us, few
+// / tiles, n x k x o; other widths were not timed, and the depth is not in the rule): 16 x 4096 x 11008 9.7
+// / 9.3, 24 of them 12.0 / 9.4, 64 21.6 / 9.8; 24 x 11008 x 4096 10.3 / 18.9, 64 of them 16.9 / 19.2, 64 x
+// 4096 x 4096 8.0 / 8.8.
 constexpr i64 FEW_ROWS = 64, FEW_ROWS_WIDE = 16, WIDE = 8192;
 // A launch has fewer than 2^32 threads; k_mx_few takes 32 an output.
 constexpr i64 FEW_OUTPUTS = i64(1) << 26;

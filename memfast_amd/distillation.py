@@ -5,8 +5,10 @@ its digital original.  The original's whole output need not be kept: ``top_logit
 largest logits per row and the logarithm of the mass of all others, and ``distillation_loss``
 the student's loss against them, with its gradient.
 
-Both run in one pass over the logits each way, hold their sums in FP32 and read nothing back
-to the host; a row whose indices are wrong has a NaN loss.  Temperatures are normal numbers of FP32.
+Sums over the classes are held in FP32, over the entries and buckets in FP64, and nothing is read
+back to the host; a row whose indices are wrong has a NaN loss.  The largest logits take one pass
+over a row, or up to ten where it holds a NaN or many candidates (it rises all along, or k is above
+about 800); the loss takes one, with its gradient two.  Temperatures are normal numbers of FP32.
 """
 
 import torch
@@ -107,7 +109,10 @@ def distillation_loss(logits, values, indices, tail=None, *, temperature=1.0, we
 
     ``weight`` [...] weighs the rows (bool or floating; a row of weight 0 is not read).
     ``reduction``: "mean" (over the weights' sum; 0 if that is 0), "sum" or "none".  The loss is FP32;
-    gradients reach ``logits`` alone.  An operand with a tangent of forward mode is refused."""
+    gradients reach ``logits`` alone.  A sum or mean writes the gradient with the loss, for a loss that is
+    differentiated itself; where it is first scaled or joined by another factor, the backward writes it
+    again (``reduction="none"`` writes it in the backward alone).  An operand with a tangent of forward
+    mode is refused."""
     _check_logits(logits)
     _check_floating("values", values)
     temperature = _check_temperature(temperature)

@@ -1422,12 +1422,6 @@ def identity(device):
     )
 
 
-__all__ = [
-    "ResourceError", "BackendError", "cache_root", "atomic_write", "partial", "program",
-    "identity", "mm", "restore", "input_tiles", "weight_tiles", "transpose_packed",
-]
-
-
 # ---------------------------------------------------------------------------
 # 4-bit microscaled operands
 # ---------------------------------------------------------------------------
@@ -1620,3 +1614,9 @@ def distill_grad(logits, indices, temperature, weight, stats, reduction, incomin
             None if none else base, incoming.data_ptr(), int(none),
             int(ready), grad.data_ptr(), _stream(logits.device)), "distillation gradient")
     return grad
+
+
+__all__ = [
+    "ResourceError", "BackendError", "cache_root", "atomic_write", "partial", "program",
+    "identity", "mm", "restore", "input_tiles", "weight_tiles", "transpose_packed",
+]

@@ -85,7 +85,8 @@ def _part(label, value, shape):
 
 
 def mx_quantize(x):
-    """``x`` (float32, bfloat16 or float16, blocked along its last dimension) as an MXTensor."""
+    """``x`` (float32, bfloat16 or float16, blocked along its last dimension) as an MXTensor.  It has
+    fewer than 2**28 rows of fewer than 2**24 values; no gradient flows through it."""
     _check_floating("x", x)
     if x.ndim == 0:
         raise ValueError("x must have at least one dimension")
@@ -126,7 +127,8 @@ def mx_linear(x, weight, bias=None):
 
     ``weight`` is an MXTensor, or a tensor of x's dtype that is quantized in the call and gets a
     gradient.  ``bias`` [o] has x's dtype.  Rows of x and o are below 2**28 and k below 2**24; where a
-    gradient is wanted, x has at most 2**24 - 1 rows and o is at most 2**22.  An operand with a tangent of forward mode is refused."""
+    gradient is wanted, x has at most 2**24 - 1 rows and o is at most 2**22.  An operand with a
+    tangent of forward mode is refused."""
     _check_floating("x", x)
     held = isinstance(weight, MXTensor)
     if not held:
