@@ -622,6 +622,58 @@ int mf_distill_grad(const void *logits, int32_t type, int64_t n, int64_t v, int6
                     const float *incoming, int64_t incoming_step, int32_t unless_one, void *grad,
                     void *stream);
 
+/* ---- gated linear recurrence (linear_recurrence.hip) ----------------------- */
+/* For every channel of every sequence, over the steps of x [steps, batch, 2 * width] (update gates g,
+ * then candidates v, values next to each other; steps xt and sequences xb values apart, neither below 0):
+ *   u = sigmoid(g), c = tanh ? tanh(v) : v, h_t = u_t h_{t-1} + (1 - u_t) c_t, y_t = h_t,
+ * from state [batch, width] (NULL: zeros), with the last h in last [batch, width].  States are FP32; y has
+ * x's type, steps yt and sequences yb apart.  lengths [batch] (NULL: steps; taken within 0 .. steps): later
+ * steps are not read, their y is 0.  reverse: from the last step of each sequence to the first.
+ * marks (NULL, or the bytes that mf_recurrence_sizes gives) receives the states that mf_recurrence_grad
+ * starts from.  The workspace (mf_recurrence_sizes bytes, which may be 0; 8-byte aligned) belongs to the one
+ * call.  steps and batch < 2^31, width <= 2^24. */
+int mf_recurrence_sizes(int64_t steps, int64_t batch, int64_t width, int64_t *marks, int64_t *workspace);
+int mf_recurrence(const void *x, int32_t type, int64_t steps, int64_t batch, int64_t width, int64_t xt,
+                  int64_t xb, const float *state, const int64_t *lengths, int32_t reverse, int32_t tanh,
+                  void *y, int64_t yt, int64_t yb, float *last, float *marks, void *workspace,
+                  int64_t bytes, void *stream);
+/* Gradients for dy (x's type, as y lies; NULL: zeros) and dlast [batch, width] (NULL: zeros): dx as x lies
+ * (steps dt, sequences db apart) with zeros in the steps that are not taken, and dstate [batch, width]
+ * (or NULL). */
+int mf_recurrence_grad(const void *x, int32_t type, int64_t steps, int64_t batch, int64_t width,
+                       int64_t xt, int64_t xb, const int64_t *lengths, int32_t reverse, int32_t tanh,
+                       const float *marks, const void *dy, int64_t yt, int64_t yb, const float *dlast,
+                       void *dx, int64_t dt, int64_t db, float *dstate, void *workspace, int64_t bytes,
+                       void *stream);
+
+/* ---- dropout (dropout.hip) -------------------------------------------------- */
+/* y [n] = (residual, or 0) + (number[i] < dropped ? 0 : x[i] * 65536 / (65536 - dropped)), with number[i]
+ * the 16 bits i % 8 (from the lowest of the first word) of Philox 4x32-10 for the counter words (i / 8,
+ * i / 8 >> 32, event, event >> 32) and the key (seed, seed >> 32).  event_at (or NULL): the event is read
+ * there, on the device.  dropped: 0 .. 65536.  The gradient of x is the same call for dy without residual. */
+int mf_dropout(const void *x, int32_t type, int64_t n, const void *residual, uint32_t dropped,
+               uint64_t seed, uint64_t event, const int64_t *event_at, void *y, void *stream);
+
+/* ---- weights held as 4-bit whole numbers (int4.hip) -------------------------- */
+/* A weight [o, k] is scale * (code - zero) with codes 0 .. 15 and a scale and a zero point (0 .. 15; NULL: 8)
+ * for each group of `group` inputs, a power of two of at least 32.  With P = ceil(k / 128) and
+ * G = ceil(k / group), codes are [ceil(o / 16), P, 1024] bytes: input i of a span of 128 and output r of a
+ * tile of 16 are in byte (i / 8 % 4) * 256 + r * 16 + i / 32 * 4 + i % 4, in its lower half if i % 8 < 4.
+ * Scales (FP32, or x's type) and zero points are [ceil(o / 16), G, 16].  Codes are 16-byte aligned.
+ * o < 2^27, k < 2^24.
+ *
+ * mf_int4_quantize: codes and scales of w [o, k] (rows ldw apart), zero points 8: scale = max|w| / 7 in the
+ * scales' type (FP32 or w's), codes to nearest even; a group with a NaN or an infinity has scale NaN. */
+int mf_int4_quantize(const void *w, int32_t type, int64_t o, int64_t k, int64_t ldw, int64_t group,
+                     uint8_t *codes, void *scales, int32_t scale_type, void *stream);
+int mf_int4_dequantize(const uint8_t *codes, const void *scales, int32_t scale_type, const uint8_t *zeros,
+                       int64_t o, int64_t k, int64_t group, void *out, int32_t type, void *stream);
+/* out [n, o] = x W^T + bias (o values of x's type, or NULL) for x [n, k] (rows ldx apart): products of
+ * codes and x are summed in FP32 by group and scaled then. */
+int mf_int4_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, const uint8_t *codes,
+                   const void *scales, int32_t scale_type, const uint8_t *zeros, int64_t o, int64_t group,
+                   const void *bias, void *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

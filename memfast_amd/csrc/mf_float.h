@@ -25,6 +25,13 @@ template <typename T> struct alignas(16) Piece {
     T v[PIECE<T>];
 };
 
+// x in T, rounded from the FP32 number x: without the barrier the compiler may join the last operation
+// of x and its rounding to FP16 in one of two variants of a kernel and not in the other.
+template <typename T> __device__ __forceinline__ T rounded(float x) {
+    asm("" : "+v"(x));
+    return T(x);
+}
+
 // Calls f(T{}) with the element type of an MF_F32 / MF_BF16 / MF_F16 code.
 template <typename F> __host__ int with_type(int32_t type, F f) {
     switch (type) {

@@ -215,6 +215,16 @@ SIGNATURES = {
                          _P, _P, _P, _P, _P, _P, _P, _P], ct.c_int),
     "mf_distill_grad": ([_P, _I32, _I64, _I64, _I64, _P, _I64, ct.c_float, _P, _P, _P, _P, _P, _P,
                          _I64, _I32, _P, _P], ct.c_int),
+    "mf_recurrence_sizes": ([_I64, _I64, _I64, ct.POINTER(_I64), ct.POINTER(_I64)], ct.c_int),
+    "mf_recurrence": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _I32, _I32, _P, _I64, _I64, _P,
+                       _P, _P, _I64, _P], ct.c_int),
+    "mf_recurrence_grad": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I32, _I32, _P, _P, _I64, _I64,
+                            _P, _P, _I64, _I64, _P, _P, _I64, _P], ct.c_int),
+    "mf_dropout": ([_P, _I32, _I64, _P, ct.c_uint32, ct.c_uint64, ct.c_uint64, _P, _P, _P], ct.c_int),
+    "mf_int4_quantize": ([_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _P], ct.c_int),
+    "mf_int4_dequantize": ([_P, _P, _I32, _P, _I64, _I64, _I64, _P, _I32, _P], ct.c_int),
+    "mf_int4_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _I64, _I64, _P, _P, _P],
+                       ct.c_int),
     "mf_rng_uniform": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
     "mf_rng_normal": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
 }
@@ -1614,6 +1624,118 @@ def distill_grad(logits, indices, temperature, weight, stats, reduction, incomin
             None if none else base, incoming.data_ptr(), int(none),
             int(ready), grad.data_ptr(), _stream(logits.device)), "distillation gradient")
     return grad
+
+
+# ---------------------------------------------------------------------------
+# Gated linear recurrence
+# ---------------------------------------------------------------------------
+@lru_cache(maxsize=4096)
+def _recurrence_sizes(steps, batch, width):
+    """Bytes of the marks and of the workspace."""
+    marks, work = _I64(), _I64()
+    check(library().mf_recurrence_sizes(steps, batch, width, ct.byref(marks), ct.byref(work)),
+          "recurrence")
+    return marks.value, work.value
+
+
+def recurrence(x, state, lengths, reverse, tanh, batch_first, keep):
+    """States [T, B, H] and last state of ``x`` [T, B, 2H] (``batch_first``: the first two dimensions
+    are exchanged), and with ``keep`` the marks that ``recurrence_grad`` starts from (mf_recurrence)."""
+    t, b = (1, 0) if batch_first else (0, 1)
+    steps, batch, width = x.shape[t], x.shape[b], x.shape[2] // 2
+    device = x.device
+    marks_bytes, work_bytes = _recurrence_sizes(steps, batch, width)
+    y = torch.empty(x.shape[:2] + (width,), dtype=x.dtype, device=device)
+    last = torch.empty((batch, width), dtype=torch.float32, device=device)
+    marks = torch.empty(marks_bytes // 4, dtype=torch.float32, device=device) if keep else None
+    work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
+    xs, ys = x.stride(), y.stride()
+    with _on(device):
+        check(library().mf_recurrence(
+            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xs[t], xs[b], _ptr(state),
+            _ptr(lengths), reverse, tanh, y.data_ptr(), ys[t], ys[b], last.data_ptr(), _ptr(marks),
+            _ptr(work), work_bytes, _stream(device)), "recurrence")
+    return y, last, marks
+
+
+def recurrence_grad(x, lengths, reverse, tanh, batch_first, marks, dy, dlast, with_state):
+    """Gradients of ``recurrence``'s x and (``with_state``) state (mf_recurrence_grad)."""
+    t, b = (1, 0) if batch_first else (0, 1)
+    steps, batch, width = x.shape[t], x.shape[b], x.shape[2] // 2
+    device = x.device
+    work_bytes = _recurrence_sizes(steps, batch, width)[1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    dstate = torch.empty((batch, width), dtype=torch.float32, device=device) if with_state else None
+    work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
+    xs, ds, ys = x.stride(), dx.stride(), (0, 0) if dy is None else dy.stride()
+    with _on(device):
+        check(library().mf_recurrence_grad(
+            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xs[t], xs[b], _ptr(lengths),
+            reverse, tanh, marks.data_ptr(), _ptr(dy), ys[t], ys[b], _ptr(dlast), dx.data_ptr(), ds[t],
+            ds[b], _ptr(dstate), _ptr(work), work_bytes, _stream(device)), "recurrence gradient")
+    return dx, dstate
+
+
+# ---------------------------------------------------------------------------
+# Dropout
+# ---------------------------------------------------------------------------
+def dropout(x, residual, dropped, seed, event):
+    """Dropout of ``x``, contiguous, added to ``residual`` if there is one (mf_dropout).  ``event`` is
+    a number or an int64 tensor of one value on x's device."""
+    out = torch.empty_like(x)
+    held = isinstance(event, torch.Tensor)
+    with _on(x.device):
+        check(library().mf_dropout(
+            x.data_ptr(), FLOAT_TYPES[x.dtype], x.numel(), _ptr(residual), dropped, seed,
+            0 if held else event, event.data_ptr() if held else None, out.data_ptr(),
+            _stream(x.device)), "dropout")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Weights held as 4-bit whole numbers
+# ---------------------------------------------------------------------------
+INT4_TILE, INT4_SPAN, INT4_TILE_BYTES = 16, 128, 1024
+
+
+def int4_quantize(weight, group, scale_type):
+    """Codes and scales of ``weight`` [o, k] (mf_int4_quantize)."""
+    require_device(weight)
+    o, k = weight.shape
+    tiles = -(-o // INT4_TILE)
+    codes = torch.empty((tiles, -(-k // INT4_SPAN), INT4_TILE_BYTES), dtype=torch.uint8,
+                        device=weight.device)
+    scales = torch.empty((tiles, -(-k // group), INT4_TILE), dtype=scale_type, device=weight.device)
+    if weight.numel():
+        with _on(weight.device):
+            check(library().mf_int4_quantize(
+                _ptr(weight), FLOAT_TYPES[weight.dtype], o, k, weight.stride(0), group, _ptr(codes),
+                _ptr(scales), FLOAT_TYPES[scale_type], _stream(weight.device)), "4-bit quantization")
+    return codes, scales
+
+
+def int4_dequantize(codes, scales, zeros, o, k, group, dtype):
+    """The values [o, k] that codes, scales and zero points stand for (mf_int4_dequantize)."""
+    require_device(codes)
+    out = torch.empty((o, k), dtype=dtype, device=codes.device)
+    if out.numel():
+        with _on(codes.device):
+            check(library().mf_int4_dequantize(
+                _ptr(codes), _ptr(scales), FLOAT_TYPES[scales.dtype], _ptr(zeros), o, k, group,
+                _ptr(out), FLOAT_TYPES[dtype], _stream(codes.device)), "4-bit dequantization")
+    return out
+
+
+def int4_linear(x, codes, scales, zeros, o, group, bias):
+    """``x W^T + bias`` [n, o] for ``x`` [n, k] and a held W (mf_int4_linear)."""
+    n, k = x.shape
+    out = torch.empty((n, o), dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        check(library().mf_int4_linear(
+            x.data_ptr(), FLOAT_TYPES[x.dtype], n, k, x.stride(0), codes.data_ptr(),
+            scales.data_ptr(), FLOAT_TYPES[scales.dtype], _ptr(zeros), o, group, _ptr(bias),
+            out.data_ptr(), _stream(x.device)), "4-bit product")
+    return out
 
 
 __all__ = [

@@ -2,6 +2,8 @@
 
 from .conversion import convert_model, reset_read_events
 from .convolution import AnalogConv2d
+from .gated import Dropout, GatedRecurrence
+from .held import Int4Linear
 from .linear import AnalogLinear
 from .microscaled import MXLinear
 from .modules import Conv2d, Linear
@@ -15,4 +17,5 @@ __all__ = [
     "Linear", "Conv2d", "AnalogLinear", "AnalogConv2d", "TrainableAnalogLinear",
     "TrainableAnalogConv2d", "HATLinear", "HATConv2d", "AnalogRNNCell", "AnalogRNN",
     "AnalogGRUCell", "AnalogGRU", "convert_model", "reset_read_events", "MXLinear",
+    "GatedRecurrence", "Dropout", "Int4Linear",
 ]

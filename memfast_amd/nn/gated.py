@@ -1,0 +1,103 @@
+"""Recurrent layers without hidden projections, and dropout that stores no mask.
+
+A ``GatedRecurrence`` projects a whole sequence at once, so that an analog projection (``convert_model``
+replaces its nn.Linear layers) makes one read a layer and direction, where ``AnalogGRU`` makes two a step,
+and leaves the gated linear recurrence of memfast_amd/recurrence.py.
+"""
+
+import torch
+from torch import nn
+
+from ..recurrence import ACTIVATIONS, gated_recurrence
+from ..regularization import _check_probability, _number, dropout
+
+
+class Dropout(nn.Module):
+    """Dropout by ``memfast_amd.dropout``: each forward in training mode is the next event of ``seed``
+    (drawn from torch's default generator where none is given).  ``seed`` and ``event`` are part of the
+    state, so a restored model goes on with the masks that it would have had."""
+
+    def __init__(self, p=0.5, *, seed=None):
+        super().__init__()
+        self.p = _check_probability(p)
+        self.seed = int(torch.randint(1 << 62, ())) if seed is None else _number("seed", seed)
+        self.event = 0
+
+    def forward(self, x, residual=None):
+        event = self.event
+        if self.training:
+            self.event += 1
+        return dropout(x, self.p, seed=self.seed, event=event, residual=residual,
+                       training=self.training)
+
+    def get_extra_state(self):
+        return {"seed": self.seed, "event": self.event}
+
+    def set_extra_state(self, state):
+        self.seed, self.event = _number("seed", state["seed"]), _number("event", state["event"])
+
+    def extra_repr(self):
+        return f"p={self.p}"
+
+
+class GatedRecurrence(nn.Module):
+    """Stacked gated linear recurrences with nn.GRU's arguments: every layer and direction is a projection
+    to update gates and candidates and ``gated_recurrence`` of them, with ``Dropout`` between layers.
+
+    ``projections`` holds the nn.Linear layers, one for each layer and direction; any layer with the same
+    outputs may take their place (analog layers, ``MXLinear``, ``Int4Linear``)."""
+
+    def __init__(self, input_size, hidden_size, num_layers=1, *, bias=True, batch_first=False,
+                 dropout=0.0, bidirectional=False, activation="tanh", device=None, dtype=None):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError("activation must be 'tanh' or None")
+        if min(input_size, hidden_size, num_layers) < 1:
+            raise ValueError("input_size, hidden_size and num_layers must be positive")
+        self.input_size, self.hidden_size, self.num_layers = input_size, hidden_size, num_layers
+        self.batch_first, self.bidirectional = bool(batch_first), bool(bidirectional)
+        self.activation = activation
+        self.directions = 2 if bidirectional else 1
+        self.projections = nn.ModuleList(
+            nn.Linear(input_size if layer == 0 else self.directions * hidden_size, 2 * hidden_size,
+                      bias=bias, device=device, dtype=dtype)
+            for layer in range(num_layers) for _ in range(self.directions))
+        self.dropouts = nn.ModuleList(Dropout(dropout) for _ in range(num_layers - 1))
+
+    def forward(self, x, hx=None, lengths=None):
+        """(states, last states [layers * directions, B, H] in FP32) of ``x`` [T, B, input_size], or
+        [B, T, input_size] with ``batch_first``, or [T, input_size]; ``hx`` as the last states, ``lengths``
+        as in ``gated_recurrence``."""
+        if not torch.is_tensor(x) or x.ndim not in (2, 3) or x.shape[-1] != self.input_size:
+            raise ValueError("input must be a sequence with matching input_size")
+        steps = x.shape[1] if x.ndim == 3 and self.batch_first else x.shape[0]
+        if steps == 0:
+            raise ValueError("sequence must contain at least one timestep")
+        if hx is not None:
+            batch = () if x.ndim == 2 else (x.shape[0] if self.batch_first else x.shape[1],)
+            expected = (len(self.projections), *batch, self.hidden_size)
+            if not torch.is_tensor(hx) or hx.shape != expected:
+                raise ValueError("hidden state must match layers, directions and batch")
+        finals = []
+        for layer in range(self.num_layers):
+            outputs = []
+            for direction in range(self.directions):
+                index = layer * self.directions + direction
+                states, final = gated_recurrence(
+                    self.projections[index](x), None if hx is None else hx[index],
+                    activation=self.activation, lengths=lengths, reverse=bool(direction),
+                    batch_first=self.batch_first)
+                outputs.append(states)
+                finals.append(final)
+            x = outputs[0] if len(outputs) == 1 else torch.cat(outputs, -1)
+            if layer + 1 < self.num_layers:
+                x = self.dropouts[layer](x)
+        return x, torch.stack(finals)
+
+    def extra_repr(self):
+        return (f"{self.input_size}, {self.hidden_size}, num_layers={self.num_layers}, "
+                f"batch_first={self.batch_first}, bidirectional={self.bidirectional}, "
+                f"activation={self.activation!r}")
+
+
+__all__ = ["Dropout", "GatedRecurrence"]
