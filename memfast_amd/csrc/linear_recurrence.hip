@@ -14,10 +14,12 @@
 
 namespace mf {
 
-// A wave takes 64 * V channels and CHUNK steps of them, the up to MOST_WAVES waves of a workgroup
-// consecutive chunks: SPAN steps at a time, whose maps they exchange in LDS.
-constexpr int CHUNK = 8, MOST_WAVES = 16, SPAN = CHUNK * MOST_WAVES;
-constexpr float LOG2E = 1.44269504f, LOG2E_LOW = 1.92596299e-8f, LN2 = 0.693147181f;
+// A wave takes 64 channels and CHUNK steps of them, the up to WAVES waves of a workgroup consecutive chunks,
+// whose maps they exchange in LDS. States are kept every SPAN steps for the gradients, which is what a
+// workgroup of either shape takes at a time: eight waves of 16 steps, and for sequences that are no longer
+// sixteen of 8.
+constexpr int SPAN = 128, MOST_WAVES = 16;
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
 
 struct RecurrenceArgs {
     const void *x;          // [steps, batch, 2 width]: gates, then candidates
@@ -43,26 +45,24 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Group {
     T v[V];
 };
 
-// exp(-x) for x >= 0: the rounding of x log2(e) is made good, so that far gates keep their digits too.
-__device__ __forceinline__ float decay(float x) {
-    const float t = -x * LOG2E;
-    const float rest = fmaf(-x, LOG2E, -t) - x * LOG2E_LOW;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return x < 126.0f ? fmaf(e, rest * LN2, e) : e;
-}
-
-// sigmoid(g) and sigmoid(-g): the smaller one is not a difference, so either end keeps its digits.
+// sigmoid(g) and sigmoid(-g) as u = 1 / (1 + e) and k = e u with e = exp(-g): no difference of near numbers
+// at either end. What the rounding of g log2(e) took from the exponent is made good, so that k keeps its
+// digits for far gates too. The bounds (which pass a NaN on) keep e finite, where u is 2^-126 and not less,
+// and let it reach 0.
 __device__ __forceinline__ void gates(float g, float &u, float &k) {
-    const float e = decay(fabsf(g)), big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
-    u = g >= 0.0f ? big : small;
-    k = g >= 0.0f ? small : big;
+    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 110.0f);
+    const float t = g * -LOG2E, rest = fmaf(g, -LOG2E, -t);
+    float e = __builtin_amdgcn_exp2f(t);
+    e = fmaf(e, rest * LN2, e);
+    u = __builtin_amdgcn_rcpf(1.0f + e);
+    k = e * u;
 }
 
-// tanh: (1 - e) / (1 + e) with e = exp(-2 |x|), and where that difference would lose digits the series
+// tanh: 1 - 2 / (1 + exp(2 x)), and where that difference would lose digits the series
 // x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835 (below 1/4 the next term is under 1e-8 of it).
 __device__ __forceinline__ float hyperbolic_tangent(float x) {
-    const float e = decay(2.0f * fabsf(x));
-    const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+    const float e = __builtin_amdgcn_exp2f(x * (2.0f * LOG2E));
+    const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
     const float s = x * x;
     float p = fmaf(s, 62.0f / 2835.0f, -17.0f / 315.0f);
     p = fmaf(s, p, 2.0f / 15.0f);
@@ -70,21 +70,23 @@ __device__ __forceinline__ float hyperbolic_tangent(float x) {
     return fabsf(x) < 0.25f ? fmaf(x * s, p, x) : far;
 }
 
-// What one workgroup works on.
+// What one workgroup works on. All but the channel is the same for a wave, so that addresses are scalar
+// but for the lane's own offset in a row, in bytes.
 template <typename T, int V> struct Place {
-    i64 b, channel, segment, length, begin, end, step;
-    bool inside;
-    const T *x;
+    i64 b, segment, length, begin, end;
+    u32 channel, lane_bytes;
+    bool inside, reverse;
 
-    __device__ __forceinline__ explicit Place(const RecurrenceArgs &a) {
+    __device__ __forceinline__ explicit Place(const RecurrenceArgs &a) : reverse(a.reverse) {
         u32 id = blockIdx.x;
         const u32 tile = id % u32(a.tiles);
         id /= u32(a.tiles);
         b = a.first + id % u32(a.batch);
         segment = id / u32(a.batch);
-        const i64 c = (i64(tile) * 64 + (threadIdx.x & 63)) * V;
+        const u32 c = (tile * 64 + (threadIdx.x & 63)) * V;
         inside = c < a.width;
         channel = inside ? c : 0;
+        lane_bytes = channel * u32(sizeof(T));
         length = a.steps;
         if (a.lengths) {
             length = a.lengths[b];
@@ -92,36 +94,66 @@ template <typename T, int V> struct Place {
         }
         begin = segment * a.segment;
         end = min(begin + a.segment, a.steps);
-        // Step s of the recurrence lies at time s, or in reverse at length - 1 - s.
-        step = a.reverse ? -a.xt : a.xt;
-        x = static_cast<const T *>(a.x) + b * a.xb + channel + (a.reverse ? (length - 1) * a.xt : 0);
     }
-    __device__ __forceinline__ i64 time(const RecurrenceArgs &a, i64 s) const {
-        return a.reverse ? length - 1 - s : s;
-    }
+    // Step s of the recurrence lies at time s, or in reverse at length - 1 - s.
+    __device__ __forceinline__ i64 time(i64 s) const { return reverse ? length - 1 - s : s; }
     __device__ __forceinline__ i64 at(const RecurrenceArgs &a) const { return b * a.width + channel; }
 };
 
-// Gates and candidates of CHUNK steps from s on. Steps past the last are read as the last one, which
-// exists (length > 0), and left out later.
-template <typename T, int V> struct Loaded {
-    Group<T, V> g[CHUNK], v[CHUNK];
-    __device__ __forceinline__ void load(const RecurrenceArgs &a, const Place<T, V> &p, i64 s) {
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            const T *row = p.x + min(s + i, p.length - 1) * p.step;
-            g[i] = *reinterpret_cast<const Group<T, V> *>(row);
-            v[i] = *reinterpret_cast<const Group<T, V> *>(row + a.width);
-        }
-    }
+// The rows of one tensor that a workgroup goes through: step s lies `step` bytes behind step s - 1.
+template <typename T, int V> struct Rows {
+    char *first;        // of step 0
+    i64 step;
+    __device__ __forceinline__ Rows(const void *p, const Place<T, V> &place, i64 sequence, i64 distance)
+        : first(static_cast<char *>(const_cast<void *>(p)) +
+                (place.b * sequence + place.time(0) * distance) * i64(sizeof(T))),
+          step((place.reverse ? -distance : distance) * i64(sizeof(T))) {}
+    __device__ __forceinline__ char *at(i64 s) const { return first + s * step; }
 };
+
+template <typename G> __device__ __forceinline__ G get(const char *row, u32 bytes) {
+    return *reinterpret_cast<const G *>(row + bytes);
+}
+template <typename G> __device__ __forceinline__ void put(char *row, u32 bytes, G v) {
+    *reinterpret_cast<G *>(row + bytes) = v;
+}
+
+// f(i, row) for the CHUNK rows of steps s + i. Rows past the last step are the last one's, which exists
+// (length > 0): what they give is left out later.
+template <int CHUNK, typename T, int V, typename F>
+__device__ __forceinline__ void each_row(const Rows<T, V> &rows, i64 s, i64 length, F f) {
+    if (s + CHUNK <= length) {
+        char *row = rows.at(s);
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i, row += rows.step) f(i, row);
+    } else {
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) f(i, rows.at(min(s + i, length - 1)));
+    }
+}
+
+// The same for the steps that exist alone.
+template <int CHUNK, typename T, int V, typename F>
+__device__ __forceinline__ void each_step(const Rows<T, V> &rows, i64 s, i64 length, F f) {
+    char *row = rows.at(s);
+    if (s + CHUNK <= length) {
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i, row += rows.step) f(i, row);
+    } else {
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i, row += rows.step)
+            if (s + i < length) f(i, row);
+    }
+}
+
+__device__ __forceinline__ int wave_of_thread() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // carry through the maps of the segments first .. last - 1, in order (BACK: from the last on): every
 // wave composes its share, whose loads it has under way together, and the shares meet in LDS.
 template <int V, bool BACK>
 __device__ __forceinline__ void fold(const RecurrenceArgs &a, i64 b, i64 channel, i64 first, i64 last,
                                      float (*maps)[2][64 * V], float (&carry)[V]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = wave_of_thread(), waves = blockDim.x >> 6;
     const i64 share = (last - first + waves - 1) / waves;
     const i64 from = min(first + wave * share, last), to = min(from + share, last);
     float A[V], S[V];
@@ -161,234 +193,206 @@ __device__ __forceinline__ void fold(const RecurrenceArgs &a, i64 b, i64 channel
     __syncthreads();
 }
 
-// Writes zeros at the times from the sequence's length on.
-template <typename T, int V>
-__device__ __forceinline__ void blank(const RecurrenceArgs &a, const Place<T, V> &p, T *rows, i64 step,
-                                      int wave, int waves, i64 second) {
+// Writes zeros at the times from the sequence's length on, in rows `distance` values apart, and where
+// `second` is not 0 again that many bytes further.
+template <typename T>
+__device__ __forceinline__ void blank(const Place<T, 1> &p, void *rows, i64 sequence, i64 distance, int wave,
+                                      int waves, u32 second) {
     if (!p.inside) return;
-    const Group<T, V> zero{};
     for (i64 t = max(p.begin, p.length) + wave; t < p.end; t += waves) {
-        *reinterpret_cast<Group<T, V> *>(rows + t * step) = zero;
-        if (second) *reinterpret_cast<Group<T, V> *>(rows + t * step + second) = zero;
+        char *row = static_cast<char *>(rows) + (p.b * sequence + t * distance) * i64(sizeof(T));
+        put(row, p.lane_bytes, T(0.0f));
+        if (second) put(row, p.lane_bytes + second, T(0.0f));
     }
 }
 
-template <typename T, int V, bool TANH>
-__global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence(const RecurrenceArgs a) {
-    __shared__ float maps[2][MOST_WAVES][2][64 * V];
-    const Place<T, V> p(a);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// Bound by its bytes and by the vector units, which are busy two thirds of the time: 8 x 4096 x 2048 BF16 in
+// 98 us (403 MB, 4.1 TB/s). Two channels a lane, for wider rows of loads, took 104; sixteen waves of eight
+// steps, which join twice as many maps, 115.
+template <typename T, bool TANH, int WAVES, int CHUNK>
+__global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs a) {
+    __shared__ float maps[2][WAVES][2][64];
+    const Place<T, 1> p(a);
+    const int lane = threadIdx.x & 63, wave = wave_of_thread(), waves = blockDim.x >> 6;
     const int span = waves * CHUNK;
-    T *y = static_cast<T *>(a.y) + p.b * a.yb + p.channel;
+    const u32 second = p.lane_bytes + u32(a.width) * u32(sizeof(T));
+    const Rows<T, 1> x(a.x, p, a.xb, a.xt), y(a.y, p, a.yb, a.yt);
     const i64 end = min(p.end, p.length);
 
-    Loaded<T, V> next;
-    if (p.begin < end) next.load(a, p, p.begin + wave * CHUNK);
-    float carry[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) carry[j] = a.state ? a.state[p.at(a) + j] : 0.0f;
+    T next_g[CHUNK], next_v[CHUNK];
+    const auto load = [&](i64 s) {
+        each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
+            next_g[i] = get<T>(row, p.lane_bytes);
+            next_v[i] = get<T>(row, second);
+        });
+    };
+    if (p.begin < end) load(p.begin + wave * CHUNK);
+    float carry[1] = {a.state ? a.state[p.at(a)] : 0.0f};
     // The state before this segment: the maps of those before it, in order.
-    if (p.segment) fold<V, false>(a, p.b, p.channel, 0, p.segment, maps[0], carry);
+    if (p.segment) fold<1, false>(a, p.b, p.channel, 0, p.segment, maps[0], carry);
 
     int turn = 0;
     for (i64 base = p.begin; base < end; base += span, turn ^= 1) {
         const i64 s = base + wave * CHUNK;
-        float u[CHUNK][V], in[CHUNK][V], A[V], S[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) A[j] = 1.0f, S[j] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float k, c = float(next.v[i].v[j]);
-                gates(float(next.g[i].v[j]), u[i][j], k);
-                if (TANH) c = hyperbolic_tangent(c);
-                const bool live = s + i < p.length;
-                u[i][j] = live ? u[i][j] : 1.0f;
-                in[i][j] = live ? k * c : 0.0f;
-                A[j] *= u[i][j];
-                S[j] = fmaf(u[i][j], S[j], in[i][j]);
-            }
-        if (base + span < end) next.load(a, p, s + span);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            maps[turn][wave][0][lane * V + j] = A[j];
-            maps[turn][wave][1][lane * V + j] = S[j];
-        }
-        __syncthreads();    // one a turn: the other turn's maps are read before its barrier
-        float h[V];
-        for (int w = 0; w < waves; ++w) {
-            if (w == wave)
-#pragma unroll
-                for (int j = 0; j < V; ++j) h[j] = carry[j];
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                carry[j] = fmaf(maps[turn][w][0][lane * V + j], carry[j],
-                                maps[turn][w][1][lane * V + j]);
-        }
-        if (a.marks && wave == 0 && p.inside) {
-            float *mark = a.marks + (base / SPAN * a.all) * a.width + p.at(a);
-#pragma unroll
-            for (int j = 0; j < V; ++j) mark[j] = h[j];
-        }
+        float u[CHUNK], in[CHUNK], A = 1.0f, S = 0.0f, h;
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i) {
-            Group<T, V> row;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                h[j] = fmaf(u[i][j], h[j], in[i][j]);
-                row.v[j] = rounded<T>(h[j]);
-            }
-            if (p.inside && s + i < p.length)
-                *reinterpret_cast<Group<T, V> *>(y + p.time(a, s + i) * a.yt) = row;
+            float k, c = float(next_v[i]);
+            gates(float(next_g[i]), u[i], k);
+            if (TANH) c = hyperbolic_tangent(c);
+            in[i] = k * c;
         }
-    }
-    blank(a, p, y, a.yt, wave, waves, 0);
-    if (wave == 0 && p.inside && p.segment == a.segments - 1)
+        if (s + CHUNK > p.length)
 #pragma unroll
-        for (int j = 0; j < V; ++j) a.last[p.at(a) + j] = carry[j];
+            for (int i = 0; i < CHUNK; ++i)
+                if (s + i >= p.length) u[i] = 1.0f, in[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) {
+            A *= u[i];
+            S = fmaf(u[i], S, in[i]);
+        }
+        if (base + span < end) load(s + span);
+        maps[turn][wave][0][lane] = A;
+        maps[turn][wave][1][lane] = S;
+        __syncthreads();    // one a turn: the other turn's maps are read before its barrier
+        for (int w = 0; w < waves; ++w) {
+            if (w == wave) h = carry[0];
+            carry[0] = fmaf(maps[turn][w][0][lane], carry[0], maps[turn][w][1][lane]);
+        }
+        if (a.marks && s % SPAN == 0 && s < p.length && p.inside)
+            a.marks[s / SPAN * a.all * a.width + p.at(a)] = h;
+        T out[CHUNK];
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) {
+            h = fmaf(u[i], h, in[i]);
+            out[i] = rounded<T>(h);
+        }
+        if (p.inside)
+            each_step<CHUNK>(y, s, p.length, [&](int i, char *row) { put(row, p.lane_bytes, out[i]); });
+    }
+    blank(p, a.y, a.yb, a.yt, wave, waves, 0);
+    if (wave == 0 && p.inside && p.segment == a.segments - 1) a.last[p.at(a)] = carry[0];
 }
 
-template <typename T, int V, bool TANH>
-__global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_grad(const RecurrenceArgs a) {
-    __shared__ float maps[2][MOST_WAVES][3][64 * V];
-    const Place<T, V> p(a);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// As above: 8 x 4096 x 2048 BF16 in 160 us (671 MB, 4.2 TB/s), with sixteen waves of eight steps 175. Two
+// channels a lane need more registers than there are.
+template <typename T, bool TANH, int WAVES, int CHUNK>
+__global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const RecurrenceArgs a) {
+    __shared__ float maps[2][WAVES][3][64];
+    const Place<T, 1> p(a);
+    const int lane = threadIdx.x & 63, wave = wave_of_thread(), waves = blockDim.x >> 6;
     const int span = waves * CHUNK;
-    const T *dy = static_cast<const T *>(a.y) + p.b * a.yb + p.channel;
-    T *dx = static_cast<T *>(a.dx) + p.b * a.db + p.channel;
+    const u32 second = p.lane_bytes + u32(a.width) * u32(sizeof(T));
+    const Rows<T, 1> x(a.x, p, a.xb, a.xt), dy(a.y, p, a.yb, a.yt), dx(a.dx, p, a.db, a.dt);
     const i64 end = min(p.end, p.length);
 
-    Loaded<T, V> next;
-    Group<T, V> next_dy[CHUNK];
-    float mark[V];
+    T next_g[CHUNK], next_v[CHUNK], next_dy[CHUNK];
+    float mark;
     const auto load = [&](i64 base) {
         const i64 s = base + wave * CHUNK;
-        next.load(a, p, s);
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i)
-            next_dy[i] = a.y ? *reinterpret_cast<const Group<T, V> *>(
-                                   dy + p.time(a, min(s + i, p.length - 1)) * a.yt)
-                             : Group<T, V>{};
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            mark[j] = a.marks[(base / SPAN * a.all) * a.width + p.at(a) + j];
+        each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
+            next_g[i] = get<T>(row, p.lane_bytes);
+            next_v[i] = get<T>(row, second);
+        });
+        if (a.y)
+            each_row<CHUNK>(dy, s, p.length,
+                            [&](int i, const char *row) { next_dy[i] = get<T>(row, p.lane_bytes); });
+        mark = a.marks[(base / SPAN * a.all) * a.width + p.at(a)];
     };
+#pragma unroll
+    for (int i = 0; i < CHUNK; ++i) next_dy[i] = T(0.0f);
     const i64 top = p.begin + (end - p.begin - 1) / span * span;
     if (p.begin < end) load(top);
     // The gradient of the state after this segment: the maps of those behind it, from the last on.
-    float carry[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) carry[j] = a.last ? a.last[p.at(a) + j] : 0.0f;
+    float carry[1] = {a.last ? a.last[p.at(a)] : 0.0f};
     if (p.segment + 1 < a.segments)
-        fold<V, true>(a, p.b, p.channel, p.segment + 1, a.segments,
-                      reinterpret_cast<float (*)[2][64 * V]>(&maps), carry);
+        fold<1, true>(a, p.b, p.channel, p.segment + 1, a.segments,
+                      reinterpret_cast<float (*)[2][64]>(&maps), carry);
 
     int turn = 0;
     if (p.begin < end)
         for (i64 base = top; base >= p.begin; base -= span, turn ^= 1) {
             const i64 s = base + wave * CHUNK;
-            float u[CHUNK][V], k[CHUNK][V], c[CHUNK][V], g[CHUNK][V], A[V], S[V], Q[V], h[V], r[V];
+            float u[CHUNK], k[CHUNK], c[CHUNK], g[CHUNK], A = 1.0f, S = 0.0f, Q = 0.0f, h = mark, r;
 #pragma unroll
-            for (int j = 0; j < V; ++j) A[j] = 1.0f, S[j] = 0.0f, Q[j] = 0.0f, h[j] = mark[j];
-#pragma unroll
-            for (int i = 0; i < CHUNK; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    gates(float(next.g[i].v[j]), u[i][j], k[i][j]);
-                    c[i][j] = float(next.v[i].v[j]);
-                    if (TANH) c[i][j] = hyperbolic_tangent(c[i][j]);
-                    const bool live = s + i < p.length;
-                    u[i][j] = live ? u[i][j] : 1.0f;
-                    k[i][j] = live ? k[i][j] : 0.0f;
-                    c[i][j] = live ? c[i][j] : 0.0f;
-                    g[i][j] = live ? float(next_dy[i].v[j]) : 0.0f;
-                    A[j] *= u[i][j];
-                    S[j] = fmaf(u[i][j], S[j], k[i][j] * c[i][j]);
-                }
-#pragma unroll
-            for (int i = CHUNK - 1; i >= 0; --i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) Q[j] = u[i][j] * (g[i][j] + Q[j]);
-            if (base > p.begin) load(base - span);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                maps[turn][wave][0][lane * V + j] = A[j];
-                maps[turn][wave][1][lane * V + j] = S[j];
-                maps[turn][wave][2][lane * V + j] = Q[j];
+            for (int i = 0; i < CHUNK; ++i) {
+                gates(float(next_g[i]), u[i], k[i]);
+                c[i] = float(next_v[i]);
+                if (TANH) c[i] = hyperbolic_tangent(c[i]);
+                g[i] = float(next_dy[i]);
             }
+            if (s + CHUNK > p.length)
+#pragma unroll
+                for (int i = 0; i < CHUNK; ++i)
+                    if (s + i >= p.length) u[i] = 1.0f, k[i] = 0.0f, c[i] = 0.0f, g[i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i) {
+                A *= u[i];
+                S = fmaf(u[i], S, k[i] * c[i]);
+            }
+#pragma unroll
+            for (int i = CHUNK - 1; i >= 0; --i) Q = u[i] * (g[i] + Q);
+            if (base > p.begin) load(base - span);
+            maps[turn][wave][0][lane] = A;
+            maps[turn][wave][1][lane] = S;
+            maps[turn][wave][2][lane] = Q;
             __syncthreads();
-            for (int w = 0; w < wave; ++w)
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    h[j] = fmaf(maps[turn][w][0][lane * V + j], h[j], maps[turn][w][1][lane * V + j]);
+            for (int w = 0; w < wave; ++w) h = fmaf(maps[turn][w][0][lane], h, maps[turn][w][1][lane]);
             for (int w = waves - 1; w >= 0; --w) {
-                if (w == wave)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) r[j] = carry[j];
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    carry[j] = fmaf(maps[turn][w][0][lane * V + j], carry[j],
-                                    maps[turn][w][2][lane * V + j]);
+                if (w == wave) r = carry[0];
+                carry[0] = fmaf(maps[turn][w][0][lane], carry[0], maps[turn][w][2][lane]);
             }
             // Factors of G in both gradients, then G from the last step back.
 #pragma unroll
-            for (int i = 0; i < CHUNK; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float before = h[j];
-                    h[j] = fmaf(u[i][j], before, k[i][j] * c[i][j]);
-                    const float dv = TANH ? k[i][j] * fmaf(-c[i][j], c[i][j], 1.0f) : k[i][j];
-                    c[i][j] = (before - c[i][j]) * (u[i][j] * k[i][j]);
-                    k[i][j] = dv;
-                }
+            for (int i = 0; i < CHUNK; ++i) {
+                const float before = h;
+                h = fmaf(u[i], before, k[i] * c[i]);
+                const float dv = TANH ? k[i] * fmaf(-c[i], c[i], 1.0f) : k[i];
+                c[i] = (before - c[i]) * (u[i] * k[i]);
+                k[i] = dv;
+            }
+            T dg[CHUNK], dv[CHUNK];
 #pragma unroll
             for (int i = CHUNK - 1; i >= 0; --i) {
-                Group<T, V> dg, dv;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float G = g[i][j] + r[j];
-                    dg.v[j] = rounded<T>(G * c[i][j]);
-                    dv.v[j] = rounded<T>(G * k[i][j]);
-                    r[j] = u[i][j] * G;
-                }
-                if (p.inside && s + i < p.length) {
-                    T *row = dx + p.time(a, s + i) * a.dt;
-                    *reinterpret_cast<Group<T, V> *>(row) = dg;
-                    *reinterpret_cast<Group<T, V> *>(row + a.width) = dv;
-                }
+                const float G = g[i] + r;
+                dg[i] = rounded<T>(G * c[i]);
+                dv[i] = rounded<T>(G * k[i]);
+                r = u[i] * G;
             }
+            if (p.inside)
+                each_step<CHUNK>(dx, s, p.length, [&](int i, char *row) {
+                    put(row, p.lane_bytes, dg[i]);
+                    put(row, second, dv[i]);
+                });
         }
-    blank(a, p, dx, a.dt, wave, waves, a.width);
-    if (a.dstate && wave == 0 && p.inside && p.segment == 0)
-#pragma unroll
-        for (int j = 0; j < V; ++j) a.dstate[p.at(a) + j] = carry[j];
+    blank(p, a.dx, a.db, a.dt, wave, waves, u32(a.width) * u32(sizeof(T)));
+    if (a.dstate && wave == 0 && p.inside && p.segment == 0) a.dstate[p.at(a)] = carry[0];
 }
 
 // A and S of every segment but the last (GRAD: A and Q of every segment but the first), each wave its
 // share of the segment's steps.
 template <typename T, int V, bool TANH, bool GRAD>
 __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const RecurrenceArgs a) {
+    constexpr int CHUNK = 8;
     __shared__ float maps[MOST_WAVES][2][64 * V];
-    Place<T, V> p(a);
+    const Place<T, V> p(a);
     if (p.segment == (GRAD ? 0 : a.segments - 1)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const T *dy = static_cast<const T *>(a.y) + p.b * a.yb + p.channel;
+    const int lane = threadIdx.x & 63, wave = wave_of_thread(), waves = blockDim.x >> 6;
+    const u32 second = p.lane_bytes + u32(a.width) * u32(sizeof(T));
+    const Rows<T, V> x(a.x, p, a.xb, a.xt), dy(a.y, p, a.yb, a.yt);
     const i64 share = a.segment / waves, end = min(p.begin + (wave + 1) * share, p.length);
     float A[V], S[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) A[j] = 1.0f, S[j] = 0.0f;
     for (i64 s = p.begin + wave * share; s < end; s += CHUNK) {
         Group<T, V> g[CHUNK], v[CHUNK];
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i) {
-            const i64 at = min(s + i, p.length - 1);
-            const T *row = p.x + at * p.step;
-            g[i] = *reinterpret_cast<const Group<T, V> *>(row);
-            if (!GRAD) v[i] = *reinterpret_cast<const Group<T, V> *>(row + a.width);
-            else v[i] = a.y ? *reinterpret_cast<const Group<T, V> *>(dy + p.time(a, at) * a.yt)
-                            : Group<T, V>{};
-        }
+        each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
+            g[i] = get<Group<T, V>>(row, p.lane_bytes);
+            v[i] = GRAD ? Group<T, V>{} : get<Group<T, V>>(row, second);
+        });
+        if (GRAD && a.y)
+            each_row<CHUNK>(dy, s, p.length,
+                            [&](int i, const char *row) { v[i] = get<Group<T, V>>(row, p.lane_bytes); });
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i)
 #pragma unroll
@@ -438,9 +442,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
 struct Split {
     i64 segments = 1, segment;
     Split(i64 steps, i64 batch, i64 width) : segment((steps + SPAN - 1) / SPAN * SPAN) {
-        const i64 columns = batch * ((width + 127) / 128), spans = segment / SPAN;
-        if (columns >= 256 || spans < 4) return;
-        const i64 wanted = std::min<i64>({(512 + columns - 1) / columns, spans / 2, 256});
+        const i64 columns = batch * ((width + 63) / 64), spans = segment / SPAN;
+        if (columns >= 256 || spans < 3) return;
+        const i64 wanted = std::min<i64>((512 + columns - 1) / columns, spans);
         segment = (spans + wanted - 1) / wanted * SPAN;
         segments = (steps + segment - 1) / segment;
     }
@@ -462,7 +466,7 @@ int check_recurrence(const void *x, int32_t type, i64 steps, i64 batch, i64 widt
     return MF_OK;
 }
 
-// Calls f(V) with the channels of a lane: two where every row of every tensor allows it.
+// Calls f(V) with the channels of a lane that reduces segments: two where every row allows it.
 template <typename F> int with_group(bool pairs, F f) {
     return pairs ? f(std::integral_constant<int, 2>{}) : f(std::integral_constant<int, 1>{});
 }
@@ -483,8 +487,6 @@ int launch_recurrence(const char *what, K kernel, RecurrenceArgs a, i64 batch, i
     }
     return MF_OK;
 }
-
-int waves_of(i64 steps) { return int(std::min<i64>(MOST_WAVES, (steps + CHUNK - 1) / CHUNK)); }
 
 }  // namespace mf
 
@@ -523,18 +525,22 @@ int mf_recurrence(const void *x, int32_t type, int64_t steps, int64_t batch, int
     hipStream_t s = static_cast<hipStream_t>(stream);
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        return with_group(pairs, [&](auto group) {
-            constexpr int V = decltype(group)::value;
-            if (a.segments > 1) {
-                const int parts = launch_recurrence(
-                    "recurrence parts", tanh ? k_recurrence_parts<T, V, true, false>
-                                             : k_recurrence_parts<T, V, false, false>,
-                    a, batch, V, MOST_WAVES, s);
-                if (parts) return parts;
-            }
-            return launch_recurrence("recurrence", tanh ? k_recurrence<T, V, true> : k_recurrence<T, V, false>,
-                                     a, batch, V, waves_of(steps), s);
-        });
+        if (a.segments > 1) {
+            const int parts = with_group(pairs, [&](auto group) {
+                constexpr int V = decltype(group)::value;
+                return launch_recurrence("recurrence parts",
+                                         tanh ? k_recurrence_parts<T, V, true, false>
+                                              : k_recurrence_parts<T, V, false, false>,
+                                         a, batch, V, MOST_WAVES, s);
+            });
+            if (parts) return parts;
+        }
+        if (steps > SPAN)
+            return launch_recurrence("recurrence", tanh ? k_recurrence<T, true, 8, 16>
+                                                        : k_recurrence<T, false, 8, 16>, a, batch, 1, 8, s);
+        return launch_recurrence("recurrence", tanh ? k_recurrence<T, true, 16, 8>
+                                                    : k_recurrence<T, false, 16, 8>,
+                                 a, batch, 1, int((steps + 7) / 8), s);
     });
 }
 
@@ -559,24 +565,25 @@ int mf_recurrence_grad(const void *x, int32_t type, int64_t steps, int64_t batch
     a.segments = split.segments, a.segment = split.segment;
     a.parts = static_cast<float *>(workspace);
     const uintptr_t pair = 2 * type_bytes(type);
-    const bool pairs = !((xt | xb | yt | yb | dt | db | width) & 1) && aligned(x, pair) &&
-                       aligned(dy, pair) && aligned(dx, pair);
+    const bool pairs = !((xt | xb | yt | yb | width) & 1) && aligned(x, pair) && aligned(dy, pair);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        return with_group(pairs, [&](auto group) {
-            constexpr int V = decltype(group)::value;
-            if (a.segments > 1) {
-                const int parts = launch_recurrence(
-                    "recurrence gradient parts", tanh ? k_recurrence_parts<T, V, true, true>
-                                                      : k_recurrence_parts<T, V, false, true>,
-                    a, batch, V, MOST_WAVES, s);
-                if (parts) return parts;
-            }
-            return launch_recurrence("recurrence gradient",
-                                     tanh ? k_recurrence_grad<T, V, true> : k_recurrence_grad<T, V, false>,
-                                     a, batch, V, waves_of(steps), s);
-        });
+        if (a.segments > 1) {
+            const int parts = with_group(pairs, [&](auto group) {
+                constexpr int V = decltype(group)::value;
+                return launch_recurrence("recurrence gradient parts", k_recurrence_parts<T, V, false, true>,
+                                         a, batch, V, MOST_WAVES, s);
+            });
+            if (parts) return parts;
+        }
+        if (steps > SPAN)
+            return launch_recurrence("recurrence gradient", tanh ? k_recurrence_grad<T, true, 8, 16>
+                                                                 : k_recurrence_grad<T, false, 8, 16>,
+                                     a, batch, 1, 8, s);
+        return launch_recurrence("recurrence gradient", tanh ? k_recurrence_grad<T, true, 16, 8>
+                                                             : k_recurrence_grad<T, false, 16, 8>,
+                                 a, batch, 1, int((steps + 7) / 8), s);
     });
 }
 
