@@ -660,7 +660,7 @@ int mf_dropout(const void *x, int32_t type, int64_t n, const void *residual, uin
  * G = ceil(k / group), codes are [ceil(o / 16), P, 1024] bytes: input i of a span of 128 and output r of a
  * tile of 16 are in byte (i / 8 % 4) * 256 + r * 16 + i / 32 * 4 + i % 4, in its lower half if i % 8 < 4.
  * Scales (FP32, or x's type) and zero points are [ceil(o / 16), G, 16].  Codes are 16-byte aligned.
- * o < 2^27, k < 2^24.
+ * o < 2^25, k < 2^24.
  *
  * mf_int4_quantize: codes and scales of w [o, k] (rows ldw apart), zero points 8: scale = max|w| / 7 in the
  * scales' type (FP32 or w's), codes to nearest even; a group with a NaN or an infinity has scale NaN. */
@@ -669,10 +669,14 @@ int mf_int4_quantize(const void *w, int32_t type, int64_t o, int64_t k, int64_t 
 int mf_int4_dequantize(const uint8_t *codes, const void *scales, int32_t scale_type, const uint8_t *zeros,
                        int64_t o, int64_t k, int64_t group, void *out, int32_t type, void *stream);
 /* out [n, o] = x W^T + bias (o values of x's type, or NULL) for x [n, k] (rows ldx apart): products of
- * codes and x are summed in FP32 by group and scaled then. */
+ * codes and x are summed in FP32 by group and scaled then.  n < 2^27.  The workspace
+ * (mf_int4_linear_workspace bytes, which may be 0; 16-byte aligned) belongs to the one call; `pieces`: x is
+ * 16-byte aligned and its rows are whole multiples of 16 bytes apart. */
+int mf_int4_linear_workspace(int32_t type, int64_t n, int64_t k, int64_t group, int32_t pieces,
+                             int64_t *bytes);
 int mf_int4_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, const uint8_t *codes,
                    const void *scales, int32_t scale_type, const uint8_t *zeros, int64_t o, int64_t group,
-                   const void *bias, void *out, void *stream);
+                   const void *bias, void *out, void *workspace, int64_t bytes, void *stream);
 
 #ifdef __cplusplus
 }

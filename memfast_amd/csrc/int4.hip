@@ -11,7 +11,7 @@
 #include <cfloat>
 #include <type_traits>
 
-#include "mf_float.h"
+#include "mf_mx.h"
 
 namespace mf {
 
@@ -30,7 +30,6 @@ struct HeldArgs {
     int shift;              // log2(group)
     const void *bias;       // [o] or nullptr
     void *out;              // [n, o]
-    bool vec;               // rows of x are whole 16-byte pieces
 };
 
 // The operand types of the matrix instructions: F16 for FP16 inputs, BF16 for the others.
@@ -78,19 +77,15 @@ template <> struct Operand<f16> {
 // x's values in the upper halves of FP32 numbers: what is left of them is exact.
 __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// Eight values of a row from k on, zeros past the row's end.
+// Eight consecutive values of a row, at a 16-byte address.
 template <typename T> struct alignas(16) Eight {
     T v[8];
-    __device__ __forceinline__ void load(const T *row, i64 k, i64 end, bool vec) {
-        if (vec && k + 8 <= end) {
+    __device__ __forceinline__ void load(const T *at) {
 #pragma unroll
-            for (int i = 0; i < 8; i += PIECE<T>)
-                *reinterpret_cast<Piece<T> *>(v + i) = *reinterpret_cast<const Piece<T> *>(row + k + i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = k + i < end ? row[k + i] : T(0.0f);
-        }
+        for (int i = 0; i < 8; i += PIECE<T>)
+            *reinterpret_cast<Piece<T> *>(v + i) = *reinterpret_cast<const Piece<T> *>(at + i);
     }
+    // The terms that add up to them.
     template <int TERMS, typename V> __device__ __forceinline__ void split(V (&t)[TERMS]) const {
         if constexpr (TERMS == 1) {
             t[0] = *reinterpret_cast<const V *>(v);
@@ -110,115 +105,136 @@ template <typename T> struct alignas(16) Eight {
 };
 
 // The four values that the quarters of a wave hold, each in all of them.
-__device__ __forceinline__ void quarters(u32 v, u32 (&all)[4]) {
+__device__ __forceinline__ void quarters(float value, float (&all)[4]) {
+    const u32 v = __float_as_uint(value);
     const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     const auto low = __builtin_amdgcn_permlane16_swap(halves[0], halves[0], false, false);
     const auto high = __builtin_amdgcn_permlane16_swap(halves[1], halves[1], false, false);
-    all[0] = low[0], all[1] = low[1], all[2] = high[0], all[3] = high[1];
+    all[0] = __uint_as_float(low[0]), all[1] = __uint_as_float(low[1]);
+    all[2] = __uint_as_float(high[0]), all[3] = __uint_as_float(high[1]);
 }
 
 // ---- few rows --------------------------------------------------------------
 // A workgroup takes OT tiles of outputs and all rows, its waves split the spans and add their sums in LDS in
 // the order of the waves.  Row 4 i + quarter of a block of 16 rows is row 4 quarter + i of the matrix
-// instruction, so that up to 4 rows need one register of its result and one scaling.
-constexpr int FEW_WAVES = 8;
-
-template <typename T, typename S, int OT, int NB, int R>
-__global__ __launch_bounds__(64 * FEW_WAVES) void k_int4_few(const HeldArgs a) {
+// instruction, so that up to 4 rows need one register of its result and one scaling.  x is a multiple of
+// 8 inputs wide, in whole 16-byte pieces.  PER: scalings in a span, 1 for groups of 128 on, else 4.
+template <typename T, typename S, int WAVES, int OT, int NB, int R, int PER, bool AHEAD>
+__global__ __launch_bounds__(64 * WAVES) void k_int4_few(const HeldArgs a) {
     typedef Operand<T> Op;
     constexpr int TERMS = Op::TERMS;
-    extern __shared__ __align__(16) float sums[];   // [FEW_WAVES][OT * NB * R][64]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4, r = lane & 15;
+    extern __shared__ __align__(16) float sums[];   // [WAVES][OT * NB * R][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = lane >> 4, r = lane & 15;
+    const int spans = int(a.spans), groups = int(a.groups), k = int(a.k);
     const i64 tiles = (a.o + TILE - 1) / TILE, tile0 = i64(blockIdx.x) * OT;
-    const T *rows[NB];
+    const T *rows[NB];      // at this lane's eight inputs of the wave's next span
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const i64 n = min(i64(16 * b + (r & 3) * 4 + (r >> 2)), a.n - 1);
-        rows[b] = static_cast<const T *>(a.x) + n * a.ldx;
+        rows[b] = static_cast<const T *>(a.x) + n * a.ldx + wave * SPAN_K + 8 * quarter;
     }
-    const u8 *codes[OT];
-    const S *scales[OT];
-    const u8 *zeros[OT];
+
+    v4u next[OT];
+    S next_s[OT];
+    u8 next_z[OT];
+    Eight<T> next_x[NB][4];
+    const auto fetch_x = [&](int span) {
+        if ((span + 1) * SPAN_K <= k) {
 #pragma unroll
-    for (int t = 0; t < OT; ++t) {
-        const i64 tile = min(tile0 + t, tiles - 1);
-        codes[t] = a.codes + tile * a.spans * SPAN_BYTES + lane * 16;
-        scales[t] = static_cast<const S *>(a.scales) + tile * a.groups * 16 + r;
-        zeros[t] = a.zeros ? a.zeros + tile * a.groups * 16 + r : nullptr;
-    }
-    // Groups in a span: 4, 2 or 1; a quarter reads one of them.
-    const int per = a.shift >= 7 ? 1 : 128 >> a.shift, group_steps = 4 / per;
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) next_x[b][j].load(rows[b] + 32 * j);
+        } else {            // the last span of a row that ends within it: zeros past the end
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool in = span * SPAN_K + 32 * j + 8 * quarter < k;
+                    next_x[b][j].load(in ? rows[b] + 32 * j : rows[b] - span * SPAN_K - 8 * quarter);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) next_x[b][j].v[i] = in ? next_x[b][j].v[i] : T(0.0f);
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) rows[b] += WAVES * SPAN_K;
+    };
+    const auto fetch = [&](int span) {
+        // A quarter reads the scale of the 32 inputs that are its number.
+        const u32 g = PER == 1 ? (span * SPAN_K) >> a.shift
+                               : min((span * SPAN_K + 32 * quarter) >> a.shift, groups - 1);
+#pragma unroll
+        for (int t = 0; t < OT; ++t) {
+            const i64 tile = min(tile0 + t, tiles - 1);
+            const u8 *at = a.codes + (tile * spans + span) * SPAN_BYTES;
+            next[t] = *reinterpret_cast<const v4u *>(at + u32(lane * 16));
+            next_s[t] = (static_cast<const S *>(a.scales) + tile * groups * 16)[g * 16 + r];
+            next_z[t] = u8(8);
+            if (a.zeros) next_z[t] = (a.zeros + tile * groups * 16)[g * 16 + r];
+        }
+        if (AHEAD) fetch_x(span);
+    };
 
     v4f total[OT][NB];
 #pragma unroll
     for (int t = 0; t < OT; ++t)
 #pragma unroll
         for (int b = 0; b < NB; ++b) total[t][b] = v4f{0, 0, 0, 0};
-
-    v4u w[OT], next[OT];
-    S s[OT], next_s[OT];
-    u8 z[OT], next_z[OT];
-    const auto fetch = [&](i64 span, v4u (&w)[OT], S (&s)[OT], u8 (&z)[OT]) {
-        const i64 g = min((span * SPAN_K >> a.shift) + (quarter & (per - 1)), a.groups - 1) * 16;
+    if (wave < spans) fetch(wave);
+    for (int span = wave; span < spans; span += WAVES) {
+        v4u w[OT];
+        Eight<T> x[NB][4];
+        float scale[OT][PER], zero[OT][PER];
+        if (!AHEAD) fetch_x(span);
 #pragma unroll
         for (int t = 0; t < OT; ++t) {
-            w[t] = *reinterpret_cast<const v4u *>(codes[t] + span * SPAN_BYTES);
-            s[t] = scales[t][g];
-            z[t] = zeros[t] ? zeros[t][g] : u8(8);
+            w[t] = next[t];
+            const float s = float(next_s[t]), z = -float(next_z[t]);
+            if constexpr (PER == 1) {
+                scale[t][0] = s, zero[t][0] = z;
+            } else {
+                quarters(s, scale[t]);
+                quarters(z, zero[t]);
+            }
         }
-    };
-    if (wave < a.spans) fetch(wave, next, next_s, next_z);
-    for (i64 span = wave; span < a.spans; span += FEW_WAVES) {
 #pragma unroll
-        for (int t = 0; t < OT; ++t) w[t] = next[t], s[t] = next_s[t], z[t] = next_z[t];
-        if (span + FEW_WAVES < a.spans) fetch(span + FEW_WAVES, next, next_s, next_z);
-        u32 scale[OT][4], zero[OT][4];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int t = 0; t < OT; ++t) {
-            quarters(__float_as_uint(float(s[t])), scale[t]);
-            quarters(__float_as_uint(float(z[t])), zero[t]);
-        }
+            for (int j = 0; j < 4; ++j) x[b][j] = next_x[b][j];
+        if (span + WAVES < spans) fetch(span + WAVES);
         v4f acc[OT][NB], sum[NB];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            typename Op::V x[NB][TERMS], q[OT];
-            const i64 k = span * SPAN_K + 32 * j + 8 * quarter;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                Eight<T> v;
-                v.load(rows[b], k, a.k, a.vec);
-                v.template split<TERMS>(x[b]);
-            }
+            typename Op::V q[OT];
+            constexpr int STEPS = 4 / PER;
 #pragma unroll
             for (int t = 0; t < OT; ++t) q[t] = Op::codes(w[t][j]);
-            const bool begins = j % group_steps == 0, ends = (j + 1) % group_steps == 0;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                sum[b] = begins ? v4f{0, 0, 0, 0} : sum[b];
+                typename Op::V xs[TERMS];
+                x[b][j].template split<TERMS>(xs);
+                if (j % STEPS == 0) {
+                    sum[b] = v4f{0, 0, 0, 0};
 #pragma unroll
-                for (int m = 0; m < TERMS; ++m) sum[b] = Op::mfma(x[b][m], Op::ones(), sum[b]);
+                    for (int t = 0; t < OT; ++t) acc[t][b] = v4f{0, 0, 0, 0};
+                }
 #pragma unroll
-                for (int t = 0; t < OT; ++t) {
-                    acc[t][b] = begins ? v4f{0, 0, 0, 0} : acc[t][b];
+                for (int m = 0; m < TERMS; ++m) {
+                    sum[b] = Op::mfma(xs[m], Op::ones(), sum[b]);
 #pragma unroll
-                    for (int m = 0; m < TERMS; ++m) acc[t][b] = Op::mfma(x[b][m], q[t], acc[t][b]);
+                    for (int t = 0; t < OT; ++t) acc[t][b] = Op::mfma(xs[m], q[t], acc[t][b]);
                 }
             }
-            if (ends) {
-                const int g = j / group_steps;
+            if ((j + 1) % STEPS == 0)
 #pragma unroll
-                for (int t = 0; t < OT; ++t) {
-                    const float sc = __uint_as_float(g == 0 ? scale[t][0] : g == 1 ? scale[t][1]
-                                                     : g == 2 ? scale[t][2] : scale[t][3]);
-                    const float ze = __uint_as_float(g == 0 ? zero[t][0] : g == 1 ? zero[t][1]
-                                                     : g == 2 ? zero[t][2] : zero[t][3]);
+                for (int t = 0; t < OT; ++t)
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int i = 0; i < R; ++i)
-                            total[t][b][i] = fmaf(sc, fmaf(-ze, sum[b][i], acc[t][b][i]), total[t][b][i]);
-                }
-            }
+                            total[t][b][i] = fmaf(scale[t][j / STEPS],
+                                                  fmaf(zero[t][j / STEPS], sum[b][i], acc[t][b][i]),
+                                                  total[t][b][i]);
         }
     }
     constexpr int VALUES = OT * NB * R;
@@ -230,16 +246,240 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_int4_few(const HeldArgs a) {
             for (int i = 0; i < R; ++i)
                 sums[(wave * VALUES + (t * NB + b) * R + i) * 64 + lane] = total[t][b][i];
     __syncthreads();
-    for (int v = wave; v < VALUES; v += FEW_WAVES) {
+    for (int v = wave; v < VALUES; v += WAVES) {
         const int t = v / (NB * R), b = v / R % NB, i = v % R;
         const i64 n = 16 * b + 4 * i + quarter, o = (tile0 + t) * TILE + r;
         float y = 0.0f;
 #pragma unroll
-        for (int u = 0; u < FEW_WAVES; ++u) y += sums[(u * VALUES + v) * 64 + lane];
+        for (int u = 0; u < WAVES; ++u) y += sums[(u * VALUES + v) * 64 + lane];
         if (n < a.n && o < a.o) {
             if (a.bias) y += float(static_cast<const T *>(a.bias)[o]);
             static_cast<T *>(a.out)[n * a.o + o] = rounded<T>(y);
         }
+    }
+}
+
+// Copies rows of x into rows of whole spans, with zeros past k: one wave a span, two inputs a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void k_int4_pad(const T *x, i64 n, i64 k, i64 ldx, i64 spans, T *out) {
+    const int lane = threadIdx.x & 63;
+    for (i64 id = i64(blockIdx.x) * 4 + (threadIdx.x >> 6); id < n * spans; id += i64(gridDim.x) * 4) {
+        const i64 row = id / spans, span = id - row * spans;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const i64 at = span * SPAN_K + lane * 2 + i;
+            out[row * spans * SPAN_K + at] = at < k ? x[row * ldx + at] : T(0.0f);
+        }
+    }
+}
+
+// ---- many rows -------------------------------------------------------------
+// Rows of x as the tile kernel copies them, and their sums: [blocks, pitch] of `factor` times the sum of each
+// row over a block of 32 inputs (`per` 4 to a span) or 128 (1), 0 past the rows.
+struct PrepareArgs {
+    const void *x;
+    i64 n, k, ldx, spans, pitch;
+    int per;
+    float factor;
+    float *sums;
+    u16 *planes;        // [TERMS, n, 128 spans], or nullptr: x is taken as it is
+};
+
+// One wave takes a span of a row, two inputs a lane.
+template <typename T> __global__ __launch_bounds__(256) void k_int4_prepare(const PrepareArgs a) {
+    typedef typename std::conditional<std::is_same<T, float>::value, bf16, T>::type Term;
+    constexpr int TERMS = Operand<T>::TERMS;
+    const int lane = threadIdx.x & 63;
+    const i64 all = a.pitch * a.spans;
+    for (i64 id = i64(blockIdx.x) * 4 + (threadIdx.x >> 6); id < all; id += i64(gridDim.x) * 4) {
+        const i64 n = id / a.spans, span = id - n * a.spans;
+        float sum = 0.0f;
+        if (n < a.n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const i64 k = span * SPAN_K + lane * 2 + i;
+                const T x = k < a.k ? static_cast<const T *>(a.x)[n * a.ldx + k] : T(0.0f);
+                sum += float(x);
+                if (a.planes) {
+                    float rest = float(x);
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const float high = TERMS == 1 ? rest : upper(rest);
+                        const Term term = Term(high);
+                        a.planes[(t * a.n + n) * a.spans * SPAN_K + k] = __builtin_bit_cast(u16, term);
+                        rest -= high;
+                    }
+                }
+            }
+#pragma unroll
+        for (int d = 1; d <= 8; d <<= 1) sum += __shfl_xor(sum, d);
+        if (a.per == 1) {
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (lane == 0) a.sums[span * a.pitch + n] = a.factor * sum;
+        } else if ((lane & 15) == 0) {
+            a.sums[(span * 4 + lane / 16) * a.pitch + n] = a.factor * sum;
+        }
+    }
+}
+
+struct TileArgs {
+    HeldArgs h;             // h.x: rows of 16-bit operands, h.ldx apart, of whole spans
+    i64 plane;              // distance of x's terms, in values
+    const float *sums;
+    i64 pitch;
+};
+
+template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v16f c) {
+    if constexpr (std::is_same<T, f16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b),
+                                                      c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a),
+                                                       __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+
+// A workgroup of four waves takes 32 NT rows and 256 outputs, a wave 64 of them: its codes go from memory to
+// registers, where they become operands once for all rows; x comes through LDS, copied by DMA a span ahead.
+// Sums over a group begin at -8 times the sum of x (the sums' table), so a zero point of 8 costs nothing;
+// others (ZEROS) are taken off with one operation more a group and result.  PER: scalings in a span, 1 for
+// groups of 128 on, else 4.
+constexpr int TILE_WAVES = 4, TILE_OUTPUTS = 64 * TILE_WAVES;
+
+template <typename T, typename S, int NT, bool ZEROS, int PER>
+__global__ __launch_bounds__(64 * TILE_WAVES) void k_int4_tile(const TileArgs t) {
+    typedef Operand<T> Op;
+    constexpr int TERMS = Op::TERMS, ROWS = 32 * NT;
+    constexpr int XBYTES = TERMS * ROWS * SPAN_K * 2, STAGE = XBYTES + 2048;
+    extern __shared__ __align__(16) u8 staged[];
+    const HeldArgs &a = t.h;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = lane >> 5, row = lane & 31, r = lane & 15;
+    const u32 tn = u32((a.n + ROWS - 1) / ROWS), to = u32((a.o + TILE_OUTPUTS - 1) / TILE_OUTPUTS);
+    u32 nx, oy;
+    xcd_tile(blockIdx.x, tn, to, nx, oy);
+    const i64 n0 = i64(nx) * ROWS, o0 = i64(oy) * TILE_OUTPUTS + wave * 64;
+    const i64 tiles = (a.o + TILE - 1) / TILE;
+
+    // Copies: 1 KiB each, four rows of x (row q's 16-byte pieces p at p ^ (q & 15)) or two rows of sums.
+    constexpr int COPIES = XBYTES / 1024 / TILE_WAVES;
+    const char *source[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+        const int q = (wave * COPIES + i) * 4 + (lane >> 4);        // a row of a term
+        const i64 n = min(n0 + q % ROWS, a.n - 1);
+        source[i] = static_cast<const char *>(a.x) +
+                    (i64(q / ROWS) * t.plane + n * a.ldx + (((lane & 15) ^ (q & 15)) * 8)) * 2;
+    }
+    const float *sums = t.sums + n0 + (lane & 31) * 4;
+    const u32 lds = lds_address(staged);
+    const auto copy = [&](i64 span, int buffer) {
+        const u32 to = lds + buffer * STAGE;
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i)
+            lds_dma_16(source[i] + span * (SPAN_K * 2),
+                       __builtin_amdgcn_readfirstlane(to + (wave * COPIES + i) * 1024));
+        if (wave < (PER + 1) / 2)
+            lds_dma_16(sums + (span * PER + min(wave * 2 + half, PER - 1)) * t.pitch,
+                       __builtin_amdgcn_readfirstlane(to + XBYTES + wave * 1024));
+    };
+
+    // A lane's output is 32 j + row of the wave's; it reads both 16-byte pieces of its half.
+    const u8 *codes[2];
+    const S *scales[2];
+    const u8 *zeros[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const i64 tile = min((o0 + 32 * j + row) / TILE, tiles - 1);
+        codes[j] = a.codes + tile * a.spans * SPAN_BYTES + half * 256 + r * 16;
+        scales[j] = static_cast<const S *>(a.scales) + tile * a.groups * 16 + r;
+        zeros[j] = ZEROS ? a.zeros + tile * a.groups * 16 + r : nullptr;
+    }
+    v4u w[2][2];
+    S s[2][PER];
+    u8 z[2][PER];
+    const auto fetch = [&](i64 span) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+                w[j][m] = *reinterpret_cast<const v4u *>(codes[j] + span * SPAN_BYTES + m * 512);
+#pragma unroll
+            for (int g = 0; g < PER; ++g) {
+                const i64 at = min((span * SPAN_K + g * 32) >> a.shift, a.groups - 1) * 16;
+                s[j][g] = scales[j][at];
+                z[j][g] = ZEROS ? zeros[j][at] : u8(8);
+            }
+        }
+    };
+
+    v16f total[NT][2] = {};
+    fetch(0);
+    copy(0, 0);
+    for (i64 span = 0; span < a.spans; ++span) {
+        wait_stage<0>();
+        if (span + 1 < a.spans) copy(span + 1, int(span + 1) & 1);
+        const u8 *stage = staged + (span & 1) * STAGE;
+        v4u q[2][8];        // operands of 16 inputs each
+        float scale[2][PER], zero[2][PER];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+                q[j][b] = __builtin_bit_cast(v4u, Op::codes(w[j][b & 1][b >> 1]));
+#pragma unroll
+            for (int g = 0; g < PER; ++g) scale[j][g] = float(s[j][g]), zero[j][g] = -float(z[j][g]);
+        }
+        if (span + 1 < a.spans) fetch(span + 1);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const u8 *x = stage + (32 * i + row) * (SPAN_K * 2);
+            v16f acc[2], sum;
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                constexpr int STEPS = 8 / PER;
+                if (b % STEPS == 0) {
+                    const float *from = reinterpret_cast<const float *>(stage + XBYTES) +
+                                        b / STEPS * 128 + 32 * i + 4 * half;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const v4f four = *reinterpret_cast<const v4f *>(from + 8 * e);
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) sum[4 * e + f] = four[f];
+                    }
+                    acc[0] = acc[1] = ZEROS ? v16f{} : sum;
+                }
+#pragma unroll
+                for (int m = 0; m < TERMS; ++m) {
+                    const v4u xf = *reinterpret_cast<const v4u *>(
+                        x + m * (ROWS * SPAN_K * 2) + ((2 * b + half) ^ r) * 16);
+                    acc[0] = mfma_wide<T>(xf, q[0][b], acc[0]);
+                    acc[1] = mfma_wide<T>(xf, q[1][b], acc[1]);
+                }
+                if ((b + 1) % STEPS == 0)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float v = ZEROS ? fmaf(zero[j][b / STEPS], sum[e], acc[j][e]) : acc[j][e];
+                            total[i][j][e] = fmaf(scale[j][b / STEPS], v, total[i][j][e]);
+                        }
+            }
+        }
+    }
+    T *out = static_cast<T *>(a.out);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const i64 o = o0 + 32 * j + row;
+        if (o >= a.o) continue;
+        const float bias = a.bias ? float(static_cast<const T *>(a.bias)[o]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const i64 n = n0 + 32 * i + 8 * (e / 4) + 4 * half + (e & 3);
+                if (n < a.n) out[n * a.o + o] = rounded<T>(total[i][j][e] + bias);
+            }
     }
 }
 
@@ -323,7 +563,7 @@ int group_shift(i64 group) {
     return -1;
 }
 
-constexpr i64 MOST_OUTPUTS = i64(1) << 27, MOST_INPUTS = i64(1) << 24;
+constexpr i64 MOST_OUTPUTS = i64(1) << 25, MOST_INPUTS = i64(1) << 24, MOST_ROWS = i64(1) << 27;
 
 int check_held(const void *codes, const void *scales, int32_t scale_type, const void *zeros, i64 o, i64 k,
                i64 group, HeldArgs &a) {
@@ -343,33 +583,113 @@ int check_held(const void *codes, const void *scales, int32_t scale_type, const 
     return MF_OK;
 }
 
-template <typename T, typename S, int OT, int NB, int R> int launch_few(const HeldArgs &a, hipStream_t s) {
+#ifndef FW
+#define FW 8
+#define FO 1
+#define FA true
+#endif
+template <typename T, typename S, int NB, int R> int launch_few(const HeldArgs &a, hipStream_t s) {
+    constexpr int WAVES = FW, OT = FO;
     const i64 tiles = (a.o + TILE - 1) / TILE;
-    const int lds = FEW_WAVES * OT * NB * R * 64 * int(sizeof(float));
-    const auto kernel = k_int4_few<T, S, OT, NB, R>;
+    const int lds = WAVES * OT * NB * R * 64 * int(sizeof(float));
+    const auto kernel = a.shift >= 7 ? k_int4_few<T, S, WAVES, OT, NB, R, 1, FA>
+                                     : k_int4_few<T, S, WAVES, OT, NB, R, 4, FA>;
     const int status = allow_lds(kernel, lds);
     if (status) return status;
-    hipLaunchKernelGGL(kernel, dim3(u32((tiles + OT - 1) / OT)), dim3(64 * FEW_WAVES), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3(u32((tiles + OT - 1) / OT)), dim3(64 * WAVES), lds, s, a);
     return check_launch("4-bit product");
 }
 
-template <typename T, typename S> int launch_held(HeldArgs a, hipStream_t s) {
-    // Blocks of up to 64 rows one after the other.
+// Few rows go to k_int4_few.
+constexpr i64 FEW_ROWS = 64, ROWS_AT_ONCE = 8192;
+
+// The kernel, how many rows go through tiles at a time, and what the workspace holds for them.
+struct HeldPlan {
+    bool few, direct;       // direct: x is read as it is
+    int per, terms;
+    i64 rows, pitch, spans, sums, bytes;
+    HeldPlan(int32_t type, i64 n, i64 k, i64 group, bool pieces) {
+        spans = (k + SPAN_K - 1) / SPAN_K;
+        few = n <= FEW_ROWS;
+        direct = few ? pieces && k % 8 == 0 : pieces && type != MF_F32 && k % SPAN_K == 0;
+        per = group >= SPAN_K ? 1 : 4;
+        terms = type == MF_F32 ? 3 : 1;
+        rows = std::min(n, ROWS_AT_ONCE);
+        pitch = (rows + 127) / 128 * 128 + 128;
+        sums = few ? 0 : spans * per * pitch * i64(sizeof(float));
+        bytes = sums + (direct ? 0 : rows * spans * SPAN_K * (few ? type_bytes(type) : 2 * terms));
+    }
+};
+
+bool rows_in_pieces(const void *x, i64 ldx, int32_t type) {
+    return aligned(x, 16) && ldx * type_bytes(type) % 16 == 0;
+}
+
+template <typename T, typename S, int NT, bool ZEROS, int PER>
+int launch_tile(const TileArgs &t, hipStream_t s) {
+    constexpr int ROWS = 32 * NT, LDS = 2 * (Operand<T>::TERMS * ROWS * SPAN_K * 2 + 2048);
+    const auto kernel = k_int4_tile<T, S, NT, ZEROS, PER>;
+    const int status = allow_lds(kernel, LDS);
+    if (status) return status;
+    const i64 tiles = (t.h.n + ROWS - 1) / ROWS * ((t.h.o + TILE_OUTPUTS - 1) / TILE_OUTPUTS);
+    hipLaunchKernelGGL(kernel, dim3(u32(tiles)), dim3(64 * TILE_WAVES), LDS, s, t);
+    return check_launch("4-bit product");
+}
+
+#ifndef NT16
+#define NT16 4
+#endif
+template <typename T, typename S> int launch_tiles(HeldArgs a, const HeldPlan &plan, void *workspace, hipStream_t s) {
+    constexpr int NT = Operand<T>::TERMS == 1 ? NT16 : 2;
     const char *x = static_cast<const char *>(a.x);
     char *out = static_cast<char *>(a.out);
-    for (i64 first = 0, n = a.n; first < n; first += 64) {
-        a.x = x + first * a.ldx * i64(sizeof(T));
+    const i64 n = a.n;
+    for (i64 first = 0; first < n; first += plan.rows) {
+        a.n = std::min(plan.rows, n - first);
         a.out = out + first * a.o * i64(sizeof(T));
-        a.n = std::min<i64>(64, n - first);
-        const int status = a.n <= 4    ? launch_few<T, S, 2, 1, 1>(a, s)
-                           : a.n <= 8  ? launch_few<T, S, 2, 1, 2>(a, s)
-                           : a.n <= 16 ? launch_few<T, S, 2, 1, 4>(a, s)
-                           : a.n <= 32 ? launch_few<T, S, 2, 2, 4>(a, s)
-                           : a.n <= 48 ? launch_few<T, S, 2, 3, 4>(a, s)
-                                       : launch_few<T, S, 2, 4, 4>(a, s);
+        const void *rows = x + first * a.ldx * i64(sizeof(T));
+        PrepareArgs p{rows, a.n, a.k, a.ldx, a.spans, plan.pitch, plan.per, a.zeros ? 1.0f : -8.0f,
+                      static_cast<float *>(workspace), nullptr};
+        TileArgs t{a, 0, p.sums, plan.pitch};
+        t.h.x = rows;
+        if (!plan.direct) {
+            p.planes = reinterpret_cast<u16 *>(static_cast<char *>(workspace) + plan.sums);
+            t.h.x = p.planes;
+            t.h.ldx = a.spans * SPAN_K;
+            t.plane = a.n * t.h.ldx;
+        }
+        hipLaunchKernelGGL(k_int4_prepare<T>, dim3(u32(std::min<i64>((p.pitch * p.spans + 3) / 4, 1 << 16))),
+                           dim3(256), 0, s, p);
+        int status = check_launch("4-bit product's rows");
+        if (status) return status;
+        if (plan.per == 1)
+            status = a.zeros ? launch_tile<T, S, NT, true, 1>(t, s) : launch_tile<T, S, NT, false, 1>(t, s);
+        else
+            status = a.zeros ? launch_tile<T, S, NT, true, 4>(t, s) : launch_tile<T, S, NT, false, 4>(t, s);
         if (status) return status;
     }
     return MF_OK;
+}
+
+template <typename T, typename S> int launch_held(HeldArgs a, const HeldPlan &plan, void *workspace,
+                                                  hipStream_t s) {
+    if (!plan.few) return launch_tiles<T, S>(a, plan, workspace, s);
+    if (!plan.direct) {
+        T *rows = static_cast<T *>(workspace);
+        hipLaunchKernelGGL(k_int4_pad<T>, dim3(u32((a.n * a.spans + 3) / 4)), dim3(256), 0, s,
+                           static_cast<const T *>(a.x), a.n, a.k, a.ldx, a.spans, rows);
+        const int status = check_launch("4-bit product's rows");
+        if (status) return status;
+        a.x = rows;
+        a.ldx = a.spans * SPAN_K;
+        a.k = a.ldx;        // zeros included: the codes past the weight's inputs are there too
+    }
+    return a.n <= 4    ? launch_few<T, S, 1, 1>(a, s)
+           : a.n <= 8  ? launch_few<T, S, 1, 2>(a, s)
+           : a.n <= 16 ? launch_few<T, S, 1, 4>(a, s)
+           : a.n <= 32 ? launch_few<T, S, 2, 4>(a, s)
+           : a.n <= 48 ? launch_few<T, S, 3, 4>(a, s)
+                       : launch_few<T, S, 4, 4>(a, s);
 }
 
 // Calls f(T{}, S{}) for the types of x and of the scales: x's own or FP32.
@@ -424,23 +744,34 @@ int mf_int4_dequantize(const uint8_t *codes, const void *scales, int32_t scale_t
     });
 }
 
+int mf_int4_linear_workspace(int32_t type, int64_t n, int64_t k, int64_t group, int32_t pieces,
+                             int64_t *bytes) {
+    if (!known_type(type) || n < 1 || k < 1 || n >= MOST_ROWS || k >= MOST_INPUTS || group_shift(group) < 0 ||
+        !bytes)
+        return fail(MF_E_INVALID, "invalid 4-bit product sizes");
+    *bytes = HeldPlan(type, n, k, group, pieces != 0).bytes;
+    return MF_OK;
+}
+
 int mf_int4_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, const uint8_t *codes,
                    const void *scales, int32_t scale_type, const uint8_t *zeros, int64_t o, int64_t group,
-                   const void *bias, void *out, void *stream) {
+                   const void *bias, void *out, void *workspace, int64_t bytes, void *stream) {
     HeldArgs a{};
     const int status = check_held(codes, scales, scale_type, zeros, o, k, group, a);
     if (status) return status;
-    if (!x || !known_type(type) || n < 1 || ldx < k || !out) 
+    if (!x || !known_type(type) || n < 1 || ldx < 0 || (n > 1 && ldx < k) || !out)
         return fail(MF_E_INVALID, "invalid 4-bit product arguments");
     const uintptr_t one = type_bytes(type);
     if (!aligned(x, one) || !aligned(bias, one) || !aligned(out, one))
         return fail(MF_E_INVALID, "4-bit product's operands are not aligned to their types");
-    if (n >= MOST_OUTPUTS)
+    if (n >= MOST_ROWS)
         return fail(MF_E_UNSUPPORTED, "4-bit product of %lld rows", (long long)n);
     a.x = x, a.n = n, a.ldx = ldx, a.bias = bias, a.out = out;
-    a.vec = aligned(x, 16) && ldx * i64(one) % 16 == 0;
+    const HeldPlan plan(type, n, k, group, rows_in_pieces(x, ldx, type));
+    if (bytes < plan.bytes || (plan.bytes && (!workspace || !aligned(workspace, 16))))
+        return fail(MF_E_INVALID, "4-bit product's workspace of %lld bytes", (long long)bytes);
     return with_types(type, scale_type, [&](auto t, auto scale) {
-        return launch_held<decltype(t), decltype(scale)>(a, static_cast<hipStream_t>(stream));
+        return launch_held<decltype(t), decltype(scale)>(a, plan, workspace, static_cast<hipStream_t>(stream));
     });
 }
 

@@ -223,7 +223,8 @@ SIGNATURES = {
     "mf_dropout": ([_P, _I32, _I64, _P, ct.c_uint32, ct.c_uint64, ct.c_uint64, _P, _P, _P], ct.c_int),
     "mf_int4_quantize": ([_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _P], ct.c_int),
     "mf_int4_dequantize": ([_P, _P, _I32, _P, _I64, _I64, _I64, _P, _I32, _P], ct.c_int),
-    "mf_int4_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _I64, _I64, _P, _P, _P],
+    "mf_int4_linear_workspace": ([_I32, _I64, _I64, _I64, _I32, ct.POINTER(_I64)], ct.c_int),
+    "mf_int4_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _I64, _I64, _P, _P, _P, _I64, _P],
                        ct.c_int),
     "mf_rng_uniform": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
     "mf_rng_normal": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
@@ -1726,15 +1727,26 @@ def int4_dequantize(codes, scales, zeros, o, k, group, dtype):
     return out
 
 
+@lru_cache(maxsize=4096)
+def _int4_workspace(kind, n, k, group, pieces):
+    size = _I64()
+    check(library().mf_int4_linear_workspace(kind, n, k, group, pieces, ct.byref(size)), "4-bit product")
+    return size.value
+
+
 def int4_linear(x, codes, scales, zeros, o, group, bias):
     """``x W^T + bias`` [n, o] for ``x`` [n, k] and a held W (mf_int4_linear)."""
     n, k = x.shape
-    out = torch.empty((n, o), dtype=x.dtype, device=x.device)
-    with _on(x.device):
+    kind, at, ldx, device = FLOAT_TYPES[x.dtype], x.data_ptr(), x.stride(0), x.device
+    pieces = at % 16 == 0 and ldx * x.element_size() % 16 == 0
+    size = _int4_workspace(kind, n, k, group, pieces)
+    out = torch.empty((n, o), dtype=x.dtype, device=device)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    with _on(device):
         check(library().mf_int4_linear(
-            x.data_ptr(), FLOAT_TYPES[x.dtype], n, k, x.stride(0), codes.data_ptr(),
-            scales.data_ptr(), FLOAT_TYPES[scales.dtype], _ptr(zeros), o, group, _ptr(bias),
-            out.data_ptr(), _stream(x.device)), "4-bit product")
+            at, kind, n, k, ldx, codes.data_ptr(), scales.data_ptr(), FLOAT_TYPES[scales.dtype],
+            _ptr(zeros), o, group, _ptr(bias), out.data_ptr(), _ptr(work), size, _stream(device)),
+            "4-bit product")
     return out
 
 

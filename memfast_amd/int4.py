@@ -15,7 +15,7 @@ import torch
 from . import hip
 from .microscaling import _check_floating, _refuse_tangents
 
-MOST_OUTPUTS, MOST_INPUTS, MOST_ROWS = (1 << 27) - 1, (1 << 24) - 1, (1 << 27) - 1
+MOST_OUTPUTS, MOST_INPUTS, MOST_ROWS = (1 << 25) - 1, (1 << 24) - 1, (1 << 27) - 1
 
 
 def _check_group(group):
@@ -142,7 +142,8 @@ def int4_linear(x, weight, bias=None):
 
     The weight's scales have x's dtype or float32, and ``bias`` [o] x's dtype.  It is a product for serving:
     an operand that wants a gradient is refused while gradients are recorded, one with a tangent of
-    forward mode always.  Rows of x and o are below 2**27 and k below 2**24.  A NaN or an infinity in a
+    forward mode always.  Rows of x are below 2**27, o below 2**25 and k
+    below 2**24.  A NaN or an infinity in a
     row of x, or sums of a group's 15 |x| beyond FP32, leave that row without finite values."""
     _check_floating("x", x)
     if not isinstance(weight, Int4Tensor):

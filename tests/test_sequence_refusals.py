@@ -185,9 +185,9 @@ def test_library_arguments():
     assert lib.mf_dropout(at + 1, 0, 4, None, 1, 0, 0, None, at, None) == hip.E_INVALID
     for group in (0, 16, 33, 1 << 25):
         assert lib.mf_int4_dequantize(at, at, 0, None, 1, 1, group, at, 0, None) == hip.E_INVALID
-    assert lib.mf_int4_linear(at, 0, 0, 1, 1, at, at, 0, None, 1, 32, None, at, None) == hip.E_INVALID
-    assert lib.mf_int4_linear(at, 0, 1, 2, 1, at, at, 0, None, 1, 32, None, at, None) == hip.E_INVALID
-    assert lib.mf_int4_linear(at, 1, 1, 1, 1, at, at, 2, None, 1, 32, None, at, None) == hip.E_INVALID
+    assert lib.mf_int4_linear(at, 0, 0, 1, 1, at, at, 0, None, 1, 32, None, at, None, 0, None) == hip.E_INVALID
+    assert lib.mf_int4_linear(at, 0, 2, 2, 1, at, at, 0, None, 1, 32, None, at, None, 0, None) == hip.E_INVALID
+    assert lib.mf_int4_linear(at, 1, 1, 1, 1, at, at, 2, None, 1, 32, None, at, None, 0, None) == hip.E_INVALID
     assert lib.mf_int4_quantize(at, 0, 1, 32, 31, 32, at, at, 0, None) == hip.E_INVALID
 
 
