@@ -672,7 +672,7 @@ int mf_int4_dequantize(const uint8_t *codes, const void *scales, int32_t scale_t
  * codes and x are summed in FP32 by group and scaled then.  n < 2^27.  The workspace
  * (mf_int4_linear_workspace bytes, which may be 0; 16-byte aligned) belongs to the one call; `pieces`: x is
  * 16-byte aligned and its rows are whole multiples of 16 bytes apart. */
-int mf_int4_linear_workspace(int32_t type, int64_t n, int64_t k, int64_t group, int32_t pieces,
+int mf_int4_linear_workspace(int32_t type, int64_t n, int64_t k, int64_t o, int64_t group, int32_t pieces,
                              int64_t *bytes);
 int mf_int4_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ldx, const uint8_t *codes,
                    const void *scales, int32_t scale_type, const uint8_t *zeros, int64_t o, int64_t group,

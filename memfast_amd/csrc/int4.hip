@@ -281,7 +281,7 @@ struct PrepareArgs {
     i64 n, k, ldx, spans, pitch;
     int per;
     float factor;
-    float *sums;
+    float *sums;        // or nullptr
     u16 *planes;        // [TERMS, n, 128 spans], or nullptr: x is taken as it is
 };
 
@@ -311,6 +311,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_int4_prepare(cons
                     }
                 }
             }
+        if (!a.sums) continue;
 #pragma unroll
         for (int d = 1; d <= 8; d <<= 1) sum += __shfl_xor(sum, d);
         if (a.per == 1) {
@@ -326,8 +327,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_int4_prepare(cons
 struct TileArgs {
     HeldArgs h;             // h.x: rows of 16-bit operands, h.ldx apart, of whole spans
     i64 plane;              // distance of x's terms, in values
-    const float *sums;
+    const float *sums;      // x's sums, or (TABLE false) nullptr
     i64 pitch;
+    i64 splits, share;      // workgroups along the spans, and the spans of each
+    float *parts;           // [splits, n, o], where there are several
 };
 
 template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v16f c) {
@@ -339,27 +342,44 @@ template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v1
                                                        __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// A workgroup of four waves takes 32 NT rows and 256 outputs, a wave 64 of them: its codes go from memory to
-// registers, where they become operands once for all rows; x comes through LDS, copied by DMA a span ahead.
-// Sums over a group begin at -8 times the sum of x (the sums' table), so a zero point of 8 costs nothing;
-// others (ZEROS) are taken off with one operation more a group and result.  PER: scalings in a span, 1 for
-// groups of 128 on, else 4.
-constexpr int TILE_WAVES = 4, TILE_OUTPUTS = 64 * TILE_WAVES;
+// A workgroup of four waves takes 32 NT rows and 128 NO outputs, a wave 32 NO of them: its codes go from
+// memory to registers, where they become operands once for all rows; x comes through LDS, copied by DMA a
+// span ahead.  With the sums' TABLE, sums over a group begin at -8 times the sum of x, so a zero point of 8
+// costs nothing; others (ZEROS) are taken off with one operation more a group and result.  Without it
+// a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for groups of 128 on, else 4.
+constexpr int TILE_WAVES = 4;
+#ifndef BAND
+#define BAND 8
+#endif
 
-template <typename T, typename S, int NT, bool ZEROS, int PER>
-__global__ __launch_bounds__(64 * TILE_WAVES) void k_int4_tile(const TileArgs t) {
+// Waves that a SIMD has to hold: with at most 256 registers each the matrix instructions' results stay where
+// the vector units reach them (else each is copied once more for its scaling).
+constexpr int tile_waves_per_simd(int nt, int no, int terms) { return nt * no == 1 ? 4 : nt * no == 2 ? 3 : 2; }
+
+template <typename T, typename S, int NT, int NO, bool TABLE, bool ZEROS, int PER>
+__global__ __launch_bounds__(64 * TILE_WAVES, tile_waves_per_simd(NT, NO, Operand<T>::TERMS)) void
+k_int4_tile(const TileArgs t) {
+    static_assert(TABLE || ZEROS, "sums that begin at 0 have the zero points taken off");
     typedef Operand<T> Op;
-    constexpr int TERMS = Op::TERMS, ROWS = 32 * NT;
-    constexpr int XBYTES = TERMS * ROWS * SPAN_K * 2, STAGE = XBYTES + 2048;
+    constexpr int TERMS = Op::TERMS, ROWS = 32 * NT, OUTPUTS = 32 * NO * TILE_WAVES;
+    constexpr int XBYTES = TERMS * ROWS * SPAN_K * 2, STAGE = XBYTES + (TABLE ? 2048 : 0);
     extern __shared__ __align__(16) u8 staged[];
     const HeldArgs &a = t.h;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = lane >> 5, row = lane & 31, r = lane & 15;
-    const u32 tn = u32((a.n + ROWS - 1) / ROWS), to = u32((a.o + TILE_OUTPUTS - 1) / TILE_OUTPUTS);
+    const u32 tn = u32((a.n + ROWS - 1) / ROWS), to = u32((a.o + OUTPUTS - 1) / OUTPUTS);
+    // Each XCD takes a run of tiles (xcd_tile), here in bands of BAND tiles of rows and all outputs, so that what
+    // it reads at a time is as much of x as of W and stays in its L2.
     u32 nx, oy;
-    xcd_tile(blockIdx.x, tn, to, nx, oy);
-    const i64 n0 = i64(nx) * ROWS, o0 = i64(oy) * TILE_OUTPUTS + wave * 64;
+    xcd_tile(blockIdx.x, 1, tn * to * u32(t.splits), nx, oy);
+    const u32 columns = to * u32(t.splits), band = oy / (BAND * columns), within = oy - band * BAND * columns;
+    const u32 high = min(u32(BAND), tn - band * BAND);
+    nx = band * BAND + within % high;
+    oy = within / high;
+    const u32 split = oy % u32(t.splits);
+    const i64 n0 = i64(nx) * ROWS, o0 = i64(oy / u32(t.splits)) * OUTPUTS + wave * (32 * NO);
     const i64 tiles = (a.o + TILE - 1) / TILE;
+    const int first = int(split * t.share), last = int(min(first + t.share, a.spans));
 
     // Copies: 1 KiB each, four rows of x (row q's 16-byte pieces p at p ^ (q & 15)) or two rows of sums.
     constexpr int COPIES = XBYTES / 1024 / TILE_WAVES;
@@ -373,113 +393,145 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void k_int4_tile(const TileArgs t)
     }
     const float *sums = t.sums + n0 + (lane & 31) * 4;
     const u32 lds = lds_address(staged);
-    const auto copy = [&](i64 span, int buffer) {
-        const u32 to = lds + buffer * STAGE;
+    const auto copy = [&](int span) {
+        const u32 to = lds + (span & 1) * STAGE;
 #pragma unroll
         for (int i = 0; i < COPIES; ++i)
-            lds_dma_16(source[i] + span * (SPAN_K * 2),
+            lds_dma_16(source[i] + i64(span) * (SPAN_K * 2),
                        __builtin_amdgcn_readfirstlane(to + (wave * COPIES + i) * 1024));
-        if (wave < (PER + 1) / 2)
-            lds_dma_16(sums + (span * PER + min(wave * 2 + half, PER - 1)) * t.pitch,
+        if (TABLE && wave < (PER + 1) / 2)
+            lds_dma_16(sums + i64(span * PER + min(wave * 2 + half, PER - 1)) * t.pitch,
                        __builtin_amdgcn_readfirstlane(to + XBYTES + wave * 1024));
     };
 
     // A lane's output is 32 j + row of the wave's; it reads both 16-byte pieces of its half.
-    const u8 *codes[2];
-    const S *scales[2];
-    const u8 *zeros[2];
+    const u8 *codes[NO];
+    const S *scales[NO];
+    const u8 *zeros[NO];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NO; ++j) {
         const i64 tile = min((o0 + 32 * j + row) / TILE, tiles - 1);
         codes[j] = a.codes + tile * a.spans * SPAN_BYTES + half * 256 + r * 16;
         scales[j] = static_cast<const S *>(a.scales) + tile * a.groups * 16 + r;
-        zeros[j] = ZEROS ? a.zeros + tile * a.groups * 16 + r : nullptr;
+        zeros[j] = ZEROS && a.zeros ? a.zeros + tile * a.groups * 16 + r : nullptr;
     }
-    v4u w[2][2];
-    S s[2][PER];
-    u8 z[2][PER];
-    const auto fetch = [&](i64 span) {
+    v4u w[NO][2];
+    S s[NO][PER];
+    u8 z[NO][PER];
+    const auto fetch = [&](int span) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NO; ++j) {
 #pragma unroll
             for (int m = 0; m < 2; ++m)
-                w[j][m] = *reinterpret_cast<const v4u *>(codes[j] + span * SPAN_BYTES + m * 512);
+                w[j][m] = *reinterpret_cast<const v4u *>(codes[j] + i64(span) * SPAN_BYTES + m * 512);
 #pragma unroll
             for (int g = 0; g < PER; ++g) {
-                const i64 at = min((span * SPAN_K + g * 32) >> a.shift, a.groups - 1) * 16;
+                const int at = min((span * SPAN_K + g * 32) >> a.shift, int(a.groups) - 1) * 16;
                 s[j][g] = scales[j][at];
-                z[j][g] = ZEROS ? zeros[j][at] : u8(8);
+                z[j][g] = u8(8);
+                if (ZEROS && a.zeros) z[j][g] = zeros[j][at];
             }
         }
     };
 
-    v16f total[NT][2] = {};
-    fetch(0);
-    copy(0, 0);
-    for (i64 span = 0; span < a.spans; ++span) {
+    v16f total[NT][NO] = {};
+    if (first < last) {
+        fetch(first);
+        copy(first);
+    }
+    for (int span = first; span < last; ++span) {
         wait_stage<0>();
-        if (span + 1 < a.spans) copy(span + 1, int(span + 1) & 1);
+        if (span + 1 < last) copy(span + 1);
         const u8 *stage = staged + (span & 1) * STAGE;
-        v4u q[2][8];        // operands of 16 inputs each
-        float scale[2][PER], zero[2][PER];
+        v4u held[NO][2];
+        float scale[NO][PER], zero[NO][PER];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NO; ++j) {
 #pragma unroll
-            for (int b = 0; b < 8; ++b)
-                q[j][b] = __builtin_bit_cast(v4u, Op::codes(w[j][b & 1][b >> 1]));
+            for (int m = 0; m < 2; ++m) held[j][m] = w[j][m];
 #pragma unroll
             for (int g = 0; g < PER; ++g) scale[j][g] = float(s[j][g]), zero[j][g] = -float(z[j][g]);
         }
-        if (span + 1 < a.spans) fetch(span + 1);
+        if (span + 1 < last) fetch(span + 1);
+        v16f acc[NT][NO], sum[NT];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const u8 *x = stage + (32 * i + row) * (SPAN_K * 2);
-            v16f acc[2], sum;
+        for (int b = 0; b < 8; ++b) {       // 16 inputs each
+            constexpr int STEPS = 8 / PER;
+            v4u q[NO];
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
-                constexpr int STEPS = 8 / PER;
+            for (int j = 0; j < NO; ++j) q[j] = __builtin_bit_cast(v4u, Op::codes(held[j][b & 1][b >> 1]));
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
                 if (b % STEPS == 0) {
-                    const float *from = reinterpret_cast<const float *>(stage + XBYTES) +
-                                        b / STEPS * 128 + 32 * i + 4 * half;
+                    sum[i] = v16f{};
+                    if (TABLE) {
+                        const float *from = reinterpret_cast<const float *>(stage + XBYTES) +
+                                            b / STEPS * 128 + 32 * i + 4 * half;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const v4f four = *reinterpret_cast<const v4f *>(from + 8 * e);
+                        for (int e = 0; e < 4; ++e) {
+                            const v4f four = *reinterpret_cast<const v4f *>(from + 8 * e);
 #pragma unroll
-                        for (int f = 0; f < 4; ++f) sum[4 * e + f] = four[f];
+                            for (int f = 0; f < 4; ++f) sum[i][4 * e + f] = four[f];
+                        }
                     }
-                    acc[0] = acc[1] = ZEROS ? v16f{} : sum;
+#pragma unroll
+                    for (int j = 0; j < NO; ++j) acc[i][j] = ZEROS ? v16f{} : sum[i];
                 }
 #pragma unroll
                 for (int m = 0; m < TERMS; ++m) {
                     const v4u xf = *reinterpret_cast<const v4u *>(
-                        x + m * (ROWS * SPAN_K * 2) + ((2 * b + half) ^ r) * 16);
-                    acc[0] = mfma_wide<T>(xf, q[0][b], acc[0]);
-                    acc[1] = mfma_wide<T>(xf, q[1][b], acc[1]);
-                }
-                if ((b + 1) % STEPS == 0)
+                        stage + (m * ROWS + 32 * i + row) * (SPAN_K * 2) + ((2 * b + half) ^ r) * 16);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < NO; ++j) acc[i][j] = mfma_wide<T>(xf, q[j], acc[i][j]);
+                    if (!TABLE) sum[i] = mfma_wide<T>(xf, __builtin_bit_cast(v4u, Op::ones()), sum[i]);
+                }
+            }
+            if ((b + 1) % STEPS == 0)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NO; ++j)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float v = ZEROS ? fmaf(zero[j][b / STEPS], sum[e], acc[j][e]) : acc[j][e];
+                            const float v =
+                                ZEROS ? fmaf(zero[j][b / STEPS], sum[i][e], acc[i][j][e]) : acc[i][j][e];
                             total[i][j][e] = fmaf(scale[j][b / STEPS], v, total[i][j][e]);
                         }
-            }
         }
     }
-    T *out = static_cast<T *>(a.out);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NO; ++j) {
         const i64 o = o0 + 32 * j + row;
         if (o >= a.o) continue;
-        const float bias = a.bias ? float(static_cast<const T *>(a.bias)[o]) : 0.0f;
+        const float bias = a.bias && t.splits == 1 ? float(static_cast<const T *>(a.bias)[o]) : 0.0f;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const i64 n = n0 + 32 * i + 8 * (e / 4) + 4 * half + (e & 3);
-                if (n < a.n) out[n * a.o + o] = rounded<T>(total[i][j][e] + bias);
+                if (n >= a.n) continue;
+                if (t.splits > 1)
+                    t.parts[(split * a.n + n) * a.o + o] = total[i][j][e];
+                else
+                    static_cast<T *>(a.out)[n * a.o + o] = rounded<T>(total[i][j][e] + bias);
             }
+    }
+}
+
+// Adds the parts of a product in their order, and the bias.
+template <typename T> __global__ __launch_bounds__(256) void k_int4_join(const TileArgs t) {
+    const i64 all = t.h.n * t.h.o;
+    for (i64 id = i64(blockIdx.x) * 256 + threadIdx.x; id < all; id += i64(gridDim.x) * 256) {
+        float y = 0.0f;
+        for (i64 s = 0; s < t.splits; s += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = t.parts[min(s + i, t.splits - 1) * all + id];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y += s + i < t.splits ? v[i] : 0.0f;
+        }
+        if (t.h.bias) y += float(static_cast<const T *>(t.h.bias)[id % t.h.o]);
+        static_cast<T *>(t.h.out)[id] = rounded<T>(y);
     }
 }
 
@@ -600,72 +652,113 @@ template <typename T, typename S, int NB, int R> int launch_few(const HeldArgs &
     return check_launch("4-bit product");
 }
 
-// Few rows go to k_int4_few.
-constexpr i64 FEW_ROWS = 64, ROWS_AT_ONCE = 8192;
+// Few rows go to k_int4_few, more to tiles of 32 or 64 rows whose spans are split over workgroups, and
+// many to large tiles.
+#ifndef FEW_ROWS
+#define FEW_ROWS 8
+#define MID_ROWS 512
+#define WANTED 512
+#endif
+constexpr i64 ROWS_AT_ONCE = 8192;
 
 // The kernel, how many rows go through tiles at a time, and what the workspace holds for them.
 struct HeldPlan {
-    bool few, direct;       // direct: x is read as it is
+    enum { FEW, MID, TILES } kernel;
+    bool direct;            // x is read as it is
     int per, terms;
-    i64 rows, pitch, spans, sums, bytes;
-    HeldPlan(int32_t type, i64 n, i64 k, i64 group, bool pieces) {
+    i64 rows, pitch, spans, sums, planes, splits = 1, share, bytes;
+    HeldPlan(int32_t type, i64 n, i64 k, i64 o, i64 group, bool pieces) {
         spans = (k + SPAN_K - 1) / SPAN_K;
-        few = n <= FEW_ROWS;
-        direct = few ? pieces && k % 8 == 0 : pieces && type != MF_F32 && k % SPAN_K == 0;
+        share = spans;
+        kernel = n <= FEW_ROWS ? FEW : n <= MID_ROWS ? MID : TILES;
+        direct = kernel == FEW ? pieces && k % 8 == 0 : pieces && type != MF_F32 && k % SPAN_K == 0;
         per = group >= SPAN_K ? 1 : 4;
         terms = type == MF_F32 ? 3 : 1;
         rows = std::min(n, ROWS_AT_ONCE);
         pitch = (rows + 127) / 128 * 128 + 128;
-        sums = few ? 0 : spans * per * pitch * i64(sizeof(float));
-        bytes = sums + (direct ? 0 : rows * spans * SPAN_K * (few ? type_bytes(type) : 2 * terms));
+        sums = kernel != TILES ? 0 : spans * per * pitch * i64(sizeof(float));
+        planes = direct ? 0 : rows * spans * SPAN_K * (kernel == FEW ? type_bytes(type) : 2 * terms);
+        if (kernel == MID) {
+            const i64 tiles = (rows + tile_rows(n) - 1) / tile_rows(n) * ((o + 127) / 128);
+            const i64 wanted = std::min((WANTED + tiles - 1) / tiles, spans / 2);
+            if (wanted > 1) {
+                share = (spans + wanted - 1) / wanted;
+                splits = (spans + share - 1) / share;
+            }
+        }
+        bytes = sums + planes + (splits > 1 ? splits * rows * o * i64(sizeof(float)) : 0);
     }
+    static i64 tile_rows(i64 n) { return n <= 32 ? 32 : 64; }
 };
 
 bool rows_in_pieces(const void *x, i64 ldx, int32_t type) {
     return aligned(x, 16) && ldx * type_bytes(type) % 16 == 0;
 }
 
-template <typename T, typename S, int NT, bool ZEROS, int PER>
+template <typename T, typename S, int NT, int NO, bool TABLE, bool ZEROS, int PER>
 int launch_tile(const TileArgs &t, hipStream_t s) {
-    constexpr int ROWS = 32 * NT, LDS = 2 * (Operand<T>::TERMS * ROWS * SPAN_K * 2 + 2048);
-    const auto kernel = k_int4_tile<T, S, NT, ZEROS, PER>;
+    constexpr int ROWS = 32 * NT, OUTPUTS = 32 * NO * TILE_WAVES;
+    constexpr int LDS = 2 * (Operand<T>::TERMS * ROWS * SPAN_K * 2 + (TABLE ? 2048 : 0));
+    const auto kernel = k_int4_tile<T, S, NT, NO, TABLE, ZEROS, PER>;
     const int status = allow_lds(kernel, LDS);
     if (status) return status;
-    const i64 tiles = (t.h.n + ROWS - 1) / ROWS * ((t.h.o + TILE_OUTPUTS - 1) / TILE_OUTPUTS);
+    const i64 tiles = (t.h.n + ROWS - 1) / ROWS * ((t.h.o + OUTPUTS - 1) / OUTPUTS) * t.splits;
     hipLaunchKernelGGL(kernel, dim3(u32(tiles)), dim3(64 * TILE_WAVES), LDS, s, t);
     return check_launch("4-bit product");
 }
 
-#ifndef NT16
-#define NT16 4
-#endif
-template <typename T, typename S> int launch_tiles(HeldArgs a, const HeldPlan &plan, void *workspace, hipStream_t s) {
-    constexpr int NT = Operand<T>::TERMS == 1 ? NT16 : 2;
+// Tiles of 64 rows and 256 outputs.
+template <typename T, typename S> int launch_large(const TileArgs &t, int per, hipStream_t s) {
+    if (per == 1)
+        return t.h.zeros ? launch_tile<T, S, 2, 2, true, true, 1>(t, s)
+                         : launch_tile<T, S, 2, 2, true, false, 1>(t, s);
+    return t.h.zeros ? launch_tile<T, S, 2, 2, true, true, 4>(t, s)
+                     : launch_tile<T, S, 2, 2, true, false, 4>(t, s);
+}
+
+// Tiles of 32 or 64 rows and 128 outputs, with the spans split.
+template <typename T, typename S> int launch_mid(const TileArgs &t, int per, hipStream_t s) {
+    int status;
+    if (HeldPlan::tile_rows(t.h.n) == 32)
+        status = per == 1 ? launch_tile<T, S, 1, 1, false, true, 1>(t, s)
+                          : launch_tile<T, S, 1, 1, false, true, 4>(t, s);
+    else
+        status = per == 1 ? launch_tile<T, S, 2, 1, false, true, 1>(t, s)
+                          : launch_tile<T, S, 2, 1, false, true, 4>(t, s);
+    if (status || t.splits == 1) return status;
+    hipLaunchKernelGGL(k_int4_join<T>, dim3(u32(std::min<i64>((t.h.n * t.h.o + 255) / 256, 1 << 16))),
+                       dim3(256), 0, s, t);
+    return check_launch("4-bit product's parts");
+}
+
+template <typename T, typename S>
+int launch_tiles(HeldArgs a, const HeldPlan &plan, void *workspace, hipStream_t s) {
     const char *x = static_cast<const char *>(a.x);
-    char *out = static_cast<char *>(a.out);
+    char *out = static_cast<char *>(a.out), *work = static_cast<char *>(workspace);
     const i64 n = a.n;
     for (i64 first = 0; first < n; first += plan.rows) {
         a.n = std::min(plan.rows, n - first);
         a.out = out + first * a.o * i64(sizeof(T));
-        const void *rows = x + first * a.ldx * i64(sizeof(T));
-        PrepareArgs p{rows, a.n, a.k, a.ldx, a.spans, plan.pitch, plan.per, a.zeros ? 1.0f : -8.0f,
-                      static_cast<float *>(workspace), nullptr};
-        TileArgs t{a, 0, p.sums, plan.pitch};
-        t.h.x = rows;
+        a.x = x + first * a.ldx * i64(sizeof(T));
+        const bool table = plan.kernel == HeldPlan::TILES;
+        PrepareArgs p{a.x, a.n, a.k, a.ldx, a.spans, table ? plan.pitch : a.n, plan.per,
+                      a.zeros ? 1.0f : -8.0f, table ? reinterpret_cast<float *>(work) : nullptr, nullptr};
+        TileArgs t{a, 0, p.sums, plan.pitch, plan.splits, plan.share,
+                   reinterpret_cast<float *>(work + plan.sums + plan.planes)};
         if (!plan.direct) {
-            p.planes = reinterpret_cast<u16 *>(static_cast<char *>(workspace) + plan.sums);
+            p.planes = reinterpret_cast<u16 *>(work + plan.sums);
             t.h.x = p.planes;
             t.h.ldx = a.spans * SPAN_K;
             t.plane = a.n * t.h.ldx;
         }
-        hipLaunchKernelGGL(k_int4_prepare<T>, dim3(u32(std::min<i64>((p.pitch * p.spans + 3) / 4, 1 << 16))),
-                           dim3(256), 0, s, p);
-        int status = check_launch("4-bit product's rows");
-        if (status) return status;
-        if (plan.per == 1)
-            status = a.zeros ? launch_tile<T, S, NT, true, 1>(t, s) : launch_tile<T, S, NT, false, 1>(t, s);
-        else
-            status = a.zeros ? launch_tile<T, S, NT, true, 4>(t, s) : launch_tile<T, S, NT, false, 4>(t, s);
+        int status = MF_OK;
+        if (table || !plan.direct) {
+            hipLaunchKernelGGL(k_int4_prepare<T>,
+                               dim3(u32(std::min<i64>((p.pitch * p.spans + 3) / 4, 1 << 16))), dim3(256), 0,
+                               s, p);
+            status = check_launch("4-bit product's rows");
+        }
+        if (!status) status = table ? launch_large<T, S>(t, plan.per, s) : launch_mid<T, S>(t, plan.per, s);
         if (status) return status;
     }
     return MF_OK;
@@ -673,7 +766,7 @@ template <typename T, typename S> int launch_tiles(HeldArgs a, const HeldPlan &p
 
 template <typename T, typename S> int launch_held(HeldArgs a, const HeldPlan &plan, void *workspace,
                                                   hipStream_t s) {
-    if (!plan.few) return launch_tiles<T, S>(a, plan, workspace, s);
+    if (plan.kernel != HeldPlan::FEW) return launch_tiles<T, S>(a, plan, workspace, s);
     if (!plan.direct) {
         T *rows = static_cast<T *>(workspace);
         hipLaunchKernelGGL(k_int4_pad<T>, dim3(u32((a.n * a.spans + 3) / 4)), dim3(256), 0, s,
@@ -744,12 +837,12 @@ int mf_int4_dequantize(const uint8_t *codes, const void *scales, int32_t scale_t
     });
 }
 
-int mf_int4_linear_workspace(int32_t type, int64_t n, int64_t k, int64_t group, int32_t pieces,
+int mf_int4_linear_workspace(int32_t type, int64_t n, int64_t k, int64_t o, int64_t group, int32_t pieces,
                              int64_t *bytes) {
-    if (!known_type(type) || n < 1 || k < 1 || n >= MOST_ROWS || k >= MOST_INPUTS || group_shift(group) < 0 ||
-        !bytes)
+    if (!known_type(type) || n < 1 || k < 1 || o < 1 || n >= MOST_ROWS || k >= MOST_INPUTS ||
+        o >= MOST_OUTPUTS || group_shift(group) < 0 || !bytes)
         return fail(MF_E_INVALID, "invalid 4-bit product sizes");
-    *bytes = HeldPlan(type, n, k, group, pieces != 0).bytes;
+    *bytes = HeldPlan(type, n, k, o, group, pieces != 0).bytes;
     return MF_OK;
 }
 
@@ -767,7 +860,7 @@ int mf_int4_linear(const void *x, int32_t type, int64_t n, int64_t k, int64_t ld
     if (n >= MOST_ROWS)
         return fail(MF_E_UNSUPPORTED, "4-bit product of %lld rows", (long long)n);
     a.x = x, a.n = n, a.ldx = ldx, a.bias = bias, a.out = out;
-    const HeldPlan plan(type, n, k, group, rows_in_pieces(x, ldx, type));
+    const HeldPlan plan(type, n, k, o, group, rows_in_pieces(x, ldx, type));
     if (bytes < plan.bytes || (plan.bytes && (!workspace || !aligned(workspace, 16))))
         return fail(MF_E_INVALID, "4-bit product's workspace of %lld bytes", (long long)bytes);
     return with_types(type, scale_type, [&](auto t, auto scale) {

@@ -223,7 +223,7 @@ SIGNATURES = {
     "mf_dropout": ([_P, _I32, _I64, _P, ct.c_uint32, ct.c_uint64, ct.c_uint64, _P, _P, _P], ct.c_int),
     "mf_int4_quantize": ([_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _P], ct.c_int),
     "mf_int4_dequantize": ([_P, _P, _I32, _P, _I64, _I64, _I64, _P, _I32, _P], ct.c_int),
-    "mf_int4_linear_workspace": ([_I32, _I64, _I64, _I64, _I32, ct.POINTER(_I64)], ct.c_int),
+    "mf_int4_linear_workspace": ([_I32, _I64, _I64, _I64, _I64, _I32, ct.POINTER(_I64)], ct.c_int),
     "mf_int4_linear": ([_P, _I32, _I64, _I64, _I64, _P, _P, _I32, _P, _I64, _I64, _P, _P, _P, _I64, _P],
                        ct.c_int),
     "mf_rng_uniform": ([_P, _I64, ct.c_uint64, ct.c_uint32, _P, _P], ct.c_int),
@@ -1728,9 +1728,9 @@ def int4_dequantize(codes, scales, zeros, o, k, group, dtype):
 
 
 @lru_cache(maxsize=4096)
-def _int4_workspace(kind, n, k, group, pieces):
+def _int4_workspace(kind, n, k, o, group, pieces):
     size = _I64()
-    check(library().mf_int4_linear_workspace(kind, n, k, group, pieces, ct.byref(size)), "4-bit product")
+    check(library().mf_int4_linear_workspace(kind, n, k, o, group, pieces, ct.byref(size)), "4-bit product")
     return size.value
 
 
@@ -1739,7 +1739,7 @@ def int4_linear(x, codes, scales, zeros, o, group, bias):
     n, k = x.shape
     kind, at, ldx, device = FLOAT_TYPES[x.dtype], x.data_ptr(), x.stride(0), x.device
     pieces = at % 16 == 0 and ldx * x.element_size() % 16 == 0
-    size = _int4_workspace(kind, n, k, group, pieces)
+    size = _int4_workspace(kind, n, k, o, group, pieces)
     out = torch.empty((n, o), dtype=x.dtype, device=device)
     work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     with _on(device):
