@@ -347,10 +347,7 @@ template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v1
 // span ahead.  With the sums' TABLE, sums over a group begin at -8 times the sum of x, so a zero point of 8
 // costs nothing; others (ZEROS) are taken off with one operation more a group and result.  Without it
 // a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for groups of 128 on, else 4.
-constexpr int TILE_WAVES = 4;
-#ifndef BAND
-#define BAND 8
-#endif
+constexpr int TILE_WAVES = 4, BAND = 8;
 
 // Waves that a SIMD has to hold: with at most 256 registers each the matrix instructions' results stay where
 // the vector units reach them (else each is copied once more for its scaling).
@@ -635,60 +632,70 @@ int check_held(const void *codes, const void *scales, int32_t scale_type, const 
     return MF_OK;
 }
 
-#ifndef FW
-#define FW 8
-#define FO 1
-#define FA true
-#endif
-template <typename T, typename S, int NB, int R> int launch_few(const HeldArgs &a, hipStream_t s) {
-    constexpr int WAVES = FW, OT = FO;
+template <typename T, typename S, int OT, int NB, int R> int launch_few(const HeldArgs &a, hipStream_t s) {
+    // x a span ahead, where there are registers for it.
+    constexpr int WAVES = 8;
+    constexpr bool AHEAD = Operand<T>::TERMS == 1 || NB < 3;
     const i64 tiles = (a.o + TILE - 1) / TILE;
     const int lds = WAVES * OT * NB * R * 64 * int(sizeof(float));
-    const auto kernel = a.shift >= 7 ? k_int4_few<T, S, WAVES, OT, NB, R, 1, FA>
-                                     : k_int4_few<T, S, WAVES, OT, NB, R, 4, FA>;
+    const auto kernel = a.shift >= 7 ? k_int4_few<T, S, WAVES, OT, NB, R, 1, AHEAD>
+                                     : k_int4_few<T, S, WAVES, OT, NB, R, 4, AHEAD>;
     const int status = allow_lds(kernel, lds);
     if (status) return status;
     hipLaunchKernelGGL(kernel, dim3(u32((tiles + OT - 1) / OT)), dim3(64 * WAVES), lds, s, a);
     return check_launch("4-bit product");
 }
 
-// Few rows go to k_int4_few, more to tiles of 32 or 64 rows whose spans are split over workgroups, and
-// many to large tiles.
-#ifndef FEW_ROWS
-#define FEW_ROWS 8
-#define MID_ROWS 512
-#define WANTED 512
-#endif
 constexpr i64 ROWS_AT_ONCE = 8192;
 
 // The kernel, how many rows go through tiles at a time, and what the workspace holds for them.
 struct HeldPlan {
-    enum { FEW, MID, TILES } kernel;
+    enum { FEW, MID, LARGE } kernel;
     bool direct;            // x is read as it is
     int per, terms;
     i64 rows, pitch, spans, sums, planes, splits = 1, share, bytes;
     HeldPlan(int32_t type, i64 n, i64 k, i64 o, i64 group, bool pieces) {
-        spans = (k + SPAN_K - 1) / SPAN_K;
-        share = spans;
-        kernel = n <= FEW_ROWS ? FEW : n <= MID_ROWS ? MID : TILES;
-        direct = kernel == FEW ? pieces && k % 8 == 0 : pieces && type != MF_F32 && k % SPAN_K == 0;
+        spans = share = (k + SPAN_K - 1) / SPAN_K;
         per = group >= SPAN_K ? 1 : 4;
         terms = type == MF_F32 ? 3 : 1;
         rows = std::min(n, ROWS_AT_ONCE);
+        kernel = few(type, n, k, o) ? FEW : large(type, rows, o) ? LARGE : MID;
+        direct = kernel == FEW ? pieces && k % 8 == 0 : pieces && type != MF_F32 && k % SPAN_K == 0;
         pitch = (rows + 127) / 128 * 128 + 128;
-        sums = kernel != TILES ? 0 : spans * per * pitch * i64(sizeof(float));
+        sums = kernel == LARGE ? spans * per * pitch * i64(sizeof(float)) : 0;
         planes = direct ? 0 : rows * spans * SPAN_K * (kernel == FEW ? type_bytes(type) : 2 * terms);
-        if (kernel == MID) {
-            const i64 tiles = (rows + tile_rows(n) - 1) / tile_rows(n) * ((o + 127) / 128);
-            const i64 wanted = std::min((WANTED + tiles - 1) / tiles, spans / 2);
-            if (wanted > 1) {
-                share = (spans + wanted - 1) / wanted;
+        if (kernel != FEW) {
+            // Spans are split until every compute unit has a workgroup, or two of those of 32 rows that
+            // scale four times a span (us, 64 x 4096 x 4096, groups of 128, 8 / 12 / 16 splits: 15 / 19 / 20;
+            // 24 x 11008 x 4096, 8 / 16: 14 / 15; 32 x 4096 x 11008, groups of 32, 2 / 5: 26 / 20).
+            const i64 tiles = kernel == LARGE ? large_tiles(rows, o)
+                                              : (rows + mid_rows(n) - 1) / mid_rows(n) * ((o + 127) / 128);
+            const i64 wanted = kernel == LARGE ? 256 / tiles : ((per == 1 ? 256 : 512) + tiles - 1) / tiles;
+            if (std::min(wanted, spans / 2) > 1) {
+                share = (spans + std::min(wanted, spans / 2) - 1) / std::min(wanted, spans / 2);
                 splits = (spans + share - 1) / share;
             }
         }
         bytes = sums + planes + (splits > 1 ? splits * rows * o * i64(sizeof(float)) : 0);
     }
-    static i64 tile_rows(i64 n) { return n <= 32 ? 32 : 64; }
+    // Workgroups of k_int4_few read all of x again for every tile, or for two (wide).
+    static bool wide(i64 n, i64 o) { return n > 4 && n <= 32 && o >= 8192; }
+    // Up to 64 rows while that is little, and a wave's chain of spans short (us, few / tiles: 24 x 4096 x
+    // 4096 8.9 / 13.3, 48 x 2048 x 2048 8.0 / 8.9, 24 x 11008 x 4096 20 / 14, 64 x 4096 x 1024 17 / 11,
+    // 32 x 4096 x 11008 20 / 16).
+    static bool few(int32_t type, i64 n, i64 k, i64 o) {
+        const i64 tiles = (o + TILE - 1) / TILE / (wide(n, o) ? 2 : 1);
+        return n <= 16 || (n <= 64 && (k + SPAN_K - 1) / SPAN_K * ((n + 15) / 16) <= 64 &&
+                           tiles * n * k * type_bytes(type) <= i64(72) << 20);
+    }
+    static i64 mid_rows(i64 n) { return n <= 32 ? 32 : 64; }
+    static i64 large_tiles(i64 n, i64 o) { return (n + 63) / 64 * ((o + 255) / 256); }
+    // The sums' launch and the wide tiles pay for many rows, of FP32, whose sums take three times the
+    // instructions, from fewer on, where they are tiles enough (us, mid / large: 256 x 4096 x 11008 47 / 41,
+    // 128 of them 31 / 30, 256 x 4096 x 4096 31 / 30 and in FP32 85 / 48, 300 x 2048 x 2048 18 / 21).
+    static bool large(int32_t type, i64 n, i64 o) {
+        return n > (type == MF_F32 ? 64 : 128) && o > 128 && large_tiles(n, o) >= 64;
+    }
 };
 
 bool rows_in_pieces(const void *x, i64 ldx, int32_t type) {
@@ -718,14 +725,14 @@ template <typename T, typename S> int launch_large(const TileArgs &t, int per, h
 
 // Tiles of 32 or 64 rows and 128 outputs, with the spans split.
 template <typename T, typename S> int launch_mid(const TileArgs &t, int per, hipStream_t s) {
-    int status;
-    if (HeldPlan::tile_rows(t.h.n) == 32)
-        status = per == 1 ? launch_tile<T, S, 1, 1, false, true, 1>(t, s)
-                          : launch_tile<T, S, 1, 1, false, true, 4>(t, s);
-    else
-        status = per == 1 ? launch_tile<T, S, 2, 1, false, true, 1>(t, s)
-                          : launch_tile<T, S, 2, 1, false, true, 4>(t, s);
-    if (status || t.splits == 1) return status;
+    if (HeldPlan::mid_rows(t.h.n) == 32)
+        return per == 1 ? launch_tile<T, S, 1, 1, false, true, 1>(t, s)
+                        : launch_tile<T, S, 1, 1, false, true, 4>(t, s);
+    return per == 1 ? launch_tile<T, S, 2, 1, false, true, 1>(t, s)
+                    : launch_tile<T, S, 2, 1, false, true, 4>(t, s);
+}
+
+template <typename T> int launch_join(const TileArgs &t, hipStream_t s) {
     hipLaunchKernelGGL(k_int4_join<T>, dim3(u32(std::min<i64>((t.h.n * t.h.o + 255) / 256, 1 << 16))),
                        dim3(256), 0, s, t);
     return check_launch("4-bit product's parts");
@@ -740,7 +747,7 @@ int launch_tiles(HeldArgs a, const HeldPlan &plan, void *workspace, hipStream_t 
         a.n = std::min(plan.rows, n - first);
         a.out = out + first * a.o * i64(sizeof(T));
         a.x = x + first * a.ldx * i64(sizeof(T));
-        const bool table = plan.kernel == HeldPlan::TILES;
+        const bool table = plan.kernel == HeldPlan::LARGE;
         PrepareArgs p{a.x, a.n, a.k, a.ldx, a.spans, table ? plan.pitch : a.n, plan.per,
                       a.zeros ? 1.0f : -8.0f, table ? reinterpret_cast<float *>(work) : nullptr, nullptr};
         TileArgs t{a, 0, p.sums, plan.pitch, plan.splits, plan.share,
@@ -759,6 +766,7 @@ int launch_tiles(HeldArgs a, const HeldPlan &plan, void *workspace, hipStream_t 
             status = check_launch("4-bit product's rows");
         }
         if (!status) status = table ? launch_large<T, S>(t, plan.per, s) : launch_mid<T, S>(t, plan.per, s);
+        if (!status && plan.splits > 1) status = launch_join<T>(t, s);
         if (status) return status;
     }
     return MF_OK;
@@ -777,12 +785,15 @@ template <typename T, typename S> int launch_held(HeldArgs a, const HeldPlan &pl
         a.ldx = a.spans * SPAN_K;
         a.k = a.ldx;        // zeros included: the codes past the weight's inputs are there too
     }
-    return a.n <= 4    ? launch_few<T, S, 1, 1>(a, s)
-           : a.n <= 8  ? launch_few<T, S, 1, 2>(a, s)
-           : a.n <= 16 ? launch_few<T, S, 1, 4>(a, s)
-           : a.n <= 32 ? launch_few<T, S, 2, 4>(a, s)
-           : a.n <= 48 ? launch_few<T, S, 3, 4>(a, s)
-                       : launch_few<T, S, 4, 4>(a, s);
+    // Two tiles a workgroup halve what is read of x, and the workgroups: 8 x 4096 x 11008 10.9 -> 9.8 us,
+    // 16 of them 14.2 -> 11.7; 16 x 4096 x 4096 6.5 -> 6.7, 1 x 4096 x 4096 3.7 -> 5.1.
+    const bool wide = HeldPlan::wide(a.n, a.o);
+    return a.n <= 4    ? launch_few<T, S, 1, 1, 1>(a, s)
+           : a.n <= 8  ? wide ? launch_few<T, S, 2, 1, 2>(a, s) : launch_few<T, S, 1, 1, 2>(a, s)
+           : a.n <= 16 ? wide ? launch_few<T, S, 2, 1, 4>(a, s) : launch_few<T, S, 1, 1, 4>(a, s)
+           : a.n <= 32 ? wide ? launch_few<T, S, 2, 2, 4>(a, s) : launch_few<T, S, 1, 2, 4>(a, s)
+           : a.n <= 48 ? launch_few<T, S, 1, 3, 4>(a, s)
+                       : launch_few<T, S, 1, 4, 4>(a, s);
 }
 
 // Calls f(T{}, S{}) for the types of x and of the scales: x's own or FP32.

@@ -88,6 +88,24 @@ def test_sizes(hip_device, kind, k, o):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,k,o", [(65, 300, 17000), (200, 1024, 4200), (129, 130, 5600), (300, 1000, 4096),
+                                   (1000, 96, 1100), (8200, 40, 300), (8193, 256, 140), (9000, 33, 100)])
+def test_large_tiles_and_many_rows(hip_device, kind, n, k, o):
+    """Tiles of 64 by 256 with their spans split or not, and rows taken 8192 at a time."""
+    for group, zeros in ((32, False), (128, True), (64, True), (256, False)):
+        check(hip_device, n, k, o, group, kind, zeros=zeros, bias=zeros)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,k,o", [(17, 600, 8200), (6, 300, 8193), (32, 264, 8192), (64, 1032, 500),
+                                   (40, 8, 33), (24, 11008, 400), (48, 4096, 300)])
+def test_between_few_rows_and_tiles(hip_device, kind, n, k, o):
+    """Both sides of the rules that choose a kernel."""
+    for group, zeros in ((32, True), (128, False)):
+        check(hip_device, n, k, o, group, kind, zeros=zeros)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("group", [32, 64, 128, 256, 1024, 1 << 24])
 @pytest.mark.parametrize("zeros", [False, True])
 def test_groups(hip_device, kind, group, zeros):
