@@ -437,13 +437,16 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
     for (int j = 0; j < V; ++j) part[j] = A[j], part[a.width + j] = S[j];
 }
 
-// Segments along the steps: where the channels alone give too few workgroups, and there are steps
-// enough for each to be SPAN of them at least.
+// Segments along the steps, where the channels alone give too few workgroups. They cost another pass over the
+// input and another launch: in tenths of a microsecond an unsplit workgroup takes 30 and 27 for 128 steps, whatever
+// the others do, split ones 90 and their bytes (BF16, 8 x 1000 x 1024: 26 us unsplit, 28 split; 12 x
+// 600 x 1024 18 and 28; 4 x 1000 x 1024 23 and 19; 1 x 1000 x 512 22 and 14).
 struct Split {
     i64 segments = 1, segment;
     Split(i64 steps, i64 batch, i64 width) : segment((steps + SPAN - 1) / SPAN * SPAN) {
         const i64 columns = batch * ((width + 63) / 64), spans = segment / SPAN;
-        if (columns >= 256 || spans < 3) return;
+        const double states = double(steps) * double(batch) * double(width);
+        if (columns >= 256 || spans < 3 || double(30 + 27 * spans) <= 90.0 + states / 45000.0) return;
         const i64 wanted = std::min<i64>((512 + columns - 1) / columns, spans);
         segment = (spans + wanted - 1) / wanted * SPAN;
         segments = (steps + segment - 1) / segment;

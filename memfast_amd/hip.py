@@ -1642,38 +1642,43 @@ def _recurrence_sizes(steps, batch, width):
 def recurrence(x, state, lengths, reverse, tanh, batch_first, keep):
     """States [T, B, H] and last state of ``x`` [T, B, 2H] (``batch_first``: the first two dimensions
     are exchanged), and with ``keep`` the marks that ``recurrence_grad`` starts from (mf_recurrence)."""
-    t, b = (1, 0) if batch_first else (0, 1)
-    steps, batch, width = x.shape[t], x.shape[b], x.shape[2] // 2
+    (steps, batch, width), (xt, xb, _) = x.shape, x.stride()
+    width //= 2
+    y = x.new_empty((steps, batch, width))
+    yt, yb = batch * width, width
+    if batch_first:
+        steps, batch, xt, xb, yt, yb = batch, steps, xb, xt, yb, yt
     device = x.device
     marks_bytes, work_bytes = _recurrence_sizes(steps, batch, width)
-    y = torch.empty(x.shape[:2] + (width,), dtype=x.dtype, device=device)
-    last = torch.empty((batch, width), dtype=torch.float32, device=device)
-    marks = torch.empty(marks_bytes // 4, dtype=torch.float32, device=device) if keep else None
-    work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
-    xs, ys = x.stride(), y.stride()
+    last = x.new_empty((batch, width), dtype=torch.float32)
+    marks = x.new_empty(marks_bytes // 4, dtype=torch.float32) if keep else None
+    work = x.new_empty(work_bytes, dtype=torch.uint8) if work_bytes else None
     with _on(device):
         check(library().mf_recurrence(
-            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xs[t], xs[b], _ptr(state),
-            _ptr(lengths), reverse, tanh, y.data_ptr(), ys[t], ys[b], last.data_ptr(), _ptr(marks),
+            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xt, xb, _ptr(state),
+            _ptr(lengths), bool(reverse), tanh, y.data_ptr(), yt, yb, last.data_ptr(), _ptr(marks),
             _ptr(work), work_bytes, _stream(device)), "recurrence")
     return y, last, marks
 
 
 def recurrence_grad(x, lengths, reverse, tanh, batch_first, marks, dy, dlast, with_state):
     """Gradients of ``recurrence``'s x and (``with_state``) state (mf_recurrence_grad)."""
-    t, b = (1, 0) if batch_first else (0, 1)
-    steps, batch, width = x.shape[t], x.shape[b], x.shape[2] // 2
+    (steps, batch, width), (xt, xb, _) = x.shape, x.stride()
+    yt, yb = (0, 0) if dy is None else dy.stride()[:2]
+    dt, db = batch * width, width
+    width //= 2
+    if batch_first:
+        steps, batch, xt, xb, yt, yb, dt, db = batch, steps, xb, xt, yb, yt, db, dt
     device = x.device
     work_bytes = _recurrence_sizes(steps, batch, width)[1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-    dstate = torch.empty((batch, width), dtype=torch.float32, device=device) if with_state else None
-    work = torch.empty(work_bytes, dtype=torch.uint8, device=device) if work_bytes else None
-    xs, ds, ys = x.stride(), dx.stride(), (0, 0) if dy is None else dy.stride()
+    dx = x.new_empty(x.shape)
+    dstate = x.new_empty((batch, width), dtype=torch.float32) if with_state else None
+    work = x.new_empty(work_bytes, dtype=torch.uint8) if work_bytes else None
     with _on(device):
         check(library().mf_recurrence_grad(
-            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xs[t], xs[b], _ptr(lengths),
-            reverse, tanh, marks.data_ptr(), _ptr(dy), ys[t], ys[b], _ptr(dlast), dx.data_ptr(), ds[t],
-            ds[b], _ptr(dstate), _ptr(work), work_bytes, _stream(device)), "recurrence gradient")
+            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xt, xb, _ptr(lengths),
+            reverse, tanh, marks.data_ptr(), _ptr(dy), yt, yb, _ptr(dlast), dx.data_ptr(), dt,
+            db, _ptr(dstate), _ptr(work), work_bytes, _stream(device)), "recurrence gradient")
     return dx, dstate
 
 
@@ -1740,8 +1745,8 @@ def int4_linear(x, codes, scales, zeros, o, group, bias):
     kind, at, ldx, device = FLOAT_TYPES[x.dtype], x.data_ptr(), x.stride(0), x.device
     pieces = at % 16 == 0 and ldx * x.element_size() % 16 == 0
     size = _int4_workspace(kind, n, k, o, group, pieces)
-    out = torch.empty((n, o), dtype=x.dtype, device=device)
-    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    out = x.new_empty((n, o))
+    work = x.new_empty(size, dtype=torch.uint8) if size else None
     with _on(device):
         check(library().mf_int4_linear(
             at, kind, n, k, ldx, codes.data_ptr(), scales.data_ptr(), FLOAT_TYPES[scales.dtype],

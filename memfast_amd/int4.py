@@ -31,11 +31,16 @@ def _check_sizes(o, k):
         raise NotImplementedError(f"more than {MOST_OUTPUTS} outputs or {MOST_INPUTS} inputs")
 
 
-def _part(label, value, dtypes, shape):
+_WHOLE, _FLOATING = (torch.uint8,), tuple(hip.FLOAT_TYPES)
+
+
+def _part(label, value, dtypes, shape, device):
     if not isinstance(value, torch.Tensor) or value.dtype not in dtypes:
         raise TypeError(f"{label} must be a tensor of {' or '.join(str(d)[6:] for d in dtypes)}")
     if value.shape != shape:
-        raise ValueError(f"{label} must have shape {tuple(shape)}")
+        raise ValueError(f"{label} must have shape {shape}")
+    if value.device != device:
+        raise ValueError(f"codes and {label} must use the same device")
     if not value.is_contiguous():
         value = value.contiguous()
     return value if value.data_ptr() % 16 == 0 else value.clone()
@@ -64,15 +69,14 @@ class Int4Tensor:
         o, k = shape
         self.group = _check_group(group)
         _check_sizes(o, k)
-        tiles, groups = -(-o // hip.INT4_TILE), -(-k // group)
-        self.codes = _part("codes", codes, (torch.uint8,),
-                           (tiles, -(-k // hip.INT4_SPAN), hip.INT4_TILE_BYTES))
-        self.scales = _part("scales", scales, tuple(hip.FLOAT_TYPES), (tiles, groups, hip.INT4_TILE))
-        self.zeros = None if zeros is None else _part("zeros", zeros, (torch.uint8,),
-                                                      (tiles, groups, hip.INT4_TILE))
-        for label, value in (("scales", scales), ("zeros", zeros)):
-            if value is not None and value.device != codes.device:
-                raise ValueError(f"codes and {label} must use the same device")
+        if not isinstance(codes, torch.Tensor):
+            raise TypeError("codes must be a tensor of uint8")
+        tiles, device = -(-o // hip.INT4_TILE), codes.device
+        table = (tiles, -(-k // group), hip.INT4_TILE)
+        self.codes = _part("codes", codes, _WHOLE, (tiles, -(-k // hip.INT4_SPAN), hip.INT4_TILE_BYTES),
+                           device)
+        self.scales = _part("scales", scales, _FLOATING, table, device)
+        self.zeros = None if zeros is None else _part("zeros", zeros, _WHOLE, table, device)
 
     @classmethod
     def pack(cls, codes, scales, *, group, zeros=None):

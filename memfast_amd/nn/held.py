@@ -1,6 +1,5 @@
 """Linear layers whose weight is held in 4-bit whole numbers (memfast_amd/int4.py)."""
 
-import torch
 from torch import nn
 
 from ..int4 import Int4Tensor, int4_linear, int4_quantize
@@ -37,11 +36,9 @@ class Int4Linear(nn.Module):
         self.register_buffer("bias", None if bias is None else bias.detach().clone())
 
     def forward(self, x):
-        weight = Int4Tensor(self.codes, self.scales, (self.out_features, self.in_features),
-                            group=self.group, zeros=self.zeros)
-        # Operands keep their dtypes under autocast, as the analog layers' do.
-        with torch.autocast(device_type=x.device.type, enabled=False):
-            return int4_linear(x, weight, self.bias)
+        # No operation of it is subject to autocast: operands keep their dtypes, as the analog layers' do.
+        return int4_linear(x, Int4Tensor(self.codes, self.scales, (self.out_features, self.in_features),
+                                         group=self.group, zeros=self.zeros), self.bias)
 
     def extra_repr(self):
         return (f"in_features={self.in_features}, out_features={self.out_features}, "

@@ -70,50 +70,54 @@ def gated_recurrence(projected, state=None, *, activation="tanh", lengths=None, 
     _check_floating("projected", projected)
     if activation not in ACTIVATIONS:
         raise ValueError("activation must be 'tanh' or None")
-    if projected.ndim not in (2, 3) or projected.shape[-1] % 2:
-        raise ValueError("projected must be [T, B, 2H], [B, T, 2H] or [T, 2H]")
     single = projected.ndim == 2
+    if projected.shape[-1] % 2 if single or projected.ndim == 3 else True:
+        raise ValueError("projected must be [T, B, 2H], [B, T, 2H] or [T, 2H]")
     x = projected.unsqueeze(1) if single else projected
     batch_first = bool(batch_first) and not single
-    t, b = (1, 0) if batch_first else (0, 1)
-    steps, batch, width = x.shape[t], x.shape[b], x.shape[2] // 2
+    steps, batch, width = x.shape
+    if batch_first:
+        steps, batch = batch, steps
+    width //= 2
     if steps > MOST_STEPS or batch > MOST_STEPS or width > MOST_WIDTH:
         raise NotImplementedError(f"more than {MOST_STEPS} steps or sequences or {MOST_WIDTH} channels")
+    device, start = projected.device, state
     if state is not None:
         _check_floating("state", state)
         if state.shape != ((width,) if single else (batch, width)):
             raise ValueError("state must have one value per sequence and channel")
         if state.dtype not in (torch.float32, projected.dtype):
             raise ValueError("state must be float32 or of the input's dtype")
-        if state.device != projected.device:
+        if state.device != device:
             raise ValueError("projected and state must use the same device")
+        if single:
+            start = start.unsqueeze(0)
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int64, torch.int32):
             raise TypeError("lengths must be an int64 or int32 tensor")
         if lengths.shape != (() if single else (batch,)):
             raise ValueError("lengths must have one value per sequence")
-        if lengths.device != projected.device:
+        if lengths.device != device:
             raise ValueError("projected and lengths must use the same device")
+        lengths = lengths.reshape(-1).to(torch.int64).contiguous()
     _refuse_tangents("gated_recurrence", projected, state)
     hip.require_device(projected)
-    start = None if state is None else (state.unsqueeze(0) if single else state).to(torch.float32)
-    if x.numel() == 0:
+    if start is not None and (start.dtype != torch.float32 or not start.is_contiguous()):
+        start = start.to(torch.float32).contiguous()
+    if steps == 0 or batch == 0 or width == 0:
         # No step to take, or no channel: states without values and the state that came in.
         y = x[..., :width] * 1
         last = start.clone() if start is not None else \
-            torch.zeros((batch, width), dtype=torch.float32, device=x.device)
+            torch.zeros((batch, width), dtype=torch.float32, device=device)
     else:
         if x.stride(2) != 1:
             x = x.contiguous()
-        if start is not None and not start.is_contiguous():
-            start = start.contiguous()
-        if lengths is not None:
-            lengths = lengths.reshape(-1).to(torch.int64).contiguous()
-        reverse, tanh = bool(reverse), activation == "tanh"
         if torch.is_grad_enabled() and (x.requires_grad or start is not None and start.requires_grad):
-            y, last = _Recurrence.apply(x, start, lengths, reverse, tanh, batch_first)
+            y, last = _Recurrence.apply(x, start, lengths, bool(reverse), activation is not None,
+                                        batch_first)
         else:
-            y, last, _ = hip.recurrence(x, start, lengths, reverse, tanh, batch_first, False)
+            y, last, _ = hip.recurrence(x, start, lengths, reverse, activation is not None, batch_first,
+                                        False)
     return (y.squeeze(1), last.squeeze(0)) if single else (y, last)
 
 
