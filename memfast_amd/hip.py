@@ -312,6 +312,19 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+def _launch(entry, device, what, *args):
+    """Calls a library entry on the current stream of ``device``, its last argument, and checks the status.
+    One frame of Python where ``_on`` and ``_stream`` take ten: the host's work is most of a small call."""
+    index = device.index
+    if _raw_stream is not None and _get_device is not None and index == _get_device():
+        status = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = entry(*args, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        check(status, what)
+
+
 def require_device(tensor):
     if not tensor.is_cuda:
         raise BackendError("memfast_amd kernels run on HIP devices only (tensor is on CPU)")
@@ -1653,11 +1666,10 @@ def recurrence(x, state, lengths, reverse, tanh, batch_first, keep):
     last = x.new_empty((batch, width), dtype=torch.float32)
     marks = x.new_empty(marks_bytes // 4, dtype=torch.float32) if keep else None
     work = x.new_empty(work_bytes, dtype=torch.uint8) if work_bytes else None
-    with _on(device):
-        check(library().mf_recurrence(
-            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xt, xb, _ptr(state),
-            _ptr(lengths), bool(reverse), tanh, y.data_ptr(), yt, yb, last.data_ptr(), _ptr(marks),
-            _ptr(work), work_bytes, _stream(device)), "recurrence")
+    _launch(library().mf_recurrence, device, "recurrence", x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch,
+            width, xt, xb, None if state is None else state.data_ptr(),
+            None if lengths is None else lengths.data_ptr(), bool(reverse), tanh, y.data_ptr(), yt, yb,
+            last.data_ptr(), _ptr(marks), _ptr(work), work_bytes)
     return y, last, marks
 
 
@@ -1674,11 +1686,9 @@ def recurrence_grad(x, lengths, reverse, tanh, batch_first, marks, dy, dlast, wi
     dx = x.new_empty(x.shape)
     dstate = x.new_empty((batch, width), dtype=torch.float32) if with_state else None
     work = x.new_empty(work_bytes, dtype=torch.uint8) if work_bytes else None
-    with _on(device):
-        check(library().mf_recurrence_grad(
-            x.data_ptr(), FLOAT_TYPES[x.dtype], steps, batch, width, xt, xb, _ptr(lengths),
-            reverse, tanh, marks.data_ptr(), _ptr(dy), yt, yb, _ptr(dlast), dx.data_ptr(), dt,
-            db, _ptr(dstate), _ptr(work), work_bytes, _stream(device)), "recurrence gradient")
+    _launch(library().mf_recurrence_grad, device, "recurrence gradient", x.data_ptr(), FLOAT_TYPES[x.dtype],
+            steps, batch, width, xt, xb, _ptr(lengths), reverse, tanh, marks.data_ptr(), _ptr(dy), yt, yb,
+            _ptr(dlast), dx.data_ptr(), dt, db, _ptr(dstate), _ptr(work), work_bytes)
     return dx, dstate
 
 
@@ -1689,12 +1699,11 @@ def dropout(x, residual, dropped, seed, event):
     """Dropout of ``x``, contiguous, added to ``residual`` if there is one (mf_dropout).  ``event`` is
     a number or an int64 tensor of one value on x's device."""
     out = torch.empty_like(x)
-    held = isinstance(event, torch.Tensor)
-    with _on(x.device):
-        check(library().mf_dropout(
-            x.data_ptr(), FLOAT_TYPES[x.dtype], x.numel(), _ptr(residual), dropped, seed,
-            0 if held else event, event.data_ptr() if held else None, out.data_ptr(),
-            _stream(x.device)), "dropout")
+    at = None
+    if isinstance(event, torch.Tensor):
+        event, at = 0, event.data_ptr()
+    _launch(library().mf_dropout, x.device, "dropout", x.data_ptr(), FLOAT_TYPES[x.dtype], x.numel(),
+            None if residual is None else residual.data_ptr(), dropped, seed, event, at, out.data_ptr())
     return out
 
 
@@ -1747,11 +1756,9 @@ def int4_linear(x, codes, scales, zeros, o, group, bias):
     size = _int4_workspace(kind, n, k, o, group, pieces)
     out = x.new_empty((n, o))
     work = x.new_empty(size, dtype=torch.uint8) if size else None
-    with _on(device):
-        check(library().mf_int4_linear(
-            at, kind, n, k, ldx, codes.data_ptr(), scales.data_ptr(), FLOAT_TYPES[scales.dtype],
-            _ptr(zeros), o, group, _ptr(bias), out.data_ptr(), _ptr(work), size, _stream(device)),
-            "4-bit product")
+    _launch(library().mf_int4_linear, device, "4-bit product", at, kind, n, k, ldx, codes.data_ptr(),
+            scales.data_ptr(), FLOAT_TYPES[scales.dtype], _ptr(zeros), o, group, _ptr(bias), out.data_ptr(),
+            _ptr(work), size)
     return out
 
 

@@ -18,19 +18,23 @@ MOST_VALUES = 1 << 40
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, dropped, seed, event):
-        held = isinstance(event, torch.Tensor)
-        ctx.save_for_backward(event if held else None)
-        ctx.options = dropped, seed, None if held else event
+        if isinstance(event, torch.Tensor):
+            ctx.save_for_backward(event)
+            ctx.options = dropped, seed, None
+        else:
+            ctx.options = dropped, seed, event
         return hip.dropout(x, residual, dropped, seed, event)
 
     @staticmethod
     def backward(ctx, dy):
         dropped, seed, event = ctx.options
-        event = ctx.saved_tensors[0] if event is None else event
+        if event is None:
+            event, = ctx.saved_tensors
+        wants_x, wants_residual = ctx.needs_input_grad[:2]
         dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _apply(dy.contiguous(), None, dropped, seed, event)   # linear in dy: differentiable again
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        if wants_x:     # linear in dy: the mask once more, and differentiable again
+            dx = _apply(dy if dy.is_contiguous() else dy.contiguous(), None, dropped, seed, event)
+        return dx, dy if wants_residual else None, None, None, None
 
 
 def _apply(x, residual, dropped, seed, event):
