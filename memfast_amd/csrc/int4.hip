@@ -285,42 +285,57 @@ struct PrepareArgs {
     u16 *planes;        // [TERMS, n, 128 spans], or nullptr: x is taken as it is
 };
 
-// One wave takes a span of a row, two inputs a lane.
-template <typename T> __global__ __launch_bounds__(256) void k_int4_prepare(const PrepareArgs a) {
+// A workgroup takes 16 spans of a row, a lane eight inputs. Bound by its bytes and launch: 2048 x 4096 BF16 in
+// PREPARE_US us.
+template <typename T, bool PIECES> __global__ __launch_bounds__(256) void k_int4_prepare(const PrepareArgs a) {
     typedef typename std::conditional<std::is_same<T, float>::value, bf16, T>::type Term;
     constexpr int TERMS = Operand<T>::TERMS;
-    const int lane = threadIdx.x & 63;
-    const i64 all = a.pitch * a.spans;
-    for (i64 id = i64(blockIdx.x) * 4 + (threadIdx.x >> 6); id < all; id += i64(gridDim.x) * 4) {
-        const i64 n = id / a.spans, span = id - n * a.spans;
-        float sum = 0.0f;
-        if (n < a.n)
+    const i64 n = blockIdx.y, span = i64(blockIdx.x) * 16 + (threadIdx.x >> 4);
+    const int piece = threadIdx.x & 15;
+    if (span >= a.spans) return;
+    Eight<T> x;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const i64 k = span * SPAN_K + lane * 2 + i;
-                const T x = k < a.k ? static_cast<const T *>(a.x)[n * a.ldx + k] : T(0.0f);
-                sum += float(x);
-                if (a.planes) {
-                    float rest = float(x);
+    for (int i = 0; i < 8; ++i) x.v[i] = T(0.0f);
+    if (n < a.n) {
+        const i64 k = span * SPAN_K + piece * 8;
+        const T *row = static_cast<const T *>(a.x) + n * a.ldx;
+        if (PIECES && k + 8 <= a.k) {
+            x.load(row + k);
+        } else {
 #pragma unroll
-                    for (int t = 0; t < TERMS; ++t) {
-                        const float high = TERMS == 1 ? rest : upper(rest);
-                        const Term term = Term(high);
-                        a.planes[(t * a.n + n) * a.spans * SPAN_K + k] = __builtin_bit_cast(u16, term);
-                        rest -= high;
-                    }
+            for (int i = 0; i < 8; ++i)
+                if (k + i < a.k) x.v[i] = row[k + i];
+        }
+        if (a.planes) {
+            alignas(16) Term terms[TERMS][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float rest = float(x.v[i]);
+#pragma unroll
+                for (int t = 0; t < TERMS; ++t) {
+                    const float high = TERMS == 1 ? rest : upper(rest);
+                    terms[t][i] = Term(high);
+                    rest -= high;
                 }
             }
-        if (!a.sums) continue;
 #pragma unroll
-        for (int d = 1; d <= 8; d <<= 1) sum += __shfl_xor(sum, d);
-        if (a.per == 1) {
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (lane == 0) a.sums[span * a.pitch + n] = a.factor * sum;
-        } else if ((lane & 15) == 0) {
-            a.sums[(span * 4 + lane / 16) * a.pitch + n] = a.factor * sum;
+            for (int t = 0; t < TERMS; ++t)
+                *reinterpret_cast<v4u *>(a.planes + ((t * a.n + n) * a.spans * SPAN_K + k)) =
+                    *reinterpret_cast<const v4u *>(terms[t]);
         }
+    }
+    if (!a.sums) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += float(x.v[i]);
+    sum += __shfl_xor(sum, 1);
+    sum += __shfl_xor(sum, 2);
+    if (a.per == 1) {
+        sum += __shfl_xor(sum, 4);
+        sum += __shfl_xor(sum, 8);
+        if (piece == 0) a.sums[span * a.pitch + n] = a.factor * sum;
+    } else if ((piece & 3) == 0) {
+        a.sums[(span * 4 + piece / 4) * a.pitch + n] = a.factor * sum;
     }
 }
 
@@ -652,9 +667,10 @@ constexpr i64 ROWS_AT_ONCE = 8192;
 struct HeldPlan {
     enum { FEW, MID, LARGE } kernel;
     bool direct;            // x is read as it is
+    int32_t type;
     int per, terms;
     i64 rows, pitch, spans, sums, planes, splits = 1, share, bytes;
-    HeldPlan(int32_t type, i64 n, i64 k, i64 o, i64 group, bool pieces) {
+    HeldPlan(int32_t type, i64 n, i64 k, i64 o, i64 group, bool pieces) : type(type) {
         spans = share = (k + SPAN_K - 1) / SPAN_K;
         per = group >= SPAN_K ? 1 : 4;
         terms = type == MF_F32 ? 3 : 1;
@@ -760,9 +776,9 @@ int launch_tiles(HeldArgs a, const HeldPlan &plan, void *workspace, hipStream_t 
         }
         int status = MF_OK;
         if (table || !plan.direct) {
-            hipLaunchKernelGGL(k_int4_prepare<T>,
-                               dim3(u32(std::min<i64>((p.pitch * p.spans + 3) / 4, 1 << 16))), dim3(256), 0,
-                               s, p);
+            const auto prepare = rows_in_pieces(a.x, a.ldx, plan.type) ? k_int4_prepare<T, true>
+                                                                        : k_int4_prepare<T, false>;
+            hipLaunchKernelGGL(prepare, dim3(u32((a.spans + 15) / 16), u32(p.pitch)), dim3(256), 0, s, p);
             status = check_launch("4-bit product's rows");
         }
         if (!status) status = table ? launch_large<T, S>(t, plan.per, s) : launch_mid<T, S>(t, plan.per, s);
