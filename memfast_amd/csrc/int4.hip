@@ -286,7 +286,7 @@ struct PrepareArgs {
 };
 
 // A workgroup takes 16 spans of a row, a lane eight inputs. Bound by its bytes and launch: 2048 x 4096 BF16 in
-// PREPARE_US us.
+// 5 us (17 MB).
 template <typename T, bool PIECES> __global__ __launch_bounds__(256) void k_int4_prepare(const PrepareArgs a) {
     typedef typename std::conditional<std::is_same<T, float>::value, bf16, T>::type Term;
     constexpr int TERMS = Operand<T>::TERMS;
