@@ -3,11 +3,11 @@
 Bounds.  With e = 2^-24: sigmoid(g) and its complement come from exp2 and rcp (each within an ulp, 2 e), an
 argument whose rounding is made good but for log2(e)'s own (e |g| / 4), a sum and a product, so within 12 e
 for |g| below 20, beyond which the smaller of them is nothing beside the other's term; tanh above 1/4 is
-1 - 2 r with r = 1 / (1 + x) and x = exp(2 v), r below 0.38 or near 1 within 4 e, so within 2 * 0.76 * 4 e / 0.25
-< 13 e of a small result and 8 e of a large one, and the series below 1/4 within less.  A step
-u h + k c adds at most (12 + 2) e u|h| + (12 + 13 + 2) e k|c| and the joined maps of eight steps, sixteen
-waves and the segments one rounding of A and one of S more for each step that they stand for; C = 32 covers
-both.  The bound of h is therefore itself a recurrence, E_t = u_t E_{t-1} + C e (u_t|h_{t-1}| + k_t|c_t|), that of
+1 - 2 r with r = 1 / (1 + x) and x = exp(2 v): r is below 0.63 beside 1/4 and within 5 e, so the difference
+within 2 * 0.63 * 5 e / 0.245 < 27 e, and the series below 1/4 within less.  A step u h + k c adds at most
+(12 + 2) e u|h| + (12 + 27 + 2) e k|c|, and the joined maps of sixteen steps, eight waves and the segments
+one rounding of A and one of S more for each step that they stand for: 2 C = 64 covers both, where C stands
+in the recurrences of the bounds and near() takes them twice.  The bound of h is therefore itself a recurrence, E_t = u_t E_{t-1} + C e (u_t|h_{t-1}| + k_t|c_t|), that of
 G is F_t = |dy| C e + u_{t+1} F_{t+1} + C e u_{t+1}|G_{t+1}|, and the gradients' bounds follow by the product
 rule.  A result of a 16-bit type is off by half a step more.
 """
