@@ -834,7 +834,7 @@ int mf_int4_quantize(const void *w, int32_t type, int64_t o, int64_t k, int64_t 
     HeldArgs h{};
     const int status = check_held(codes, scales, scale_type, nullptr, o, k, group, h);
     if (status) return status;
-    if (!w || !known_type(type) || ldw < k || !aligned(w, type_bytes(type)))
+    if (!w || !known_type(type) || ldw < 0 || (o > 1 && ldw < k) || !aligned(w, type_bytes(type)))
         return fail(MF_E_INVALID, "invalid 4-bit quantization arguments");
     const Int4QuantizeArgs a{w, o, k, ldw, h.groups, h.spans, h.shift, codes, scales};
     const i64 units = (o + TILE - 1) / TILE * TILE * h.groups;

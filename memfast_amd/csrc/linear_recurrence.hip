@@ -515,8 +515,9 @@ int mf_recurrence(const void *x, int32_t type, int64_t steps, int64_t batch, int
                   int64_t bytes, void *stream) {
     const int status = check_recurrence(x, type, steps, batch, width, xt, xb);
     if (status) return status;
-    if (!y || !last || yt < 0 || yb < 0 || !aligned(y, type_bytes(type)))
-        return fail(MF_E_INVALID, "invalid recurrence outputs");
+    if (!y || !last || yt < 0 || yb < 0 || !aligned(y, type_bytes(type)) || !aligned(state, 4) ||
+        !aligned(lengths, 8) || !aligned(last, 4) || !aligned(marks, 4) || !aligned(workspace, 8))
+        return fail(MF_E_INVALID, "invalid recurrence operands");
     const Split split(steps, batch, width);
     if (bytes < split.bytes(batch, width) || (split.segments > 1 && !workspace))
         return fail(MF_E_INVALID, "recurrence workspace of %lld bytes", (long long)bytes);
@@ -558,7 +559,8 @@ int mf_recurrence_grad(const void *x, int32_t type, int64_t steps, int64_t batch
     const int status = check_recurrence(x, type, steps, batch, width, xt, xb);
     if (status) return status;
     if (!marks || !dx || dt < 0 || db < 0 || yt < 0 || yb < 0 || !aligned(dx, type_bytes(type)) ||
-        !aligned(dy, type_bytes(type)))
+        !aligned(dy, type_bytes(type)) || !aligned(lengths, 8) || !aligned(marks, 4) || !aligned(dlast, 4) ||
+        !aligned(dstate, 4) || !aligned(workspace, 8))
         return fail(MF_E_INVALID, "invalid recurrence gradient arguments");
     const Split split(steps, batch, width);
     if (bytes < split.bytes(batch, width) || (split.segments > 1 && !workspace))

@@ -1724,8 +1724,8 @@ def int4_quantize(weight, group, scale_type):
     if weight.numel():
         with _on(weight.device):
             check(library().mf_int4_quantize(
-                _ptr(weight), FLOAT_TYPES[weight.dtype], o, k, weight.stride(0), group, _ptr(codes),
-                _ptr(scales), FLOAT_TYPES[scale_type], _stream(weight.device)), "4-bit quantization")
+                _ptr(weight), FLOAT_TYPES[weight.dtype], o, k, weight.stride(0) if o > 1 else k, group,
+                _ptr(codes), _ptr(scales), FLOAT_TYPES[scale_type], _stream(weight.device)), "4-bit quantization")
     return codes, scales
 
 
@@ -1751,7 +1751,8 @@ def _int4_workspace(kind, n, k, o, group, pieces):
 def int4_linear(x, codes, scales, zeros, o, group, bias):
     """``x W^T + bias`` [n, o] for ``x`` [n, k] and a held W (mf_int4_linear)."""
     n, k = x.shape
-    kind, at, ldx, device = FLOAT_TYPES[x.dtype], x.data_ptr(), x.stride(0), x.device
+    kind, at, device = FLOAT_TYPES[x.dtype], x.data_ptr(), x.device
+    ldx = x.stride(0) if n > 1 else k       # one row's own distance may be any
     pieces = at % 16 == 0 and ldx * x.element_size() % 16 == 0
     size = _int4_workspace(kind, n, k, o, group, pieces)
     out = x.new_empty((n, o))

@@ -167,9 +167,10 @@ def int4_linear(x, weight, bias=None):
         raise ValueError("x and weight have incompatible reduction dimensions")
     if bias is not None and bias.shape != (o,):
         raise ValueError("bias must have one value per output")
-    if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.scales.requires_grad or
+                                    bias is not None and bias.requires_grad):
         raise NotImplementedError("int4_linear has no gradient; call it under torch.no_grad()")
-    _refuse_tangents("int4_linear", x, bias)
+    _refuse_tangents("int4_linear", x, weight.scales, bias)
     hip.require_device(x)
     shape = x.shape[:-1] + (o,)
     if x.numel() == 0 or o == 0:

@@ -9,32 +9,22 @@ import torch
 from torch import nn
 
 from ..recurrence import ACTIVATIONS, gated_recurrence
-from ..regularization import _check_probability, _number, dropout
+from ..regularization import _check_probability, dropout
 
 
 class Dropout(nn.Module):
-    """Dropout by ``memfast_amd.dropout``: each forward in training mode is the next event of ``seed``
-    (drawn from torch's default generator where none is given).  ``seed`` and ``event`` are part of the
-    state, so a restored model goes on with the masks that it would have had."""
+    """Dropout by ``memfast_amd.dropout``, each forward in training mode with a seed that it draws from torch's
+    default CPU generator: ``torch.manual_seed`` makes the masks again, and so does a checkpointed
+    layer's second forward, for which torch restores the generator.  A captured graph keeps the one mask of
+    its capture; ``memfast_amd.dropout`` with an event on the device makes new ones."""
 
-    def __init__(self, p=0.5, *, seed=None):
+    def __init__(self, p=0.5):
         super().__init__()
         self.p = _check_probability(p)
-        self.seed = int(torch.randint(1 << 62, ())) if seed is None else _number("seed", seed)
-        self.event = 0
 
     def forward(self, x, residual=None):
-        event = self.event
-        if self.training:
-            self.event += 1
-        return dropout(x, self.p, seed=self.seed, event=event, residual=residual,
-                       training=self.training)
-
-    def get_extra_state(self):
-        return {"seed": self.seed, "event": self.event}
-
-    def set_extra_state(self, state):
-        self.seed, self.event = _number("seed", state["seed"]), _number("event", state["event"])
+        seed = int(torch.randint(1 << 62, ())) if self.training and self.p else 0
+        return dropout(x, self.p, seed=seed, residual=residual, training=self.training)
 
     def extra_repr(self):
         return f"p={self.p}"

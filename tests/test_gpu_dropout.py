@@ -209,14 +209,32 @@ def test_second_derivatives_and_checkpoints(hip_device):
 
 
 def test_layer(hip_device):
-    layer = Dropout(0.3, seed=77).to(hip_device)
-    x = torch.randn(100, device=hip_device)
+    """Masks come from torch's default generator, one seed a forward."""
+    layer = Dropout(0.3).to(hip_device)
+    x = torch.randn(4000, device=hip_device)
+    torch.manual_seed(5)
     outputs = [layer(x) for _ in range(3)]
-    for event, y in enumerate(outputs):
-        assert torch.equal(y, memfast.dropout(x, 0.3, seed=77, event=event))
-    other = Dropout(0.3)
-    other.load_state_dict(layer.state_dict())
-    assert torch.equal(other(x), layer(x))
+    torch.manual_seed(5)
+    for y in outputs:
+        seed = int(torch.randint(1 << 62, ()))
+        assert torch.equal(y, memfast.dropout(x, 0.3, seed=seed))
+    assert not torch.equal(outputs[0], outputs[1])
+    r = torch.randn_like(x)
+    torch.manual_seed(5)
+    assert torch.equal(layer(x, residual=r) == r, outputs[0] == 0)
     layer.eval()
-    assert layer(x) is x and layer.event == 4
-    assert torch.equal(layer(x, residual=x), x + x)
+    before = torch.get_rng_state()
+    assert layer(x) is x and torch.equal(layer(x, residual=r), r + x)
+    assert torch.equal(torch.get_rng_state(), before)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_layer_keeps_its_mask(hip_device, reentrant):
+    """The second forward, in the backward, drops what the first one dropped."""
+    layer = Dropout(0.5).to(hip_device)
+    x = torch.ones(3000, device=hip_device, requires_grad=True)
+    for _ in range(2):
+        y = torch.utils.checkpoint.checkpoint(lambda v: layer(v * v), x, use_reentrant=reentrant)
+        x.grad = None
+        y.sum().backward()
+        assert torch.equal(x.grad != 0, y != 0)

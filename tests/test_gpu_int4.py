@@ -175,6 +175,28 @@ def test_values_that_are_not_finite(hip_device):
             assert torch.equal(y[rest][:, others], fine[rest][:, others])
 
 
+def test_one_row_of_any_distance(hip_device):
+    flat = torch.randn(64, device=hip_device)
+    q, s, z, held = weight(hip_device, 20, 64, 32, torch.float32, False)
+    one = flat.as_strided((1, 64), (1, 1))
+    assert torch.equal(memfast.int4_linear(one, held), memfast.int4_linear(flat, held)[None])
+    assert torch.equal(memfast.int4_quantize(one).codes, memfast.int4_quantize(flat[None]).codes)
+
+
+def test_subnormal_inputs(hip_device):
+    """FP16's subnormal numbers, and FP32 numbers whose lower terms are far below, count."""
+    for n in (1, 40, 150):
+        for o in (40, 6000):
+            q, s, z, held = weight(hip_device, o, 256, 32, torch.float32, False)
+            x = (torch.randint(-8, 9, (n, 256)).float() * 2.0**-24).half().to(hip_device)
+            y, terms = expected(x, q, s, z, 32, None)
+            got = memfast.int4_linear(x, held)
+            assert bool(((got.double().cpu() - y).abs() <= 2.0**-25 + 2.0**-12 * terms).all())
+            assert float(y.abs().max()) > 2.0**-22
+            x = torch.randn(n, 256, device=hip_device) * 2.0**-90
+            near(memfast.int4_linear(x, held), *expected(x, q, s, z, 32, None), 256, 32)
+
+
 def test_exact_sums(hip_device):
     """Whole numbers whose sums fit FP32 come out exactly, in every type, whatever is split."""
     for kind in TYPES:

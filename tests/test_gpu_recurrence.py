@@ -405,7 +405,10 @@ def test_layer(hip_device, first, both):
     x = torch.randn(4, 30, 12, device=hip_device) if first else torch.randn(30, 4, 12, device=hip_device)
     lengths = torch.tensor([30, 7, 0, 12], device=hip_device)
     hx = torch.randn(2 * ways, 4, 10, device=hip_device)
+    torch.manual_seed(4)
     y, last = layer(x, hx, lengths)
+    torch.manual_seed(4)
+    seed = int(torch.randint(1 << 62, ()))
     h, finals = x, []
     for n in range(2):
         outputs = []
@@ -418,13 +421,12 @@ def test_layer(hip_device, first, both):
             finals.append(final)
         h = torch.cat(outputs, -1)
         if n == 0:
-            h = memfast.dropout(h, 0.25, seed=layer.dropouts[0].seed, event=0)
+            h = memfast.dropout(h, 0.25, seed=seed)
     assert torch.equal(y, h) and torch.equal(last, torch.stack(finals))
-    assert layer.dropouts[0].event == 1
     y.sum().backward()
     assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in layer.parameters())
     layer.eval()
-    assert torch.equal(layer(x, hx, lengths)[0], layer(x, hx, lengths)[0]) and layer.dropouts[0].event == 1
+    assert torch.equal(layer(x, hx, lengths)[0], layer(x, hx, lengths)[0])
 
 
 def test_trained_held_and_stepped(hip_device):
@@ -477,5 +479,5 @@ def test_converted_projections(hip_device, training):
             y, _ = model(x)
         assert all(p._event == 1 for p in model.projections)
     # 8-bit operands: steps of 1/127 of a group's peak, sums of 32, two layers.
-    digital = layer(x)[0]
-    assert float((y - digital).abs().max()) < 0.15
+    digital = layer(x)[0].detach()
+    assert float((y.detach() - digital).abs().max()) < 0.15
