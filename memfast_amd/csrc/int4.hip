@@ -104,6 +104,9 @@ template <typename T> struct alignas(16) Eight {
     }
 };
 
+// The wave's number in its workgroup, the same for all its lanes.
+__device__ __forceinline__ int wave_of_workgroup() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // The four values that the quarters of a wave hold, each in all of them.
 __device__ __forceinline__ void quarters(float value, float (&all)[4]) {
     const u32 v = __float_as_uint(value);
@@ -119,12 +122,16 @@ __device__ __forceinline__ void quarters(float value, float (&all)[4]) {
 // the order of the waves.  Row 4 i + quarter of a block of 16 rows is row 4 quarter + i of the matrix
 // instruction, so that up to 4 rows need one register of its result and one scaling.  x is a multiple of
 // 8 inputs wide, in whole 16-byte pieces.  PER: scalings in a span, 1 for groups of 128 on, else 4.
+// 1 x 4096 x 11008 BF16, groups of 32, in 7.5 us (25 MB, 3.4 TB/s), 1 x 4096 x 4096, groups of 128, in 3.7, a
+// launch: bound by a wave's chain of four or five spans and the 57% of the time that the vector units take for
+// conversions and scalings. More rows read x again for every tile from the L2: 16 x 4096 x 11008 12 us. Waves
+// a workgroup: 4 / 8 / 16 for the first 7.7 / 7.4 / 8.8 us; x fetched with its span 7.6.
 template <typename T, typename S, int WAVES, int OT, int NB, int R, int PER, bool AHEAD>
 __global__ __launch_bounds__(64 * WAVES) void k_int4_few(const HeldArgs a) {
     typedef Operand<T> Op;
     constexpr int TERMS = Op::TERMS;
     extern __shared__ __align__(16) float sums[];   // [WAVES][OT * NB * R][64]
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
     const int quarter = lane >> 4, r = lane & 15;
     const int spans = int(a.spans), groups = int(a.groups), k = int(a.k);
     const i64 tiles = (a.o + TILE - 1) / TILE, tile0 = i64(blockIdx.x) * OT;
@@ -259,7 +266,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_int4_few(const HeldArgs a) {
     }
 }
 
-// Copies rows of x into rows of whole spans, with zeros past k: one wave a span, two inputs a lane.
+// Copies rows of x into rows of whole spans, with zeros past k: one wave a span, two inputs a lane. For few rows
+// that are not whole 16-byte pieces; bound by its launch.
 template <typename T>
 __global__ __launch_bounds__(256) void k_int4_pad(const T *x, i64 n, i64 k, i64 ldx, i64 spans, T *out) {
     const int lane = threadIdx.x & 63;
@@ -362,14 +370,19 @@ template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v1
 // span ahead.  With the sums' TABLE, sums over a group begin at -8 times the sum of x, so a zero point of 8
 // costs nothing; others (ZEROS) are taken off with one operation more a group and result.  Without it
 // a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for groups of 128 on, else 4.
+// 2048 x 4096 x 11008 BF16, groups of 128, in 181 us (1020 TFLOP/s): bound by the matrix cores, which take 182
+// with nothing but their instructions left; with tiles of 128 rows, one wave a SIMD, it takes 265, with the
+// whole span's codes converted first the same. Groups of 32, four scalings a span, 240: the vector units. In small
+// tiles a span's copies are waited for (24 x 11008 x 4096 FP16 11 us); four stages of them with the codes among
+// them leave one workgroup a compute unit and take 15.
 constexpr int TILE_WAVES = 4, BAND = 8;
 
 // Waves that a SIMD has to hold: with at most 256 registers each the matrix instructions' results stay where
 // the vector units reach them (else each is copied once more for its scaling).
-constexpr int tile_waves_per_simd(int nt, int no, int terms) { return nt * no == 1 ? 4 : nt * no == 2 ? 3 : 2; }
+constexpr int tile_waves_per_simd(int nt, int no) { return nt * no == 1 ? 4 : nt * no == 2 ? 3 : 2; }
 
 template <typename T, typename S, int NT, int NO, bool TABLE, bool ZEROS, int PER>
-__global__ __launch_bounds__(64 * TILE_WAVES, tile_waves_per_simd(NT, NO, Operand<T>::TERMS)) void
+__global__ __launch_bounds__(64 * TILE_WAVES, tile_waves_per_simd(NT, NO)) void
 k_int4_tile(const TileArgs t) {
     static_assert(TABLE || ZEROS, "sums that begin at 0 have the zero points taken off");
     typedef Operand<T> Op;
@@ -377,7 +390,7 @@ k_int4_tile(const TileArgs t) {
     constexpr int XBYTES = TERMS * ROWS * SPAN_K * 2, STAGE = XBYTES + (TABLE ? 2048 : 0);
     extern __shared__ __align__(16) u8 staged[];
     const HeldArgs &a = t.h;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = wave_of_workgroup();
     const int half = lane >> 5, row = lane & 31, r = lane & 15;
     const u32 tn = u32((a.n + ROWS - 1) / ROWS), to = u32((a.o + OUTPUTS - 1) / OUTPUTS);
     // Each XCD takes a run of tiles (xcd_tile), here in bands of BAND tiles of rows and all outputs, so that what
@@ -530,7 +543,7 @@ k_int4_tile(const TileArgs t) {
     }
 }
 
-// Adds the parts of a product in their order, and the bias.
+// Adds the parts of a product in their order, and the bias. Bound by its launch (2 to 4 us).
 template <typename T> __global__ __launch_bounds__(256) void k_int4_join(const TileArgs t) {
     const i64 all = t.h.n * t.h.o;
     for (i64 id = i64(blockIdx.x) * 256 + threadIdx.x; id < all; id += i64(gridDim.x) * 256) {
@@ -558,65 +571,101 @@ struct Int4QuantizeArgs {
     void *scales;
 };
 
-// One wave takes a group of one output: its peak, the scale peak / 7 in the scales' type, and the codes
-// round(w / scale) + 8.  The bytes of codes are joined by the lanes of their two inputs.
-template <typename T, typename S>
+// A wave works on 512 inputs of an output, eight a lane: the four bytes of codes that a lane's word of a tile is.
+constexpr int WAVE_INPUTS = 512;
+
+// Where the codes of output o and inputs k to k + 7 lie.
+__device__ __forceinline__ i64 word_of(i64 o, i64 k, i64 spans) {
+    const int in = int(k) & (SPAN_K - 1);
+    return ((o / TILE) * spans + (k >> 7)) * SPAN_BYTES + (in >> 3 & 3) * 256 + (o & 15) * 16 + (in >> 5) * 4;
+}
+
+// The peak of each group, the scale peak / 7 in the scales' type, and the codes round(w / scale) + 8. A group of more
+// than 512 inputs is read twice. It runs once a weight: 11008 x 4096 BF16 in 52 us (113 MB, 2.2 TB/s).
+// Its words are 16 bytes apart in a tile, which the L2 joins.
+template <typename T, typename S, bool PIECES>
 __global__ __launch_bounds__(256) void k_int4_quantize(const Int4QuantizeArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const i64 all = (a.o + TILE - 1) / TILE * TILE * a.groups;
-    for (i64 id = i64(blockIdx.x) * 4 + wave; id < all; id += i64(gridDim.x) * 4) {
-        const i64 o = id / a.groups, g = id - o * a.groups;
-        const i64 first = g << a.shift, last = min(first + (i64(1) << a.shift), a.k);
+    const int lane = threadIdx.x & 63;
+    const i64 step = std::max<i64>(WAVE_INPUTS, i64(1) << a.shift), padded = a.spans * SPAN_K;
+    const i64 chunks = (padded + step - 1) / step, all = (a.o + TILE - 1) / TILE * TILE * chunks;
+    const int lanes = a.shift >= 9 ? 64 : 1 << (a.shift - 3);       // of a group
+    for (i64 id = i64(blockIdx.x) * 4 + wave_of_workgroup(); id < all; id += i64(gridDim.x) * 4) {
+        const i64 o = id / chunks, first = (id - o * chunks) * step + lane * 8;
+        const i64 end = min(first - lane * 8 + step, padded);
         const T *w = static_cast<const T *>(a.w) + o * a.ldw;
+        Eight<T> v;
+        const auto load = [&](i64 k) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v.v[i] = T(0.0f);
+            if (o >= a.o) return;
+            if (PIECES && k + 8 <= a.k) {
+                v.load(w + k);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k + i < a.k) v.v[i] = w[k + i];
+            }
+        };
         float peak = 0.0f;
         bool bad = false;
-        if (o < a.o)
-            for (i64 k = first + lane; k < last; k += 64) {
-                const float v = fabsf(float(w[k]));
-                bad |= !(v <= FLT_MAX);
-                peak = fmaxf(peak, v);
-            }
+        for (i64 k = first; k < end; k += WAVE_INPUTS) {
+            load(k);
 #pragma unroll
-        for (int d = 32; d; d >>= 1) {
+            for (int i = 0; i < 8; ++i) {
+                const float size = fabsf(float(v.v[i]));
+                bad |= !(size <= FLT_MAX);
+                peak = fmaxf(peak, size);
+            }
+        }
+        for (int d = lanes >> 1; d; d >>= 1) {
             peak = fmaxf(peak, __shfl_xor(peak, d));
             bad |= __shfl_xor(int(bad), d) != 0;
         }
         S held = S(peak > 0.0f ? peak / 7.0f : 1.0f);
         if (peak > 0.0f && !(float(held) > 0.0f)) held = S(1.0f);     // beneath the type: codes of 0
         if (bad) held = S(NAN);
-        const float scale = float(held);
-        if (lane == 0) static_cast<S *>(a.scales)[(o / TILE * a.groups + g) * 16 + o % TILE] = o < a.o ? held : S(0.0f);
-        // Bytes hold inputs k and k + 4 of eight; zero codes' bytes past the last input are 8 twice.
-        const i64 end = g + 1 == a.groups ? a.spans * SPAN_K : last;
-        for (i64 p = (first >> 1) + lane; p < end >> 1; p += 64) {
-            const i64 k = (p >> 2) * 8 + (p & 3);
-            u32 byte = 0;
+        const i64 g = first >> a.shift;
+        if ((lane & (lanes - 1)) == 0 && g < a.groups)
+            static_cast<S *>(a.scales)[(o / TILE * a.groups + g) * 16 + (o & 15)] = o < a.o ? held : S(0.0f);
+        for (i64 k = first; k < end; k += WAVE_INPUTS) {
+            if (step > WAVE_INPUTS) load(k);
+            u32 word = 0;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float c = 0.0f;
-                if (o < a.o && k + 4 * i < last && !bad) c = rintf(float(w[k + 4 * i]) / scale);
+            for (int i = 0; i < 8; ++i) {
+                float c = bad ? 0.0f : rintf(float(v.v[i]) / float(held));
                 c = fminf(fmaxf(c, -8.0f), 7.0f);
-                byte |= u32(int(c) + 8) << (4 * i);
+                word |= u32(int(c) + 8) << (8 * (i & 3) + (i & 4));
             }
-            const i64 in = k & (SPAN_K - 1);
-            a.codes[((o / TILE) * a.spans + (k >> 7)) * SPAN_BYTES + (in >> 3 & 3) * 256 + o % TILE * 16 +
-                    (in >> 5) * 4 + (in & 3)] = u8(byte);
+            *reinterpret_cast<u32 *>(a.codes + word_of(o, k, a.spans)) = word;
         }
     }
 }
 
-// One lane restores one value.
-template <typename T, typename S>
+// A lane restores eight values: 11008 x 4096 to BF16 in 50 us.
+template <typename T, typename S, bool PIECES>
 __global__ __launch_bounds__(256) void k_int4_dequantize(const HeldArgs a) {
-    const i64 all = a.o * a.k;
-    for (i64 id = i64(blockIdx.x) * 256 + threadIdx.x; id < all; id += i64(gridDim.x) * 256) {
-        const i64 o = id / a.k, k = id - o * a.k, in = k & (SPAN_K - 1);
-        const u32 byte = a.codes[((o / TILE) * a.spans + (k >> 7)) * SPAN_BYTES + (in >> 3 & 3) * 256 +
-                                 o % TILE * 16 + (in >> 5) * 4 + (in & 3)];
-        const i64 g = (o / TILE * a.groups + (k >> a.shift)) * 16 + o % TILE;
-        const float zero = a.zeros ? float(a.zeros[g]) : 8.0f;
-        const float q = float(byte >> (in & 4) & 15u);
-        static_cast<T *>(a.out)[id] = T(float(static_cast<const S *>(a.scales)[g]) * (q - zero));
+    const int lane = threadIdx.x & 63;
+    const i64 chunks = (a.k + WAVE_INPUTS - 1) / WAVE_INPUTS, all = a.o * chunks;
+    for (i64 id = i64(blockIdx.x) * 4 + wave_of_workgroup(); id < all; id += i64(gridDim.x) * 4) {
+        const i64 o = id / chunks, k = (id - o * chunks) * WAVE_INPUTS + lane * 8;
+        if (k >= a.k) continue;
+        const u32 word = *reinterpret_cast<const u32 *>(a.codes + word_of(o, k, a.spans));
+        const i64 g = (o / TILE * a.groups + (k >> a.shift)) * 16 + (o & 15);   // eight inputs are of one group
+        const float scale = float(static_cast<const S *>(a.scales)[g]), zero = a.zeros ? float(a.zeros[g]) : 8.0f;
+        alignas(16) T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = rounded<T>(scale * (float(word >> (8 * (i & 3) + (i & 4)) & 15u) - zero));
+        T *out = static_cast<T *>(a.out) + o * a.k + k;
+        if (PIECES && k + 8 <= a.k) {
+#pragma unroll
+            for (int i = 0; i < 8; i += PIECE<T>)
+                *reinterpret_cast<Piece<T> *>(out + i) = *reinterpret_cast<const Piece<T> *>(v + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k + i < a.k) out[i] = v[i];
+        }
     }
 }
 
@@ -837,11 +886,15 @@ int mf_int4_quantize(const void *w, int32_t type, int64_t o, int64_t k, int64_t 
     if (!w || !known_type(type) || ldw < 0 || (o > 1 && ldw < k) || !aligned(w, type_bytes(type)))
         return fail(MF_E_INVALID, "invalid 4-bit quantization arguments");
     const Int4QuantizeArgs a{w, o, k, ldw, h.groups, h.spans, h.shift, codes, scales};
-    const i64 units = (o + TILE - 1) / TILE * TILE * h.groups;
-    const u32 grid = u32(std::min<i64>((units + 3) / 4, i64(1) << 20));
+    const i64 step = std::max<i64>(WAVE_INPUTS, group);
+    const i64 waves = (o + TILE - 1) / TILE * TILE * ((h.spans * SPAN_K + step - 1) / step);
+    const u32 grid = u32(std::min<i64>((waves + 3) / 4, i64(1) << 20));
+    const bool pieces = rows_in_pieces(w, o > 1 ? ldw : 0, type);
     return with_types(type, scale_type, [&](auto x, auto scale) {
-        hipLaunchKernelGGL((k_int4_quantize<decltype(x), decltype(scale)>), dim3(grid), dim3(256), 0,
-                           static_cast<hipStream_t>(stream), a);
+        typedef decltype(x) T;
+        typedef decltype(scale) S;
+        hipLaunchKernelGGL((pieces ? k_int4_quantize<T, S, true> : k_int4_quantize<T, S, false>), dim3(grid),
+                           dim3(256), 0, static_cast<hipStream_t>(stream), a);
         return check_launch("4-bit quantization");
     });
 }
@@ -854,11 +907,15 @@ int mf_int4_dequantize(const uint8_t *codes, const void *scales, int32_t scale_t
     if (!out || !known_type(type) || !aligned(out, type_bytes(type)))
         return fail(MF_E_INVALID, "invalid 4-bit dequantization arguments");
     a.out = out;
-    const u32 grid = u32(std::min<i64>((o * k + 255) / 256, i64(1) << 20));
+    const i64 waves = o * ((k + WAVE_INPUTS - 1) / WAVE_INPUTS);
+    const u32 grid = u32(std::min<i64>((waves + 3) / 4, i64(1) << 20));
+    const bool pieces = rows_in_pieces(out, o > 1 ? k : 0, type);
     return with_type(type, [&](auto x) {
         return with_type(scale_type, [&](auto scale) {
-            hipLaunchKernelGGL((k_int4_dequantize<decltype(x), decltype(scale)>), dim3(grid), dim3(256), 0,
-                               static_cast<hipStream_t>(stream), a);
+            typedef decltype(x) T;
+            typedef decltype(scale) S;
+            hipLaunchKernelGGL((pieces ? k_int4_dequantize<T, S, true> : k_int4_dequantize<T, S, false>),
+                               dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), a);
             return check_launch("4-bit dequantization");
         });
     });

@@ -212,7 +212,8 @@ def test_exact_sums(hip_device):
 
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("o,k,group", [(1, 1, 32), (17, 100, 32), (33, 300, 64), (16, 128, 128),
-                                       (40, 1000, 256)])
+                                       (40, 1000, 256), (20, 700, 512), (5, 3000, 1024),
+                                       (3, 5001, 4096)])
 def test_quantization(hip_device, kind, o, k, group):
     """Scales max|w| / 7 in their type, nearest codes, and the values that they stand for."""
     dtype = TYPES[kind]
@@ -262,9 +263,10 @@ def test_quantization_at_the_edges(hip_device):
     assert memfast.int4_linear(torch.zeros(0, 64, device=hip_device), held).shape == (0, 3)
 
 
-@pytest.mark.parametrize("n", [1, 24, 150])
-def test_captured_streams_and_repeats(hip_device, n):
-    x, held, b, y = check(hip_device, n, 1100, 300, 64, "bf16", zeros=True)
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,o", [(1, 300), (24, 300), (150, 300), (200, 4200)])
+def test_captured_streams_and_repeats(hip_device, kind, n, o):
+    x, held, b, y = check(hip_device, n, 1100, o, 64, kind, zeros=True)
     for _ in range(5):
         assert torch.equal(memfast.int4_linear(x, held, b), y)
     graph = torch.cuda.CUDAGraph()
@@ -307,6 +309,25 @@ def test_codes_beyond_32_bits(hip_device):
         y = memfast.int4_linear(torch.ones(n, k, device=hip_device), held)
         tail = o - (o - 1) // 16 * 16
         assert bool((y[:, :-tail] == 0).all()) and bool((y[:, -tail:] == k).all())
+
+
+def test_models_with_held_layers_are_converted(hip_device):
+    """convert_model copies and keeps them; moving the model moves codes and tables."""
+    torch.manual_seed(1)
+    config = memfast.Config(activation_bits=8, weight_bits=8, input_slice=(1, 1, 2, 2, 2),
+                            weight_slice=(1, 1, 2, 2, 2), array_size=(128, 128), rows_per_read=32,
+                            nonidealities=memfast.Nonidealities(write_variation=0.0))
+    head = Int4Linear(nn.Linear(24, 10).to(hip_device))
+    model = nn.Sequential(nn.Linear(40, 24).to(hip_device), head)
+    analog = memfast.convert_model(model, memfast.Simulator(config, device=hip_device))
+    assert isinstance(analog[0], memfast.AnalogLinear) and isinstance(analog[1], Int4Linear)
+    x = torch.randn(5, 40, device=hip_device)
+    with torch.no_grad():
+        assert torch.equal(analog(x), head(analog[0](x)))
+        short = Int4Linear(nn.Linear(24, 10).to(hip_device)).bfloat16()
+        y = short(x[:, :24].bfloat16())
+        assert y.dtype == torch.bfloat16 and short.codes.dtype == torch.uint8
+    assert analog[1].cpu().codes.device.type == "cpu"
 
 
 def test_layer(hip_device):
