@@ -23,7 +23,7 @@ class Dropout(nn.Module):
         self.p = _check_probability(p)
 
     def forward(self, x, residual=None):
-        seed = int(torch.randint(1 << 62, ())) if self.training and self.p else 0
+        seed = int(torch.randint(1 << 62, (), device="cpu")) if self.training and self.p else 0
         return dropout(x, self.p, seed=seed, residual=residual, training=self.training)
 
     def extra_repr(self):

@@ -238,3 +238,16 @@ def test_a_checkpointed_layer_keeps_its_mask(hip_device, reentrant):
         x.grad = None
         y.sum().backward()
         assert torch.equal(x.grad != 0, y != 0)
+
+
+def test_the_layers_seeds_stay_on_the_cpu(hip_device):
+    """A default device moves neither the generator nor the masks, and no draw waits for the GPU."""
+    layer = Dropout(0.4)
+    x = torch.ones(777, device=hip_device)
+    torch.manual_seed(11)
+    expected = layer(x)
+    torch.manual_seed(11)
+    state = torch.cuda.get_rng_state(hip_device)
+    with torch.device(hip_device):
+        assert torch.equal(layer(x), expected)
+    assert torch.equal(torch.cuda.get_rng_state(hip_device), state)
