@@ -124,8 +124,8 @@ class Int4Tensor:
 def int4_quantize(weight, *, group=32, scale_dtype=None):
     """``weight`` [o, k] (float32, bfloat16 or float16) as an Int4Tensor: scales ``max|w| / 7`` of each
     group, rounded to ``scale_dtype`` (the weight's dtype by default, or float32), and the nearest codes
-    of -7 .. 7 about a zero point of 8.  A group with a NaN or an infinity stands for NaN, as one does
-    whose scale passes the dtype's range.  No gradient flows through it."""
+    about a zero point of 8: -7 .. 7, and -8 .. 7 where a subnormal scale was rounded down.  A group with a NaN
+    or an infinity stands for NaN.  No gradient flows through it."""
     _check_floating("weight", weight)
     _check_group(group)
     if weight.ndim != 2:

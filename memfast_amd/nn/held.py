@@ -7,7 +7,7 @@ from ..int4 import Int4Tensor, int4_linear, int4_quantize
 
 class Int4Linear(nn.Module):
     """``nn.Linear`` for serving: the weight is quantized once, on its own device, and held in codes and
-    scales (buffers; 5 bits a value with groups of 32 and 16-bit scales), the input is not quantized.
+    scales (buffers; 4.5 bits a value with groups of 32 and 16-bit scales), the input is not quantized.
     ``from_tensor`` takes an Int4Tensor that is held already, imported codes among them.  It has no
     gradient: call it where none are recorded."""
 
