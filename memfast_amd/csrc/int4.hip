@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void k_int4_pad(const T *x, i64 n, i64 k, i64 
 
 // ---- many rows -------------------------------------------------------------
 // Rows of x as the tile kernel copies them, and their sums: [blocks, pitch] of `factor` times the sum of each
-// row over a block of 32 inputs (`per` 4 to a span) or 128 (1), 0 past the rows.
+// row over a block of 32 inputs (`per` 4 to a span), 64 (2) or 128 (1), 0 past the rows.
 struct PrepareArgs {
     const void *x;
     i64 n, k, ldx, spans, pitch;
@@ -338,13 +338,10 @@ template <typename T, bool PIECES> __global__ __launch_bounds__(256) void k_int4
     for (int i = 0; i < 8; ++i) sum += float(x.v[i]);
     sum += __shfl_xor(sum, 1);
     sum += __shfl_xor(sum, 2);
-    if (a.per == 1) {
-        sum += __shfl_xor(sum, 4);
-        sum += __shfl_xor(sum, 8);
-        if (piece == 0) a.sums[span * a.pitch + n] = a.factor * sum;
-    } else if ((piece & 3) == 0) {
-        a.sums[(span * 4 + piece / 4) * a.pitch + n] = a.factor * sum;
-    }
+    if (a.per < 4) sum += __shfl_xor(sum, 4);
+    if (a.per < 2) sum += __shfl_xor(sum, 8);
+    const int shift = a.per == 4 ? 2 : a.per == 2 ? 3 : 4;     // log2 of a block's pieces
+    if ((piece & ((1 << shift) - 1)) == 0) a.sums[(span * a.per + (piece >> shift)) * a.pitch + n] = a.factor * sum;
 }
 
 struct TileArgs {
@@ -368,11 +365,14 @@ template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v1
 // A workgroup of four waves takes 32 NT rows and 128 NO outputs, a wave 32 NO of them: its codes go from
 // memory to registers, where they become operands once for all rows; x comes through LDS, copied by DMA a
 // span ahead.  With the sums' TABLE, sums over a group begin at -8 times the sum of x, so a zero point of 8
-// costs nothing; others (ZEROS) are taken off with one operation more a group and result.  Without it
-// a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for groups of 128 on, else 4.
+// costs nothing; others (ZEROS) are taken off with one operation more a group and result, the sums read when
+// they are (held from the group's start they spill: with zero points and groups of 32 BF16 takes 359 -> 318 us,
+// FP16 442 -> 344).  Without it a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for
+// groups of 128 on, 2 for 64, 4 for 32 (2048 x 4096 x 11008 BF16 with groups of 64: four 250 us, two 210; 24 x
+// 11008 x 4096 18 and 16).
 // 2048 x 4096 x 11008 BF16, groups of 128, in 181 us (1020 TFLOP/s): bound by the matrix cores, which take 182
 // with nothing but their instructions left; with tiles of 128 rows, one wave a SIMD, it takes 265, with the
-// whole span's codes converted first the same. Groups of 32, four scalings a span, 240: the vector units. In small
+// whole span's codes converted first the same. Groups of 32, four scalings a span, 245: the vector units. In small
 // tiles a span's copies are waited for (24 x 11008 x 4096 FP16 11 us); four stages of them with the codes among
 // them leave one workgroup a compute unit and take 15.
 constexpr int TILE_WAVES = 4, BAND = 8;
@@ -451,11 +451,22 @@ k_int4_tile(const TileArgs t) {
                 w[j][m] = *reinterpret_cast<const v4u *>(codes[j] + i64(span) * SPAN_BYTES + m * 512);
 #pragma unroll
             for (int g = 0; g < PER; ++g) {
-                const int at = min((span * SPAN_K + g * 32) >> a.shift, int(a.groups) - 1) * 16;
+                const int at = min((span * SPAN_K + g * (SPAN_K / PER)) >> a.shift, int(a.groups) - 1) * 16;
                 s[j][g] = scales[j][at];
                 z[j][g] = u8(8);
                 if (ZEROS && a.zeros) z[j][g] = zeros[j][at];
             }
+        }
+    };
+
+    // The staged sums of group g of a span for this lane's results of 32 rows.
+    const auto read_sums = [&](const u8 *stage, int g, int i, v16f &to) {
+        const float *from = reinterpret_cast<const float *>(stage + XBYTES) + g * 128 + 32 * i + 4 * half;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const v4f four = *reinterpret_cast<const v4f *>(from + 8 * e);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) to[4 * e + f] = four[f];
         }
     };
 
@@ -488,17 +499,8 @@ k_int4_tile(const TileArgs t) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 if (b % STEPS == 0) {
-                    sum[i] = v16f{};
-                    if (TABLE) {
-                        const float *from = reinterpret_cast<const float *>(stage + XBYTES) +
-                                            b / STEPS * 128 + 32 * i + 4 * half;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const v4f four = *reinterpret_cast<const v4f *>(from + 8 * e);
-#pragma unroll
-                            for (int f = 0; f < 4; ++f) sum[i][4 * e + f] = four[f];
-                        }
-                    }
+                    if (TABLE && !ZEROS) read_sums(stage, b / STEPS, i, sum[i]);
+                    else sum[i] = v16f{};
 #pragma unroll
                     for (int j = 0; j < NO; ++j) acc[i][j] = ZEROS ? v16f{} : sum[i];
                 }
@@ -513,7 +515,8 @@ k_int4_tile(const TileArgs t) {
             }
             if ((b + 1) % STEPS == 0)
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 0; i < NT; ++i) {
+                    if (TABLE && ZEROS) read_sums(stage, b / STEPS, i, sum[i]);
 #pragma unroll
                     for (int j = 0; j < NO; ++j)
 #pragma unroll
@@ -522,6 +525,7 @@ k_int4_tile(const TileArgs t) {
                                 ZEROS ? fmaf(zero[j][b / STEPS], sum[i][e], acc[i][j][e]) : acc[i][j][e];
                             total[i][j][e] = fmaf(scale[j][b / STEPS], v, total[i][j][e]);
                         }
+                }
         }
     }
 #pragma unroll
@@ -721,7 +725,7 @@ struct HeldPlan {
     i64 rows, pitch, spans, sums, planes, splits = 1, share, bytes;
     HeldPlan(int32_t type, i64 n, i64 k, i64 o, i64 group, bool pieces) : type(type) {
         spans = share = (k + SPAN_K - 1) / SPAN_K;
-        per = group >= SPAN_K ? 1 : 4;
+        per = group >= SPAN_K ? 1 : int(SPAN_K / group);
         terms = type == MF_F32 ? 3 : 1;
         rows = std::min(n, ROWS_AT_ONCE);
         kernel = few(type, n, k, o) ? FEW : large(type, rows, o) ? LARGE : MID;
@@ -779,22 +783,29 @@ int launch_tile(const TileArgs &t, hipStream_t s) {
     return check_launch("4-bit product");
 }
 
+// Calls f(PER) for 1, 2 or 4 scalings in a span.
+template <typename F> int with_per(int per, F f) {
+    return per == 1   ? f(std::integral_constant<int, 1>{})
+           : per == 2 ? f(std::integral_constant<int, 2>{})
+                      : f(std::integral_constant<int, 4>{});
+}
+
 // Tiles of 64 rows and 256 outputs.
 template <typename T, typename S> int launch_large(const TileArgs &t, int per, hipStream_t s) {
-    if (per == 1)
-        return t.h.zeros ? launch_tile<T, S, 2, 2, true, true, 1>(t, s)
-                         : launch_tile<T, S, 2, 2, true, false, 1>(t, s);
-    return t.h.zeros ? launch_tile<T, S, 2, 2, true, true, 4>(t, s)
-                     : launch_tile<T, S, 2, 2, true, false, 4>(t, s);
+    return with_per(per, [&](auto p) {
+        constexpr int PER = decltype(p)::value;
+        return t.h.zeros ? launch_tile<T, S, 2, 2, true, true, PER>(t, s)
+                         : launch_tile<T, S, 2, 2, true, false, PER>(t, s);
+    });
 }
 
 // Tiles of 32 or 64 rows and 128 outputs, with the spans split.
 template <typename T, typename S> int launch_mid(const TileArgs &t, int per, hipStream_t s) {
-    if (HeldPlan::mid_rows(t.h.n) == 32)
-        return per == 1 ? launch_tile<T, S, 1, 1, false, true, 1>(t, s)
-                        : launch_tile<T, S, 1, 1, false, true, 4>(t, s);
-    return per == 1 ? launch_tile<T, S, 2, 1, false, true, 1>(t, s)
-                    : launch_tile<T, S, 2, 1, false, true, 4>(t, s);
+    return with_per(per, [&](auto p) {
+        constexpr int PER = decltype(p)::value;
+        return HeldPlan::mid_rows(t.h.n) == 32 ? launch_tile<T, S, 1, 1, false, true, PER>(t, s)
+                                               : launch_tile<T, S, 2, 1, false, true, PER>(t, s);
+    });
 }
 
 template <typename T> int launch_join(const TileArgs &t, hipStream_t s) {

@@ -97,6 +97,17 @@ def test_large_tiles_and_many_rows(hip_device, kind, n, k, o):
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_scalings_of_a_span(hip_device, kind, group, zeros):
+    """One, two and four in the wide tiles and in both of the small ones, scales of either type."""
+    for n, k, o in ((260, 1000, 4100), (70, 900, 300), (30, 3000, 600)):
+        check(hip_device, n, k, o, group, kind, zeros=zeros)
+        if kind != "fp32":
+            check(hip_device, n, k, o, group, kind, zeros=zeros, scales=torch.float32)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("n,k,o", [(17, 600, 8200), (6, 300, 8193), (32, 264, 8192), (64, 1032, 500),
                                    (40, 8, 33), (24, 11008, 400), (48, 4096, 300)])
 def test_between_few_rows_and_tiles(hip_device, kind, n, k, o):
