@@ -759,11 +759,14 @@ struct HeldPlan {
     }
     static i64 mid_rows(i64 n) { return n <= 32 ? 32 : 64; }
     static i64 large_tiles(i64 n, i64 o) { return (n + 63) / 64 * ((o + 255) / 256); }
-    // The sums' launch and the wide tiles pay for many rows, of FP32, whose sums take three times the
-    // instructions, from fewer on, where they are tiles enough (us, mid / large: 256 x 4096 x 11008 47 / 41,
-    // 128 of them 31 / 30, 256 x 4096 x 4096 31 / 30 and in FP32 85 / 48, 300 x 2048 x 2048 18 / 21).
+    // The sums' launch and the wide tiles pay for many rows where they are tiles enough (us, mid / large: 256 x
+    // 4096 x 11008 47 / 41, 128 of them 31 / 30, 256 x 4096 x 4096 31 / 30, 300 x 2048 x 2048 16 / 19, 512 x 4096
+    // x 1024 21 / 26). FP32 has a launch before its tiles anyway and sums that take three times the instructions:
+    // from fewer on (70 x 11008 x 4096 87 / 48, 40 x 4096 x 11008 72 / 33, 100 x 4096 x 2048 33 / 26, 64 x
+    // 4096 x 4096 34 / 27; 100 x 1024 x 2048 17 / 18; 77 x 1500 x 1111, ten tiles, 17 / 18).
     static bool large(int32_t type, i64 n, i64 o) {
-        return n > (type == MF_F32 ? 64 : 128) && o > 128 && large_tiles(n, o) >= 64;
+        return type == MF_F32 ? n > 32 && o > 128 && large_tiles(n, o) >= 16
+                              : n > 128 && o > 128 && large_tiles(n, o) >= 64;
     }
 };
 

@@ -101,7 +101,7 @@ def test_large_tiles_and_many_rows(hip_device, kind, n, k, o):
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_scalings_of_a_span(hip_device, kind, group, zeros):
     """One, two and four in the wide tiles and in both of the small ones, scales of either type."""
-    for n, k, o in ((260, 1000, 4100), (70, 900, 300), (30, 3000, 600)):
+    for n, k, o in ((260, 1000, 4100), (70, 900, 300), (30, 3000, 600), (48, 4000, 4100)):
         check(hip_device, n, k, o, group, kind, zeros=zeros)
         if kind != "fp32":
             check(hip_device, n, k, o, group, kind, zeros=zeros, scales=torch.float32)
