@@ -49,10 +49,11 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Group {
 // at either end. What the rounding of g log2(e) took from the exponent is made good, so that k keeps its
 // digits for far gates too, and the reciprocal (within an ulp) is refined to a rounding, since hundreds of u are
 // multiplied where a channel remembers long: without it the gradient of the first state is off by up to 1e-6
-// after 4096 steps, with it by 2.5e-7 (8 x 4096 x 2048 with gradients 251 -> 256 us). The bounds (which pass a
-// NaN on) keep e finite, where u is 2^-126 and not less, and let it reach 0.
+// after 4096 steps, with it by 2.5e-7 (8 x 4096 x 2048 with gradients 251 -> 256 us). For gates within FAR_GATE,
+// where e and u are normal numbers of FP32; a NaN gives NaN.
+constexpr float FAR_GATE = 87.0f;
+
 __device__ __forceinline__ void gates(float g, float &u, float &k) {
-    g = __builtin_elementwise_minimum(__builtin_elementwise_maximum(g, -87.0f), 110.0f);
     const float t = g * -LOG2E, rest = fmaf(g, -LOG2E, -t);
     float e = __builtin_amdgcn_exp2f(t);
     e = fmaf(e, rest * LN2, e);
@@ -60,6 +61,22 @@ __device__ __forceinline__ void gates(float g, float &u, float &k) {
     u = fmaf(r, fmaf(-d, r, 1.0f), r);
     k = e * u;
 }
+
+// The same for a gate beyond them: the smaller is exp(-|g|), in FP32's subnormal numbers too and then 0 (exp2
+// itself gives normal numbers alone: it is taken of 64 more), so that a closed gate drops a state of any size, and
+// the other is 1.
+__device__ __forceinline__ void far_gates(float g, float &u, float &k) {
+    const float size = fminf(fabsf(g), 200.0f), t = size * LOG2E, rest = fmaf(size, LOG2E, -t);
+    const float e = __builtin_amdgcn_exp2f(64.0f - t), least = fmaf(e, -rest * LN2, e) * 0x1p-64f;
+    u = g < 0.0f ? least : 1.0f;
+    k = g < 0.0f ? 1.0f : least;
+}
+
+// The largest of |g| so far, NaN once there was one; and whether a lane of the wave has gates to be taken again.
+__device__ __forceinline__ float farthest(float most, float g) {
+    return __builtin_elementwise_maximum(most, fabsf(g));
+}
+__device__ __forceinline__ bool any_far(float most) { return __builtin_expect(__any(!(most <= FAR_GATE)), 0); }
 
 // tanh: 1 - 2 / (1 + exp(2 x)), and where that difference would lose digits the series
 // x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835 (below 1/4 the next term is under 1e-8 of it).
@@ -237,18 +254,33 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs 
     int turn = 0;
     for (i64 base = p.begin; base < end; base += span, turn ^= 1) {
         const i64 s = base + wave * CHUNK;
-        float u[CHUNK], in[CHUNK], A = 1.0f, S = 0.0f, h;
+        float u[CHUNK], in[CHUNK], A = 1.0f, S = 0.0f, most = 0.0f, h;
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i) {
+            const float g = float(next_g[i]);
             float k, c = float(next_v[i]);
-            gates(float(next_g[i]), u[i], k);
+            most = farthest(most, g);
+            gates(g, u[i], k);
             if (TANH) c = hyperbolic_tangent(c);
             in[i] = k * c;
         }
-        if (s + CHUNK > p.length)
+        // What is seldom needed, behind one branch. Rows of far gates are read again: held until here they would
+        // take a quarter more registers.
+        const bool far = any_far(most);
+        if (far || s + CHUNK > p.length) {
+            if (far)
+                each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
+                    const float g = float(get<T>(row, p.lane_bytes));
+                    float u_far, k, c = float(get<T>(row, second));
+                    far_gates(g, u_far, k);
+                    if (TANH) c = hyperbolic_tangent(c);
+                    u[i] = fabsf(g) > FAR_GATE ? u_far : u[i];
+                    in[i] = fabsf(g) > FAR_GATE ? k * c : in[i];
+                });
 #pragma unroll
             for (int i = 0; i < CHUNK; ++i)
                 if (s + i >= p.length) u[i] = 1.0f, in[i] = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i) {
             A *= u[i];
@@ -317,17 +349,29 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const Recurrence
         for (i64 base = top; base >= p.begin; base -= span, turn ^= 1) {
             const i64 s = base + wave * CHUNK;
             float u[CHUNK], k[CHUNK], c[CHUNK], g[CHUNK], A = 1.0f, S = 0.0f, Q = 0.0f, h = mark, r;
+            float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < CHUNK; ++i) {
+                most = farthest(most, float(next_g[i]));
                 gates(float(next_g[i]), u[i], k[i]);
                 c[i] = float(next_v[i]);
                 if (TANH) c[i] = hyperbolic_tangent(c[i]);
                 g[i] = float(next_dy[i]);
             }
-            if (s + CHUNK > p.length)
+            const bool far = any_far(most);
+            if (far || s + CHUNK > p.length) {
+                if (far)
+                    each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
+                        const float gate = float(get<T>(row, p.lane_bytes));
+                        float u_far, k_far;
+                        far_gates(gate, u_far, k_far);
+                        u[i] = fabsf(gate) > FAR_GATE ? u_far : u[i];
+                        k[i] = fabsf(gate) > FAR_GATE ? k_far : k[i];
+                    });
 #pragma unroll
                 for (int i = 0; i < CHUNK; ++i)
                     if (s + i >= p.length) u[i] = 1.0f, k[i] = 0.0f, c[i] = 0.0f, g[i] = 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < CHUNK; ++i) {
                 A *= u[i];
@@ -397,22 +441,43 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
         if (GRAD && a.y)
             each_row<CHUNK>(dy, s, p.length,
                             [&](int i, const char *row) { v[i] = get<Group<T, V>>(row, p.lane_bytes); });
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) most = farthest(most, float(g[i].v[j]));
+        // What a step adds, and the maps of the share with it (GRAD: r -> A u (dy + r) + S).
+        const auto added = [&](float k, float c) { return GRAD ? c : k * (TANH ? hyperbolic_tangent(c) : c); };
+        const auto step = [&](int j, float u, float add) {
+            A[j] *= u;
+            S[j] = GRAD ? fmaf(A[j], add, S[j]) : fmaf(u, S[j], add);
+        };
+        if (any_far(most)) {
+#pragma unroll 1
+            for (i64 n = s; n < min(s + CHUNK, end); ++n) {
+                const Group<T, V> gates_at = get<Group<T, V>>(x.at(n), p.lane_bytes);
+                const Group<T, V> values = GRAD ? (a.y ? get<Group<T, V>>(dy.at(n), p.lane_bytes) : Group<T, V>{})
+                                                : get<Group<T, V>>(x.at(n), second);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float gate = float(gates_at.v[j]);
+                    float u, k;
+                    if (fabsf(gate) > FAR_GATE) far_gates(gate, u, k);
+                    else gates(gate, u, k);
+                    step(j, u, added(k, float(values.v[j])));
+                }
+            }
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const bool live = s + i < end;
-                float u, k, c = float(v[i].v[j]);
+                float u, k;
                 gates(float(g[i].v[j]), u, k);
-                u = live ? u : 1.0f;
-                if (GRAD) {     // r -> A u (dy + r) + S
-                    A[j] *= u;
-                    S[j] = fmaf(A[j], live ? c : 0.0f, S[j]);
-                } else {
-                    if (TANH) c = hyperbolic_tangent(c);
-                    A[j] *= u;
-                    S[j] = fmaf(u, S[j], live ? k * c : 0.0f);
-                }
+                const float add = added(k, float(v[i].v[j]));
+                step(j, live ? u : 1.0f, live ? add : 0.0f);
             }
     }
 #pragma unroll
