@@ -78,6 +78,25 @@ __device__ __forceinline__ float farthest(float most, float g) {
 }
 __device__ __forceinline__ bool any_far(float most) { return __builtin_expect(__any(!(most <= FAR_GATE)), 0); }
 
+// Products of u are 0 only where one of their factors is: what gets beneath FP32 is held at its smallest number, so
+// that an infinite state stays infinite, as it does step by step, and no finite one is off by more than 2^-149 of
+// itself. Of two such products (a NaN is passed on), and of a wave's u, whose plain product is A.
+constexpr float SMALLEST = 0x1p-149f;
+
+__device__ __forceinline__ float joined(float a, float b) {
+    const float least = __builtin_elementwise_minimum(__builtin_elementwise_minimum(a, b), SMALLEST);
+    return __builtin_elementwise_maximum(a * b, least);
+}
+template <int N> __device__ __forceinline__ float product(float A, const float (&u)[N]) {
+    if (__builtin_expect(A == 0.0f, 0)) {
+        bool closed = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) closed |= u[i] == 0.0f;
+        A = closed ? 0.0f : SMALLEST;
+    }
+    return A;
+}
+
 // tanh: 1 - 2 / (1 + exp(2 x)), and where that difference would lose digits the series
 // x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835 (below 1/4 the next term is under 1e-8 of it).
 __device__ __forceinline__ float hyperbolic_tangent(float x) {
@@ -194,7 +213,7 @@ __device__ __forceinline__ void fold(const RecurrenceArgs &a, i64 b, i64 channel
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const bool live = n + i < to - from;
-                A[j] *= live ? pa[i][j] : 1.0f;
+                A[j] = joined(A[j], live ? pa[i][j] : 1.0f);
                 S[j] = live ? fmaf(pa[i][j], S[j], ps[i][j]) : S[j];
             }
     }
@@ -286,6 +305,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs 
             A *= u[i];
             S = fmaf(u[i], S, in[i]);
         }
+        A = product(A, u);
         if (base + span < end) load(s + span);
         maps[turn][wave][0][lane] = A;
         maps[turn][wave][1][lane] = S;
@@ -377,6 +397,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const Recurrence
                 A *= u[i];
                 S = fmaf(u[i], S, k[i] * c[i]);
             }
+            A = product(A, u);
 #pragma unroll
             for (int i = CHUNK - 1; i >= 0; --i) Q = u[i] * (g[i] + Q);
             if (base > p.begin) load(base - span);
@@ -429,9 +450,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
     const u32 second = p.lane_bytes + u32(a.width) * u32(sizeof(T));
     const Rows<T, V> x(a.x, p, a.xb, a.xt), dy(a.y, p, a.yb, a.yt);
     const i64 share = a.segment / waves, end = min(p.begin + (wave + 1) * share, p.length);
-    float A[V], S[V];
+    float A[V], S[V], low[V];       // low: the least u
 #pragma unroll
-    for (int j = 0; j < V; ++j) A[j] = 1.0f, S[j] = 0.0f;
+    for (int j = 0; j < V; ++j) A[j] = low[j] = 1.0f, S[j] = 0.0f;
     for (i64 s = p.begin + wave * share; s < end; s += CHUNK) {
         Group<T, V> g[CHUNK], v[CHUNK];
         each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
@@ -449,8 +470,9 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
         // What a step adds, and the maps of the share with it (GRAD: r -> A u (dy + r) + S).
         const auto added = [&](float k, float c) { return GRAD ? c : k * (TANH ? hyperbolic_tangent(c) : c); };
         const auto step = [&](int j, float u, float add) {
-            A[j] *= u;
+            A[j] = GRAD ? joined(A[j], u) : A[j] * u;
             S[j] = GRAD ? fmaf(A[j], add, S[j]) : fmaf(u, S[j], add);
+            low[j] = __builtin_elementwise_minimum(low[j], u);
         };
         if (any_far(most)) {
 #pragma unroll 1
@@ -482,6 +504,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+        if (!GRAD && A[j] == 0.0f && low[j] > 0.0f) A[j] = SMALLEST;
         maps[wave][0][lane * V + j] = A[j];
         maps[wave][1][lane * V + j] = S[j];
     }
@@ -497,7 +520,7 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
             }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            A[j] *= maps[w][0][lane * V + j];
+            A[j] = joined(A[j], maps[w][0][lane * V + j]);
             S[j] = fmaf(maps[w][0][lane * V + j], S[j], maps[w][1][lane * V + j]);
         }
     }

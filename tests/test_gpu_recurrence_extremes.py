@@ -113,3 +113,43 @@ def test_closed_and_open_gates_of_a_large_gradient(hip_device, kind, steps, at):
     got = run(*(t.to(hip_device) for t in given))
     for label, pair in reference(*given).items():
         near(got[label], pair, label)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("steps", [3, 16, 40, 300, 700, 9000])
+def test_infinite_states_stay(hip_device, kind, reverse, steps):
+    """Gates of -10 take a state's share beneath FP32 within a stretch of nine steps; an infinite one is
+    infinite after every step all the same, as u h is for every u above 0, and so are gradients."""
+    gen = torch.Generator().manual_seed(steps)
+    x = torch.randn(steps, 2, 8, generator=gen)
+    x[..., :4] = -10.0
+    state = torch.tensor([math.inf, -math.inf, 1.0, 0.0]).expand(2, 4).contiguous()
+    x, state = x.to(TYPES[kind]).to(hip_device), state.to(hip_device)
+    leaf, start = x.clone().requires_grad_(True), state.clone().requires_grad_(True)
+    y, last = memfast.gated_recurrence(leaf, start, activation=None, reverse=reverse)
+    for channel, sign in ((0, 1), (1, -1)):
+        assert bool((y[..., channel] == sign * math.inf).all())
+        assert bool((last[..., channel] == sign * math.inf).all())
+    assert bool(y[..., 2:].isfinite().all()) and bool(last[..., 2:].isfinite().all())
+    # The gradients of a last state, and of one step's state, in steps where the state is finite.
+    at = steps // 2
+    dlast = torch.zeros_like(last)
+    dlast[:, 2], dlast[:, 3] = math.inf, 1.0
+    dx, dstate = torch.autograd.grad((y, last), (leaf, start), (torch.zeros_like(y), dlast), retain_graph=True)
+    assert bool((dx[..., 6] == math.inf).all()) and bool((dstate[:, 2] == math.inf).all())
+    assert bool(dx[..., 2].isinf().all()) and bool(dx[..., 7].isfinite().all())
+    dy = torch.zeros_like(y)
+    dy[at, :, 2] = -math.inf
+    dx, dstate = torch.autograd.grad((y, last), (leaf, start), (dy, torch.zeros_like(last)))
+    reached = torch.arange(steps, device=hip_device) >= at if reverse else \
+        torch.arange(steps, device=hip_device) <= at
+    assert bool((dx[reached][..., 6] == -math.inf).all()) and bool((dx[~reached][..., 6] == 0).all())
+    assert bool((dstate[:, 2] == -math.inf).all()) and bool((dstate[:, 3] == 0).all())
+    # A candidate, from its step on.
+    x[at, :, 4 + 3] = math.inf
+    y, last = memfast.gated_recurrence(x, state, activation=None, reverse=reverse)
+    after = ~reached if reverse else torch.arange(steps, device=hip_device) >= at
+    after[at] = True
+    assert bool((y[after][..., 3] == math.inf).all()) and bool((last[:, 3] == math.inf).all())
+    assert bool(y[~after][..., 3].isfinite().all()) and bool(y[..., 2].isfinite().all())
