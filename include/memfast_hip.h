@@ -653,6 +653,8 @@ int mf_recurrence_grad(const void *x, int32_t type, int64_t steps, int64_t batch
  * there, on the device.  dropped: 0 .. 65536.  The gradient of x is the same call for dy without residual. */
 int mf_dropout(const void *x, int32_t type, int64_t n, const void *residual, uint32_t dropped,
                uint64_t seed, uint64_t event, const int64_t *event_at, void *y, void *stream);
+/* The number of the capture that `stream` is part of, or 0 (id on the host; nothing is launched). */
+int mf_capture_id(void *stream, uint64_t *id);
 
 /* ---- weights held as 4-bit whole numbers (int4.hip) -------------------------- */
 /* A weight [o, k] is scale * (code - zero) with codes 0 .. 15 and a scale and a zero point (0 .. 15; NULL: 8)

@@ -107,3 +107,13 @@ extern "C" int mf_dropout(const void *x, int32_t type, int64_t n, const void *re
         return check_launch("dropout");
     });
 }
+
+extern "C" int mf_capture_id(void *stream, uint64_t *id) {
+    if (!id) return fail(MF_E_INVALID, "no place for a capture's number");
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long number = 0;
+    const hipError_t e = hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &number);
+    if (e != hipSuccess) return fail(MF_E_HIP, "capture of a stream: %s", hipGetErrorString(e));
+    *id = status == hipStreamCaptureStatusActive ? u64(number) : 0;
+    return MF_OK;
+}

@@ -221,6 +221,7 @@ SIGNATURES = {
     "mf_recurrence_grad": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I32, _I32, _P, _P, _I64, _I64,
                             _P, _P, _I64, _I64, _P, _P, _I64, _P], ct.c_int),
     "mf_dropout": ([_P, _I32, _I64, _P, ct.c_uint32, ct.c_uint64, ct.c_uint64, _P, _P, _P], ct.c_int),
+    "mf_capture_id": ([_P, ct.POINTER(ct.c_uint64)], ct.c_int),
     "mf_int4_quantize": ([_P, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _P], ct.c_int),
     "mf_int4_dequantize": ([_P, _P, _I32, _P, _I64, _I64, _I64, _P, _I32, _P], ct.c_int),
     "mf_int4_linear_workspace": ([_I32, _I64, _I64, _I64, _I64, _I32, ct.POINTER(_I64)], ct.c_int),
@@ -1705,6 +1706,13 @@ def dropout(x, residual, dropped, seed, event):
     _launch(library().mf_dropout, x.device, "dropout", x.data_ptr(), FLOAT_TYPES[x.dtype], x.numel(),
             None if residual is None else residual.data_ptr(), dropped, seed, event, at, out.data_ptr())
     return out
+
+
+def capture_id(device):
+    """The number of the capture that the current stream of ``device`` is part of, or 0 (mf_capture_id)."""
+    number = ct.c_uint64()
+    check(library().mf_capture_id(_stream(device), ct.byref(number)), "capture")
+    return number.value
 
 
 # ---------------------------------------------------------------------------

@@ -8,23 +8,60 @@ and leaves the gated linear recurrence of memfast_amd/recurrence.py.
 import torch
 from torch import nn
 
+from .. import hip
 from ..recurrence import ACTIVATIONS, gated_recurrence
 from ..regularization import _check_probability, dropout
+
+
+# What captured dropouts count up, by device index: events from 1 on, where eager passes have 0. Graphs hold their
+# addresses, so they stay for the process.
+_counters = {}
 
 
 class Dropout(nn.Module):
     """Dropout by ``memfast_amd.dropout``, each forward in training mode with a seed that it draws from torch's
     default CPU generator: ``torch.manual_seed`` makes the masks again, and so does a checkpointed
-    layer's second forward, for which torch restores the generator.  A captured graph keeps the one mask of
-    its capture; ``memfast_amd.dropout`` with an event on the device makes new ones."""
+    layer's second forward, for which torch restores the generator.
+
+    A captured forward keeps the seed of its capture and takes its event from a counter on the device, which the
+    graph counts up: every replay has a mask of its own, and a captured backward that of its forward, also where
+    checkpointing takes the forward again. The counter is made by the first forward in training mode on a
+    device, so one has to run there before a capture."""
 
     def __init__(self, p=0.5):
         super().__init__()
         self.p = _check_probability(p)
+        self._captured = {}     # by seed: the capture and its event, until an eager forward (then None)
+
+    def _event(self, x, seed):
+        if torch._C._current_graph_task_id() != -1:     # within a backward: a checkpointed forward once more
+            event = self._captured.get(seed, (0, 0))[1]
+            if event is None:
+                raise RuntimeError("a captured forward is taken again after an eager one in training mode")
+            return event
+        capture = hip.capture_id(x.device)
+        counter = _counters.get(x.device.index)
+        if not capture:
+            if counter is None:
+                with torch.inference_mode(False):
+                    _counters[x.device.index] = torch.ones(1, dtype=torch.int64, device=x.device)
+            self._captured = {s: (0, None) for s in self._captured if s != seed}
+            return 0
+        if counter is None:
+            raise RuntimeError("a Dropout layer in training mode has to run on the device before one is captured")
+        known = self._captured.get(seed)
+        if known is None or known[0] != capture:
+            # A sum, not a copy: kernels alone in the graph. The counter goes on before the backward reads it.
+            self._captured[seed] = capture, counter + 0
+            counter.add_(1)
+        return self._captured[seed][1]
 
     def forward(self, x, residual=None):
-        seed = int(torch.randint(1 << 62, (), device="cpu")) if self.training and self.p else 0
-        return dropout(x, self.p, seed=seed, residual=residual, training=self.training)
+        if not (self.training and self.p):
+            return dropout(x, self.p, seed=0, residual=residual, training=self.training)
+        seed = int(torch.randint(1 << 62, (), device="cpu"))
+        event = self._event(x, seed) if isinstance(x, torch.Tensor) and x.is_cuda else 0
+        return dropout(x, self.p, seed=seed, event=event, residual=residual)
 
     def extra_repr(self):
         return f"p={self.p}"
