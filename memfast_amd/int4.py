@@ -50,7 +50,7 @@ def _by_tile(table):
     """[tiles, groups, 16] of a table [o, groups], with zeros past o."""
     o, groups = table.shape
     table = torch.nn.functional.pad(table, (0, 0, 0, -o % hip.INT4_TILE))
-    return table.view(-1, hip.INT4_TILE, groups).transpose(1, 2).contiguous()
+    return table.view(len(table) // hip.INT4_TILE, hip.INT4_TILE, groups).transpose(1, 2).contiguous()
 
 
 class Int4Tensor:
