@@ -67,6 +67,8 @@ class Int4Tensor:
         if len(shape) != 2:
             raise ValueError("an Int4Tensor has two dimensions")
         o, k = shape
+        if o < 0 or k < 0:
+            raise ValueError("an Int4Tensor has no negative dimension")
         self.group = _check_group(group)
         _check_sizes(o, k)
         if not isinstance(codes, torch.Tensor):

@@ -17,3 +17,12 @@ def test_weights_without_values_are_packed(o, k, zeros):
     assert held.shape == (o, k) and held.codes.shape == (tiles, -(-k // 128), 1024)
     assert held.scales.shape == (tiles, groups, 16)
     assert held.zeros is None or held.zeros.shape == (tiles, groups, 16)
+
+
+@pytest.mark.parametrize("o,k", [(-1, 64), (16, -1), (-15, -20)])
+def test_negative_shapes_are_refused(o, k):
+    """Parts without values, as rounding up makes them of such a shape, are no weight."""
+    codes = torch.zeros(-(-o // 16), -(-k // 128), 1024, dtype=torch.uint8)
+    scales = torch.ones(-(-o // 16), -(-k // 32), 16)
+    with pytest.raises(ValueError, match="negative"):
+        memfast.Int4Tensor(codes, scales, (o, k), group=32)
