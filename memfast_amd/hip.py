@@ -1710,6 +1710,8 @@ def dropout(x, residual, dropped, seed, event):
 
 def capture_id(device):
     """The number of the capture that the current stream of ``device`` is part of, or 0 (mf_capture_id)."""
+    if device.index == _current_device() and not torch.cuda.is_current_stream_capturing():
+        return 0
     number = ct.c_uint64()
     check(library().mf_capture_id(_stream(device), ct.byref(number)), "capture")
     return number.value

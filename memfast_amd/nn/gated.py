@@ -45,7 +45,8 @@ class Dropout(nn.Module):
             if counter is None:
                 with torch.inference_mode(False):
                     _counters[x.device.index] = torch.ones(1, dtype=torch.int64, device=x.device)
-            self._captured = {s: (0, None) for s in self._captured if s != seed}
+            if self._captured:
+                self._captured = {s: (0, None) for s in self._captured if s != seed}
             return 0
         if counter is None:
             raise RuntimeError("a Dropout layer in training mode has to run on the device before one is captured")
