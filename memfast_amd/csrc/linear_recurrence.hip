@@ -98,7 +98,8 @@ template <int N> __device__ __forceinline__ float product(float A, const float (
 }
 
 // tanh: 1 - 2 / (1 + exp(2 x)), and where that difference would lose digits the series
-// x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835 (below 1/4 the next term is under 1e-8 of it).
+// x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835 (below 1/4 the next term is under 1e-8 of it). The
+// reciprocal is not refined: tanh's error does not grow over the steps.
 __device__ __forceinline__ float hyperbolic_tangent(float x) {
     const float e = __builtin_amdgcn_exp2f(x * (2.0f * LOG2E));
     const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
@@ -246,7 +247,7 @@ __device__ __forceinline__ void blank(const Place<T, 1> &p, void *rows, i64 sequ
 }
 
 // Bound by its bytes and by the vector units, which are busy two thirds of the time: 8 x 4096 x 2048 BF16 in
-// 100 us (403 MB, 4.0 TB/s). Two channels a lane, for wider rows of loads, took 104; sixteen waves of eight
+// 95 us (403 MB, 4.2 TB/s). Two channels a lane, for wider rows of loads, took 104; sixteen waves of eight
 // steps, which join twice as many maps, 115.
 template <typename T, bool TANH, int WAVES, int CHUNK>
 __global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs a) {
@@ -438,8 +439,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const Recurrence
 }
 
 // A and S of every segment but the last (GRAD: A and Q of every segment but the first), each wave its
-// share of the segment's steps. Bound by its bytes and the vector units: 65536 x 512 BF16 in 31 us (134 MB,
-// 4.3 TB/s); the segments' own pass reads them again (42 us with the states written).
+// share of the segment's steps. Bound by its bytes and the vector units: 65536 x 512 BF16 in 33 us (134 MB,
+// 4.1 TB/s); the segments' own pass reads them again (42 us with the states written).
 template <typename T, int V, bool TANH, bool GRAD>
 __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const RecurrenceArgs a) {
     constexpr int CHUNK = 8;

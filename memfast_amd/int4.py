@@ -148,9 +148,9 @@ def int4_linear(x, weight, bias=None):
 
     The weight's scales have x's dtype or float32, and ``bias`` [o] x's dtype.  It is a product for serving:
     an operand that wants a gradient is refused while gradients are recorded, one with a tangent of
-    forward mode always.  Rows of x are below 2**27, o below 2**25 and k
-    below 2**24.  A NaN or an infinity in a
-    row of x, or sums of a group's 15 |x| beyond FP32, leave that row without finite values."""
+    forward mode always.  Rows of x are below 2**27, o below 2**25 and k below 2**24.  A NaN or an infinity in a
+    row of x, or sums of a group's 15 |x| beyond FP32, leave that row without finite values.  Codes are summed as
+    they are and the zero point's share is taken off, so the sums' roundings are those of ``|x| s (q + z)``."""
     _check_floating("x", x)
     if not isinstance(weight, Int4Tensor):
         raise TypeError("weight must be an Int4Tensor")

@@ -66,8 +66,8 @@ def gated_recurrence(projected, state=None, *, activation="tanh", lengths=None, 
     ``reverse`` runs from the last step of each sequence to the first.  States have the input's dtype
     (float32, bfloat16 or float16); ``state`` has that or float32, and the last state is float32, so
     that a sequence taken in parts is the sequence.  A gate below -104, whose ``u`` is 0 in float32, drops a
-    state of any size (an infinite one becomes NaN there, and stays infinite before).  Fewer than 2**31 steps and sequences, H at
-    most 2**24.  An operand with a tangent of forward mode is refused."""
+    state of any size (an infinite one becomes NaN there, and stays infinite before).  Fewer than 2**31
+    steps and sequences, H at most 2**24.  An operand with a tangent of forward mode is refused."""
     _check_floating("projected", projected)
     if activation not in ACTIVATIONS:
         raise ValueError("activation must be 'tanh' or None")
