@@ -50,8 +50,8 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Group {
 // digits for far gates too, and the reciprocal (within an ulp) is refined to a rounding, since hundreds of u are
 // multiplied where a channel remembers long: without it the gradient of the first state is off by up to 1e-6
 // after 4096 steps, with it by 2.5e-7 (8 x 4096 x 2048 with gradients 251 -> 256 us). For gates within FAR_GATE,
-// where e and u are normal numbers of FP32; a NaN gives NaN.
-constexpr float FAR_GATE = 87.0f;
+// where e and u are normal numbers of FP32, which is all that these instructions give; a NaN gives NaN.
+constexpr float FAR_GATE = 87.0f, FAR_VALUE = 1.64581143e-38f;     // exp(-87)
 
 __device__ __forceinline__ void gates(float g, float &u, float &k) {
     const float t = g * -LOG2E, rest = fmaf(g, -LOG2E, -t);
@@ -62,17 +62,17 @@ __device__ __forceinline__ void gates(float g, float &u, float &k) {
     k = e * u;
 }
 
-// The same for a gate beyond them: the smaller is exp(-|g|), in FP32's subnormal numbers too and then 0 (exp2
-// itself gives normal numbers alone: it is taken of 64 more), so that a closed gate drops a state of any size, and
-// the other is 1.
+// Puts in their place what they are for a gate beyond: the smaller exp(-|g|), subnormal numbers and then 0, so that a
+// closed gate drops a state of any size, and the other 1. Others are left. A wave comes here where one of its lanes
+// has such a gate: 8 x 4096 x 2048 BF16 with one gate in a hundred closed, which is all waves, 123 us for 100.
 __device__ __forceinline__ void far_gates(float g, float &u, float &k) {
-    const float size = fminf(fabsf(g), 200.0f), t = size * LOG2E, rest = fmaf(size, LOG2E, -t);
-    const float e = __builtin_amdgcn_exp2f(64.0f - t), least = fmaf(e, -rest * LN2, e) * 0x1p-64f;
-    u = g < 0.0f ? least : 1.0f;
-    k = g < 0.0f ? 1.0f : least;
+    const float least = FAR_VALUE * __builtin_amdgcn_exp2f((FAR_GATE - fabsf(g)) * LOG2E);
+    const bool far = fabsf(g) > FAR_GATE, closed = g < 0.0f;
+    u = far ? (closed ? least : 1.0f) : u;
+    k = far ? (closed ? 1.0f : least) : k;
 }
 
-// The largest of |g| so far, NaN once there was one; and whether a lane of the wave has gates to be taken again.
+// The largest of |g| so far, NaN once there was one; and whether a wave has gates beyond FAR_GATE (or NaN).
 __device__ __forceinline__ float farthest(float most, float g) {
     return __builtin_elementwise_maximum(most, fabsf(g));
 }
@@ -247,7 +247,7 @@ __device__ __forceinline__ void blank(const Place<T, 1> &p, void *rows, i64 sequ
 }
 
 // Bound by its bytes and by the vector units, which are busy two thirds of the time: 8 x 4096 x 2048 BF16 in
-// 95 us (403 MB, 4.2 TB/s). Two channels a lane, for wider rows of loads, took 104; sixteen waves of eight
+// 100 us (403 MB, 4.0 TB/s). Two channels a lane, for wider rows of loads, took 104; sixteen waves of eight
 // steps, which join twice as many maps, 115.
 template <typename T, bool TANH, int WAVES, int CHUNK>
 __global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs a) {
@@ -274,33 +274,23 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs 
     int turn = 0;
     for (i64 base = p.begin; base < end; base += span, turn ^= 1) {
         const i64 s = base + wave * CHUNK;
-        float u[CHUNK], in[CHUNK], A = 1.0f, S = 0.0f, most = 0.0f, h;
+        float u[CHUNK], k[CHUNK], in[CHUNK], A = 1.0f, S = 0.0f, most = 0.0f, h;
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i) {
-            const float g = float(next_g[i]);
-            float k, c = float(next_v[i]);
-            most = farthest(most, g);
-            gates(g, u[i], k);
-            if (TANH) c = hyperbolic_tangent(c);
-            in[i] = k * c;
+            most = farthest(most, float(next_g[i]));
+            gates(float(next_g[i]), u[i], k[i]);
+            in[i] = float(next_v[i]);
+            if (TANH) in[i] = hyperbolic_tangent(in[i]);
         }
-        // What is seldom needed, behind one branch. Rows of far gates are read again: held until here they would
-        // take a quarter more registers.
-        const bool far = any_far(most);
-        if (far || s + CHUNK > p.length) {
-            if (far)
-                each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
-                    const float g = float(get<T>(row, p.lane_bytes));
-                    float u_far, k, c = float(get<T>(row, second));
-                    far_gates(g, u_far, k);
-                    if (TANH) c = hyperbolic_tangent(c);
-                    u[i] = fabsf(g) > FAR_GATE ? u_far : u[i];
-                    in[i] = fabsf(g) > FAR_GATE ? k * c : in[i];
-                });
+        if (any_far(most))
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i) far_gates(float(next_g[i]), u[i], k[i]);
+#pragma unroll
+        for (int i = 0; i < CHUNK; ++i) in[i] *= k[i];
+        if (__builtin_expect(s + CHUNK > p.length, 0))
 #pragma unroll
             for (int i = 0; i < CHUNK; ++i)
                 if (s + i >= p.length) u[i] = 1.0f, in[i] = 0.0f;
-        }
 #pragma unroll
         for (int i = 0; i < CHUNK; ++i) {
             A *= u[i];
@@ -330,7 +320,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence(const RecurrenceArgs 
     if (wave == 0 && p.inside && p.segment == a.segments - 1) a.last[p.at(a)] = carry[0];
 }
 
-// As above: 8 x 4096 x 2048 BF16 in 160 us (671 MB, 4.2 TB/s), with sixteen waves of eight steps 175. Two
+// As above: 8 x 4096 x 2048 BF16 in 155 us (671 MB, 4.3 TB/s), with sixteen waves of eight steps 175. Two
 // channels a lane need more registers than there are.
 template <typename T, bool TANH, int WAVES, int CHUNK>
 __global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const RecurrenceArgs a) {
@@ -379,20 +369,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const Recurrence
                 if (TANH) c[i] = hyperbolic_tangent(c[i]);
                 g[i] = float(next_dy[i]);
             }
-            const bool far = any_far(most);
-            if (far || s + CHUNK > p.length) {
-                if (far)
-                    each_row<CHUNK>(x, s, p.length, [&](int i, const char *row) {
-                        const float gate = float(get<T>(row, p.lane_bytes));
-                        float u_far, k_far;
-                        far_gates(gate, u_far, k_far);
-                        u[i] = fabsf(gate) > FAR_GATE ? u_far : u[i];
-                        k[i] = fabsf(gate) > FAR_GATE ? k_far : k[i];
-                    });
+            if (any_far(most))
+#pragma unroll
+                for (int i = 0; i < CHUNK; ++i) far_gates(float(next_g[i]), u[i], k[i]);
+            if (__builtin_expect(s + CHUNK > p.length, 0))
 #pragma unroll
                 for (int i = 0; i < CHUNK; ++i)
                     if (s + i >= p.length) u[i] = 1.0f, k[i] = 0.0f, c[i] = 0.0f, g[i] = 0.0f;
-            }
 #pragma unroll
             for (int i = 0; i < CHUNK; ++i) {
                 A *= u[i];
@@ -439,8 +422,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_recurrence_grad(const Recurrence
 }
 
 // A and S of every segment but the last (GRAD: A and Q of every segment but the first), each wave its
-// share of the segment's steps. Bound by its bytes and the vector units: 65536 x 512 BF16 in 33 us (134 MB,
-// 4.1 TB/s); the segments' own pass reads them again (42 us with the states written).
+// share of the segment's steps. Bound by its bytes and the vector units: 65536 x 512 BF16 in 32 us (134 MB,
+// 4.2 TB/s); the segments' own pass reads them again (42 us with the states written).
 template <typename T, int V, bool TANH, bool GRAD>
 __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const RecurrenceArgs a) {
     constexpr int CHUNK = 8;
@@ -475,33 +458,23 @@ __global__ __launch_bounds__(64 * MOST_WAVES) void k_recurrence_parts(const Recu
             S[j] = GRAD ? fmaf(A[j], add, S[j]) : fmaf(u, S[j], add);
             low[j] = __builtin_elementwise_minimum(low[j], u);
         };
-        if (any_far(most)) {
-#pragma unroll 1
-            for (i64 n = s; n < min(s + CHUNK, end); ++n) {
-                const Group<T, V> gates_at = get<Group<T, V>>(x.at(n), p.lane_bytes);
-                const Group<T, V> values = GRAD ? (a.y ? get<Group<T, V>>(dy.at(n), p.lane_bytes) : Group<T, V>{})
-                                                : get<Group<T, V>>(x.at(n), second);
+        const auto steps = [&](auto far) {
+#pragma unroll
+            for (int i = 0; i < CHUNK; ++i)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float gate = float(gates_at.v[j]);
-                    float u, k;
-                    if (fabsf(gate) > FAR_GATE) far_gates(gate, u, k);
-                    else gates(gate, u, k);
-                    step(j, u, added(k, float(values.v[j])));
+                    const bool live = s + i < end;
+                    float gate = float(g[i].v[j]), value = float(v[i].v[j]), u, k;
+                    // What the two forms have in common is not to be taken before the branch: it would be held there.
+                    if (decltype(far)::value) asm("" : "+v"(gate), "+v"(value));
+                    gates(gate, u, k);
+                    if (decltype(far)::value) far_gates(gate, u, k);
+                    const float add = added(k, value);
+                    step(j, live ? u : 1.0f, live ? add : 0.0f);
                 }
-            }
-            continue;
-        }
-#pragma unroll
-        for (int i = 0; i < CHUNK; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const bool live = s + i < end;
-                float u, k;
-                gates(float(g[i].v[j]), u, k);
-                const float add = added(k, float(v[i].v[j]));
-                step(j, live ? u : 1.0f, live ? add : 0.0f);
-            }
+        };
+        if (any_far(most)) steps(std::true_type{});
+        else steps(std::false_type{});
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {

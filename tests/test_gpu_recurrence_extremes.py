@@ -153,3 +153,28 @@ def test_infinite_states_stay(hip_device, kind, reverse, steps):
     after[at] = True
     assert bool((y[after][..., 3] == math.inf).all()) and bool((last[:, 3] == math.inf).all())
     assert bool(y[~after][..., 3].isfinite().all()) and bool(y[..., 2].isfinite().all())
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("steps,batch,width", [(1, 1, 70), (20, 3, 33), (600, 1, 40), (700, 2, 5), (600, 256, 5)])
+@pytest.mark.parametrize("activation", ["tanh", None])
+def test_far_gates_leave_other_channels_alone(hip_device, kind, steps, batch, width, activation):
+    """A closed gate, an open one and a NaN in some channels of a wave: the others' bits are the same."""
+    gen = torch.Generator().manual_seed(steps + width)
+    x = torch.randn(steps, batch, 2 * width, generator=gen).to(TYPES[kind]).to(hip_device)
+    state, dlast = (torch.randn(batch, width, generator=gen).to(hip_device) for _ in range(2))
+    dy = torch.randn(steps, batch, width, generator=gen).to(TYPES[kind]).to(hip_device)
+
+    def call(x):
+        leaf, start = x.detach().requires_grad_(True), state.clone().requires_grad_(True)
+        y, last = memfast.gated_recurrence(leaf, start, activation=activation)
+        dx, dstate = torch.autograd.grad((y, last), (leaf, start), (dy, dlast))
+        return y, last, dx[..., :width], dx[..., width:], dstate
+
+    expected = call(x)
+    x[steps // 2, :, 0], x[steps // 3, :, 1], x[steps - 1, 0, 2] = -200.0, 300.0, math.nan
+    got = call(x)
+    for a, b in zip(got, expected):
+        assert torch.equal(a[..., 3:], b[..., 3:])
+    assert not bool(got[1][:, :2].isnan().any()) and bool(got[1][0, 2].isnan())
+    assert bool(got[4][0, 2].isnan()) and not bool(got[4][1:].isnan().any())
