@@ -366,18 +366,17 @@ template <typename T> __device__ __forceinline__ v16f mfma_wide(v4u a, v4u b, v1
 // memory to registers, where they become operands once for all rows; x comes through LDS, copied by DMA a
 // span ahead.  With the sums' TABLE, sums over a group begin at -8 times the sum of x, so a zero point of 8
 // costs nothing; others (ZEROS) are taken off with one operation more a group and result, the sums read when
-// they are (held from the group's start, with zero points and groups of 32, BF16 takes 359 us for 318 and FP16 442 for
-// 344). A third of the variants spill up to 16 registers, nearly all outside the span's loop (FP32 in tiles of 64 by
-// 128 with groups of 32 reads nine back a span, three others one).  Without it a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for
+// they are (held from the group's start, with zero points and groups of 32, BF16 takes 359 us for 318 and FP16
+// 442 for 344).  Without it a matrix instruction with ones gives the sums.  PER: scalings in a span, 1 for
 // groups of 128 on, 2 for 64, 4 for 32 (2048 x 4096 x 11008 BF16 with groups of 64: four 250 us, two 210; 24 x
-// 11008 x 4096 18 and 16).
+// 11008 x 4096 18 and 16).  A third of the variants spill up to 16 registers, nearly all outside the span's loop
+// (FP32 in tiles of 64 by 128 with groups of 32 reads nine back a span, three others one).
 // 2048 x 4096 x 11008 BF16, groups of 128, in 181 us (1020 TFLOP/s). No one unit bounds it: matrix units are busy
 // 54% of the time and vector issue 59%, and of two waves a SIMD each waits for a busy unit 40% of its time and for a
 // stage 17%. Without conversions, scalings and LDS reads the loop takes 182 too, not the matrix units' 110; tiles
 // of 128 rows, one wave a SIMD, take 265, with the whole span's codes converted first it is the same. Groups of
-// 32, four scalings a span, 245: the vector units. In small
-// tiles a span's copies are waited for (24 x 11008 x 4096 FP16 11 us); four stages of them with the codes among
-// them leave one workgroup a compute unit and take 15.
+// 32, four scalings a span, 245: the vector units. In small tiles a span's copies are waited for (24 x 11008 x
+// 4096 FP16 11 us); four stages of them with the codes among them leave one workgroup a compute unit and take 15.
 constexpr int TILE_WAVES = 4, BAND = 8;
 
 // Waves that a SIMD has to hold: with at most 256 registers each the matrix instructions' results stay where

@@ -33,6 +33,12 @@ class Dropout(nn.Module):
         self.p = _check_probability(p)
         self._captured = {}     # by seed: the capture and its event, until an eager forward (then None)
 
+    def __getstate__(self):     # copies and pickles have captured nothing
+        return {**self.__dict__, "_captured": {}}
+
+    def __setstate__(self, state):
+        super().__setstate__({"_captured": {}, **state})
+
     def _event(self, x, seed):
         if torch._C._current_graph_task_id() != -1:     # within a backward: a checkpointed forward once more
             event = self._captured.get(seed, (0, 0))[1]

@@ -1,6 +1,8 @@
 """Dropout layers in captured graphs: every replay drops other values, its backward those of its forward."""
 
 import copy
+import gc
+import pickle
 
 import pytest
 import torch
@@ -10,6 +12,18 @@ import memfast_amd as memfast
 from memfast_amd.nn import Dropout, GatedRecurrence, gated
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_garbage_within_captures():
+    """Graphed callables and tracebacks hold their graphs in cycles. A graph that the collector destroys waits for
+    the device, which ends the process while another is being captured: they go between tests alone, and
+    none is left to other files' captures."""
+    gc.collect()
+    gc.disable()
+    yield
+    gc.enable()
+    gc.collect()
 
 
 def captured(call):
@@ -225,3 +239,19 @@ def test_graphs_outlive_their_layers(hip_device):
     torch.cuda.synchronize()
     assert all(bool((o == -1).all()) for o in others)
     assert not any(torch.equal(a, b) for n, a in enumerate(seen) for b in seen[:n])
+
+
+def test_copies_and_pickles_have_captured_nothing(hip_device):
+    """The events of a capture are its layer's own; a layer that was pickled without a place for them has one."""
+    x = torch.ones(100, device=hip_device)
+    layer = Dropout(0.5)
+    captured(lambda: layer(x))
+    assert len(layer._captured) == 1
+    older = Dropout(0.5)
+    older.__setstate__({k: v for k, v in layer.__dict__.items() if k != "_captured"})
+    for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer)), older):
+        assert other._captured == {} and other.p == 0.5
+        torch.manual_seed(3)
+        y = other(x)
+        torch.manual_seed(3)
+        assert torch.equal(y, memfast.dropout(x, 0.5, seed=int(torch.randint(1 << 62, ()))))
